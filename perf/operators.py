@@ -219,7 +219,7 @@ def _quantise(x, kind, tile=False):
         code = ((amax.view(torch.int32) + 0x1FFFFF) >> 23) - 8
         scale, inverse = code.to(torch.uint8).view(torch.float8_e8m0fnu), ((254 - code) << 23).view(torch.float32)
     else:
-        scale, inverse = amax / FP8_MAX, FP8_MAX / amax
+        scale, inverse = amax / FP8_MAX, torch.full_like(amax, FP8_MAX) / amax  # a number over a tensor would round twice
     return (x * _spread(inverse, rows, cols, tile)).clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn), scale
 
 
@@ -316,7 +316,7 @@ def _exact_blocks(x, kind, high, tile=False):
         scale = torch.exp2(torch.ceil(torch.log2(top / FP8_MAX)))
         factor = 1 / scale
     else:  # both are 32-bit numbers by definition
-        scale, factor = (top / FP8_MAX).float().double(), (FP8_MAX / top).float().double()
+        scale, factor = (top / FP8_MAX).float().double(), (torch.full_like(top, FP8_MAX) / top).float().double()
     by = scale[:, None, :, None]
     codes = (grid * factor[:, None, :, None]).clamp(-FP8_MAX, FP8_MAX).float().to(torch.float8_e4m3fn)
     back = lambda t: t.reshape(pad.shape)[:rows, :cols]  # noqa: E731
