@@ -12,10 +12,12 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HIP_SOURCES = ["bn.hip", "pool.hip", "scoring.hip", "optim.hip", "igemm.hip",
-               "wgrad.hip", "kcenter.hip", "linear.hip"]
-BINDING = "bindings.cpp"
+               "wgrad.hip", "kcenter.hip", "linear.hip", "rmsnorm.hip", "fp8.hip"]
+BINDINGS = ["bindings.cpp", "head_bindings.cpp"]
+HEADERS = ["al_common.h", "al_fp8.h"]
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))  # .../active_learning_amd
 HIP_DIR = os.path.join(PKG_DIR, "ops", "hip")
@@ -47,27 +49,31 @@ def _run(cmd):
 
 
 def _stale(obj, src):
-    return (not os.path.exists(obj)
-            or os.path.getmtime(obj) < os.path.getmtime(src)
-            or os.path.getmtime(obj) < os.path.getmtime(
-                os.path.join(HIP_DIR, "al_common.h")))
+    """Older than its source, a header, or the flags in this file."""
+    if not os.path.exists(obj):
+        return True
+    inputs = [src, os.path.abspath(__file__)]
+    inputs += [os.path.join(HIP_DIR, h) for h in HEADERS]
+    return os.path.getmtime(obj) < max(os.path.getmtime(p) for p in inputs)
 
 
 def build(verbose=True):
     os.makedirs(BUILD_DIR, exist_ok=True)
     includes, lib_dirs, libs, defines = _torch_flags()
-    common = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC"]
-    objs = []
-    for src in HIP_SOURCES:
-        obj = os.path.join(BUILD_DIR, src.replace(".hip", ".o"))
+    # no packed fp32 arithmetic: some forms of it have given wrong results on
+    # this hardware now and then
+    common = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
+              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    objs, todo = [], []
+    for src in HIP_SOURCES + BINDINGS:
+        obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
         objs.append(obj)
         if _stale(obj, os.path.join(HIP_DIR, src)):
-            _run(["hipcc", *common, "-c", os.path.join(HIP_DIR, src), "-o", obj])
-    bind_obj = os.path.join(BUILD_DIR, "bindings.o")
-    if _stale(bind_obj, os.path.join(HIP_DIR, BINDING)):
-        _run(["hipcc", *common, *defines, *includes, "-c",
-              os.path.join(HIP_DIR, BINDING), "-o", bind_obj])
-    objs.append(bind_obj)
+            extra = [*defines, *includes] if src in BINDINGS else []
+            todo.append(["hipcc", *common, *extra, "-c",
+                         os.path.join(HIP_DIR, src), "-o", obj])
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        list(pool.map(_run, todo))
     import torch
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     _run(["hipcc", "-shared", "-fPIC", *objs, *lib_dirs, *libs,

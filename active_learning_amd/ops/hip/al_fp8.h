@@ -1,0 +1,133 @@
+// e4m3 blocks: what the kernels that write or read 8-bit operands share.
+//
+// A matrix is held as e4m3 values in rows of `pitch` bytes (a multiple of 128,
+// zero behind the last column) with one scale for each 1x128 or 128x128 block.
+// The scale is a power of two (one e8m0 byte) or a 32-bit float; with
+// a = max|v| of the block, at least 2^-110:
+//   e8m0: scale = the smallest 2^e with a <= 448 * 2^e,  code = v * 2^-e
+//   f32:  scale = a / 448,                               code = v * (448 / a)
+// A block that holds an infinity or a NaN gets a NaN scale and NaN codes.
+#pragma once
+
+#include "al_common.h"
+#include <hip/hip_fp16.h>
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
+
+constexpr int kQB = 128;  // values along a row that share a scale
+
+enum ScaleKind { kE8M0 = 0, kF32 = 1 };
+enum { kTypeBF16 = 0, kTypeF16 = 1, kTypeF32 = 2 };
+
+// Eight values at an address that is aligned to one value only: rows of odd
+// length start anywhere. gfx950 takes such 16-byte accesses in hardware.
+template <typename T> struct Vec8;
+template <> struct Vec8<__bf16> { typedef bf16x8v V; };
+template <> struct Vec8<_Float16> { typedef f16x8v V; };
+template <> struct Vec8<float> { typedef f32x8 V; };
+
+template <typename T> AL_DEV f32x8 load8(const T* p) {
+  typename Vec8<T>::V v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return __builtin_convertvector(v, f32x8);
+}
+template <typename T> AL_DEV void store8(T* p, f32x8 f) {
+  typename Vec8<T>::V v = __builtin_convertvector(f, typename Vec8<T>::V);
+  __builtin_memcpy(p, &v, sizeof(v));
+}
+// the first `left` of eight values, zero behind them
+template <typename T> AL_DEV f32x8 load8_upto(const T* p, int left) {
+  if (left >= 8) return load8(p);
+  f32x8 f = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < left) f[i] = (float)p[i];
+  return f;
+}
+template <typename T> AL_DEV void store8_upto(T* p, f32x8 f, int left) {
+  if (left >= 8) { store8(p, f); return; }
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < left) p[i] = (T)f[i];
+}
+
+// max of |v| as bits: an infinity or NaN stays the largest (fmaxf drops NaN)
+AL_DEV unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+AL_DEV unsigned amax8(f32x8 f) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
+  return m;
+}
+
+struct BlockScale {
+  float inv;      // codes are value * inv
+  unsigned code;  // e8m0 byte, or the bits of the 32-bit scale
+};
+
+template <int KIND> AL_DEV BlockScale block_scale(unsigned amax) {
+  BlockScale s;
+  if (amax >= 0x7f800000u) {  // infinity or NaN in the block
+    s.inv = __uint_as_float(0x7fc00000u);
+    s.code = KIND == kE8M0 ? 255u : 0x7fc00000u;
+    return s;
+  }
+  amax = max(amax, 17u << 23);  // 2^-110: scale and its inverse stay normal
+  if (KIND == kE8M0) {
+    // 448 = 1.75 * 2^8: a mantissa above 1.75 carries into the exponent
+    s.code = ((amax + 0x1fffffu) >> 23) - 8;
+    s.inv = __uint_as_float((254 - s.code) << 23);
+  } else {
+    const float a = __uint_as_float(amax);
+    s.inv = 448.f / a;
+    s.code = __float_as_uint(a / 448.f);
+  }
+  return s;
+}
+
+template <int KIND> AL_DEV void store_scale(void* p, long at, unsigned code) {
+  if (KIND == kE8M0) ((unsigned char*)p)[at] = (unsigned char)code;
+  else ((unsigned*)p)[at] = code;
+}
+template <int KIND> AL_DEV float load_scale(const void* p, long at) {
+  if (KIND == kF32) return ((const float*)p)[at];
+  const unsigned c = ((const unsigned char*)p)[at];
+  return __uint_as_float(c == 255u ? 0x7fc00000u : c << 23);
+}
+
+// eight values to eight e4m3 codes, rounded to nearest even
+AL_DEV i32x2 to_fp8(f32x8 f, float inv) {
+  i32x2 r;
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, 0, false);
+  r[0] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, 0, false);
+  r[1] = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
+  return r;
+}
+
+// the first `left` of eight codes, zero behind them (also where the codes are NaN)
+AL_DEV i32x2 keep_upto(i32x2 codes, int left) {
+  if (left >= 8) return codes;
+  if (left <= 0) return i32x2{0, 0};
+  return __builtin_bit_cast(i32x2, __builtin_bit_cast(unsigned long, codes) &
+                                       ((1ul << (left * 8)) - 1));
+}
+
+// maximum over the 16 lanes that hold one block's 128 values, eight each
+AL_DEV unsigned max_over_16(unsigned m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+  return m;
+}
+
+AL_DEV float wave_allsum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}

@@ -85,6 +85,8 @@ void al_linear_bwd(const float* dy, const float* x, const float* w, float* dx,
                    float* dw, float* db, int B, int M, int C, void* stream);
 }
 
+void register_head_ops(py::module_& m);  // head_bindings.cpp
+
 namespace {
 
 void* cur_stream() { return (void*)c10::hip::getCurrentHIPStream().stream(); }
@@ -667,4 +669,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_fwd", &linear_fwd);
   m.def("linear_bwd", &linear_bwd);
   m.def("adam_step", &adam_step);
+  register_head_ops(m);
 }

@@ -1,0 +1,452 @@
+// Torch bindings of the norm, the e4m3 products and the clipped optimizer steps
+// (rmsnorm.hip, fp8.hip, optim.hip). Everything runs on the current stream of
+// the tensors' own device; scratch memory is torch's, taken for each call, so
+// that neither streams nor captured graphs share any.
+
+#include <torch/extension.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <optional>
+#include <vector>
+
+using torch::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+extern "C" {
+void al_rms_fwd(int type, int wtype, const void* x, long x_stride, const void* res,
+                long res_stride, const void* w, void* y, void* total, float* rstd, void* q,
+                void* scale, int out, long rows, int dim, int pitch, int scale_stride, float eps,
+                void* stream);
+int al_rms_bwd_parts(long rows, int dim);
+void al_rms_bwd(int type, int wtype, const void* s, long s_stride, const void* dy,
+                const void* dsum, const void* w, const float* rstd, void* dx, float* part,
+                void* dw, int parts, long rows, int dim, void* stream);
+void al_col_sum(const float* part, void* out, int type, int parts, int dim, void* stream);
+void al_quant_rows(int type, int kind, const void* x, long row_stride, long col_stride, void* q,
+                   void* scale, long rows, int dim, int pitch, int scale_stride, void* stream);
+void al_quant_tile(int type, int kind, int tile, const void* x, long row_stride, int rows,
+                   int cols, void* q, void* scale, int pitch, int scale_stride, void* qt,
+                   void* scale_t, int pitch_t, int scale_t_stride, float* part, void* stream);
+int al_fp8_gemm_splits(int m, int n, int blocks);
+void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, int sa_stride, const void* b,
+                 const void* sb, long ldb, int sb_stride, int b_tile, int m, int n, int blocks,
+                 const void* bias, int bias_type, void* out, int out_type, float* split_out,
+                 int splits, void* stream);
+void al_fp8_few_rows(int kind, int type, const void* x, long x_stride, int dim, const void* b,
+                     const void* sb, long ldb, int sb_stride, int b_tile, int m, int n, int blocks,
+                     const void* bias, int bias_type, void* out, void* stream);
+int al_norm_batch_bytes();
+void al_norm_batch_clear(void* batch);
+int al_norm_batch_add(void* batch, void* p, long n);
+int al_norm_blocks(const void* batch);
+void al_sq_sum(int type, const void* batch, double* part, void* stream);
+void al_norm_factor(const double* part, int parts, float max_norm, const float* max_dev,
+                    float* out, void* stream);
+void al_scale_by_factor(int type, const void* batch, const float* norm_factor, void* stream);
+void al_sgd_step_multi_clip(const void* table, int nchunks, float lr, float momentum, float wd,
+                            const float* hyper, const float* norm_factor, int zero_grad,
+                            void* stream);
+void al_sgd_step_clip(float* p, const float* g, float* buf, float lr, float momentum, float wd,
+                      const float* hyper, long n, void* shadow, const float* norm_factor,
+                      void* stream);
+void al_adam_step_clip(float* p, const float* g, float* m, float* v, float lr, float b1, float b2,
+                       float eps, float wd, float bc1, float bc2, long n,
+                       const float* norm_factor, void* stream);
+}
+
+namespace {
+
+constexpr long kBlock = 128;  // values that share a scale
+
+void* cur_stream() { return (void*)c10::hip::getCurrentHIPStream().stream(); }
+
+void check_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  TORCH_CHECK(e == hipSuccess, what, ": ", hipGetErrorString(e));
+}
+
+int type_of(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kBFloat16: return 0;
+    case torch::kFloat16: return 1;
+    case torch::kFloat32: return 2;
+    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+  }
+}
+
+// a matrix with its last axis dense, on x's device
+void check_rows(const Tensor& t, const char* name, const Tensor& x) {
+  TORCH_CHECK(t.is_cuda() && t.device() == x.device(), name, " must be on ", x.device());
+  TORCH_CHECK(t.dim() == 2, name, " must have two axes");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name, " must be dense along its last axis");
+  TORCH_CHECK(t.size(1) <= INT_MAX - kBlock, name, " has too long rows");
+}
+
+long row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+long blocks_of(long n) { return (n + kBlock - 1) / kBlock; }
+
+// storage of e4m3 codes: rows of whole blocks
+Tensor new_codes(const Tensor& like, long rows, long cols) {
+  return torch::empty({rows, blocks_of(cols) * kBlock}, like.options().dtype(torch::kFloat8_e4m3fn));
+}
+// storage of scales: e8m0 rows are whole 4-byte words, since kernels read them so
+Tensor new_scales(const Tensor& like, long rows, long cols, long kind) {
+  const long n = blocks_of(cols);
+  return kind == 0 ? torch::empty({rows, (n + 3) / 4 * 4}, like.options().dtype(torch::kFloat8_e8m0fnu))
+                   : torch::empty({rows, n}, like.options().dtype(torch::kFloat32));
+}
+
+const Tensor& value(const OptTensor& t) { return *t; }
+
+void check_norm(const Tensor& x, const Tensor& w, const OptTensor& res) {
+  check_rows(x, "input", x);
+  TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous(),
+              "weight must be a dense vector of the last axis' length on the input's device");
+  TORCH_CHECK(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(),
+              "weight must be float32 or of the input's type");
+  if (res) {
+    check_rows(value(res), "residual", x);
+    TORCH_CHECK(value(res).sizes() == x.sizes() && value(res).scalar_type() == x.scalar_type(),
+                "residual must have the input's shape and type");
+  }
+}
+
+// (y, stored sum or x, 1 / root)
+std::vector<Tensor> rms_norm_fwd(const Tensor& x, const Tensor& w, const OptTensor& res,
+                                 double eps, bool need_rstd) {
+  check_norm(x, w, res);
+  const int type = type_of(x, "input"), wtype = type_of(w, "weight");
+  c10::OptionalDeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
+  Tensor y = torch::empty({rows, dim}, x.options());
+  Tensor total = res ? torch::empty({rows, dim}, x.options()) : x;
+  Tensor rstd = need_rstd ? torch::empty({rows}, x.options().dtype(torch::kFloat32)) : Tensor();
+  if (rows && dim) {
+    al_rms_fwd(type, wtype, x.data_ptr(), row_stride(x), res ? value(res).data_ptr() : nullptr,
+               res ? row_stride(value(res)) : 0, w.data_ptr(), y.data_ptr(),
+               res ? total.data_ptr() : nullptr, need_rstd ? rstd.data_ptr<float>() : nullptr,
+               nullptr, nullptr, 0, rows, (int)dim, 0, 0, (float)eps, cur_stream());
+    check_launch("rms_norm");
+  }
+  return {y, total, need_rstd ? rstd : torch::empty({0}, w.options().dtype(torch::kFloat32))};
+}
+
+// (codes, scales, stored sum)
+std::vector<Tensor> rms_norm_quant(const Tensor& x, const Tensor& w, const OptTensor& res,
+                                   double eps, long kind) {
+  check_norm(x, w, res);
+  const int type = type_of(x, "input"), wtype = type_of(w, "weight");
+  c10::OptionalDeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
+  Tensor q = new_codes(x, rows, dim), scale = new_scales(x, rows, dim, kind);
+  Tensor total = res ? torch::empty({rows, dim}, x.options()) : x;
+  if (rows && dim) {
+    al_rms_fwd(type, wtype, x.data_ptr(), row_stride(x), res ? value(res).data_ptr() : nullptr,
+               res ? row_stride(value(res)) : 0, w.data_ptr(), nullptr,
+               res ? total.data_ptr() : nullptr, nullptr, q.data_ptr(), scale.data_ptr(),
+               kind == 0 ? 1 : 2, rows, (int)dim, (int)q.size(1), (int)scale.size(1), (float)eps,
+               cur_stream());
+    check_launch("rms_norm_fp8");
+  }
+  return {q, scale, total};
+}
+
+// (dx, dw): dw is empty where it is not asked for
+std::vector<Tensor> rms_norm_bwd(const Tensor& s, const Tensor& w, const Tensor& rstd,
+                                 const Tensor& dy_in, const OptTensor& dsum_in, bool need_dw) {
+  check_norm(s, w, std::nullopt);
+  const int type = type_of(s, "input"), wtype = type_of(w, "weight");
+  TORCH_CHECK(dy_in.sizes() == s.sizes() && dy_in.scalar_type() == s.scalar_type() &&
+                  dy_in.device() == s.device(), "gradient must match the output");
+  c10::OptionalDeviceGuard guard(s.device());
+  const Tensor dy = dy_in.contiguous();
+  Tensor dsum;
+  if (dsum_in) {
+    TORCH_CHECK(value(dsum_in).sizes() == s.sizes() && value(dsum_in).scalar_type() == s.scalar_type() &&
+                    value(dsum_in).device() == s.device(), "gradient must match the sum");
+    dsum = value(dsum_in).contiguous();
+  }
+  const long rows = s.size(0), dim = s.size(1);
+  TORCH_CHECK(rstd.numel() == rows && rstd.scalar_type() == torch::kFloat32 && rstd.is_contiguous() &&
+                  rstd.device() == s.device(), "rstd must hold one float a row");
+  Tensor dx = torch::empty({rows, dim}, s.options());
+  Tensor dw = need_dw ? torch::empty({dim}, w.options()) : torch::empty({0}, w.options());
+  if (!rows || !dim) {
+    if (need_dw) dw.zero_();
+    return {dx, dw};
+  }
+  const int parts = al_rms_bwd_parts(rows, (int)dim);
+  Tensor part;
+  if (need_dw) part = torch::empty({parts, dim}, s.options().dtype(torch::kFloat32));
+  al_rms_bwd(type, wtype, s.data_ptr(), row_stride(s), dy.data_ptr(),
+             dsum.defined() ? dsum.data_ptr() : nullptr, w.data_ptr(), rstd.data_ptr<float>(),
+             dx.data_ptr(), need_dw ? part.data_ptr<float>() : nullptr,
+             need_dw ? dw.data_ptr() : nullptr, parts, rows, (int)dim, cur_stream());
+  check_launch("rms_norm backward");
+  return {dx, dw};
+}
+
+// (codes, scales) of 1x128 blocks; any strides
+std::vector<Tensor> fp8_quant_rows(const Tensor& x, long kind) {
+  const int type = type_of(x, "input");
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "input must be a matrix on the GPU");
+  c10::OptionalDeviceGuard guard(x.device());
+  const long rows = x.size(0), dim = x.size(1);
+  TORCH_CHECK(dim <= INT_MAX - kBlock, "input has too long rows");
+  Tensor q = new_codes(x, rows, dim), scale = new_scales(x, rows, dim, kind);
+  if (rows && dim) {
+    al_quant_rows(type, (int)kind, x.data_ptr(), x.stride(0), dim > 1 ? x.stride(1) : 1, q.data_ptr(),
+                  scale.data_ptr(), rows, (int)dim, (int)q.size(1), (int)scale.size(1), cur_stream());
+    check_launch("quantize_fp8");
+  }
+  return {q, scale};
+}
+
+// (codes, scales, transposed codes, transposed scales, column sums), each empty
+// where it is not asked for
+std::vector<Tensor> fp8_quant_tile(const Tensor& x, long kind, bool tile, bool plain, bool transposed,
+                                   std::optional<torch::ScalarType> sums) {
+  const int type = type_of(x, "input");
+  check_rows(x, "input", x);
+  c10::OptionalDeviceGuard guard(x.device());
+  const long rows = x.size(0), cols = x.size(1);
+  TORCH_CHECK(rows <= kBlock * 65535, "input has too many rows");
+  Tensor none = torch::empty({0}, x.options().dtype(torch::kFloat32));
+  Tensor q = none, scale = none, qt = none, scale_t = none, part, sum = none;
+  if (plain) {
+    q = new_codes(x, rows, cols);
+    scale = new_scales(x, tile ? blocks_of(rows) : rows, cols, kind);
+  }
+  if (transposed) {
+    qt = new_codes(x, cols, rows);
+    scale_t = new_scales(x, tile ? blocks_of(cols) : cols, rows, kind);
+  }
+  if (sums) sum = torch::empty({cols}, x.options().dtype(*sums));
+  if (!rows || !cols) {
+    if (sums) sum.zero_();
+    return {q, scale, qt, scale_t, sum};
+  }
+  if (sums) part = torch::empty({blocks_of(rows), cols}, x.options().dtype(torch::kFloat32));
+  al_quant_tile(type, (int)kind, tile, x.data_ptr(), row_stride(x), (int)rows, (int)cols,
+                plain ? q.data_ptr() : nullptr, plain ? scale.data_ptr() : nullptr,
+                plain ? (int)q.size(1) : 0, plain ? (int)scale.size(1) : 0,
+                transposed ? qt.data_ptr() : nullptr, transposed ? scale_t.data_ptr() : nullptr,
+                transposed ? (int)qt.size(1) : 0, transposed ? (int)scale_t.size(1) : 0,
+                sums ? part.data_ptr<float>() : nullptr, cur_stream());
+  if (sums)
+    al_col_sum(part.data_ptr<float>(), sum.data_ptr(), type_of(sum, "sum"), (int)part.size(0),
+               (int)cols, cur_stream());
+  check_launch("quantize_fp8");
+  return {q, scale, qt, scale_t, sum};
+}
+
+int kind_of(const Tensor& scale) { return scale.scalar_type() == torch::kFloat8_e8m0fnu ? 0 : 1; }
+
+void check_codes(const Tensor& q, const Tensor& s, long rows, long cols, bool tile, const char* name) {
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kFloat8_e4m3fn && q.dim() == 2 &&
+                  q.is_contiguous() && q.size(0) == rows && q.size(1) == blocks_of(cols) * kBlock &&
+                  (uintptr_t)q.data_ptr() % 16 == 0, name, " codes are not laid out as blocks");
+  TORCH_CHECK(s.device() == q.device() && s.is_contiguous() && s.dim() == 2 &&
+                  (s.scalar_type() == torch::kFloat32 || s.scalar_type() == torch::kFloat8_e8m0fnu) &&
+                  s.size(0) == (tile ? blocks_of(rows) : rows) && s.size(1) >= blocks_of(cols) &&
+                  (kind_of(s) || s.size(1) % 4 == 0) && (uintptr_t)s.data_ptr() % 4 == 0,
+              name, " scales are not laid out as blocks");
+  TORCH_CHECK(rows <= INT_MAX && cols <= INT_MAX - kBlock, name, " is too large");
+}
+
+void check_bias(const OptTensor& bias, long n, const Tensor& like) {
+  if (!bias) return;
+  type_of(value(bias), "bias");
+  TORCH_CHECK(value(bias).device() == like.device() && value(bias).dim() == 1 && value(bias).size(0) == n &&
+                  value(bias).is_contiguous(),
+              "bias must be a dense vector of one value for each output column, on the operands' device");
+}
+
+Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool b_tile,
+                long m, long n, long k, const OptTensor& bias, torch::ScalarType out_type) {
+  check_codes(a, sa, m, k, false, "left operand's");
+  check_codes(b, sb, n, k, b_tile, "right operand's");
+  TORCH_CHECK(a.device() == b.device(), "operands must be on one device");
+  TORCH_CHECK(kind_of(sa) == kind_of(sb), "operands must have scales of one type");
+  check_bias(bias, n, a);
+  c10::OptionalDeviceGuard guard(a.device());
+  Tensor out = torch::empty({m, n}, a.options().dtype(out_type));
+  const int ot = type_of(out, "output"), blocks = (int)blocks_of(k);
+  if (!m || !n) return out;
+  const int splits = al_fp8_gemm_splits((int)m, (int)n, blocks);
+  Tensor split;
+  if (splits > 1) split = torch::empty({splits, m, n}, a.options().dtype(torch::kFloat32));
+  al_fp8_gemm(kind_of(sa), a.data_ptr(), sa.data_ptr(), a.size(1), (int)sa.size(1), b.data_ptr(),
+              sb.data_ptr(), b.size(1), (int)sb.size(1), b_tile, (int)m, (int)n, blocks,
+              bias ? value(bias).data_ptr() : nullptr, bias ? type_of(value(bias), "bias") : 0,
+              out.data_ptr(), ot, splits > 1 ? split.data_ptr<float>() : nullptr, splits, cur_stream());
+  check_launch("fp8_matmul");
+  return out;
+}
+
+// x [m <= 16, k] in its own type times the blocks of b
+Tensor fp8_few_rows(const Tensor& x, const Tensor& b, const Tensor& sb, bool b_tile, long n,
+                    const OptTensor& bias) {
+  const int type = type_of(x, "input");
+  check_rows(x, "input", b);
+  const long m = x.size(0), k = x.size(1);
+  check_codes(b, sb, n, k, b_tile, "weight's");
+  TORCH_CHECK(m <= 16, "at most 16 rows");
+  check_bias(bias, n, x);
+  c10::OptionalDeviceGuard guard(x.device());
+  Tensor out = torch::empty({m, n}, x.options());
+  if (!m || !n) return out;
+  al_fp8_few_rows(kind_of(sb), type, x.data_ptr(), row_stride(x), (int)k, b.data_ptr(), sb.data_ptr(),
+                  b.size(1), (int)sb.size(1), b_tile, (int)m, (int)n, (int)blocks_of(k),
+                  bias ? value(bias).data_ptr() : nullptr, bias ? type_of(value(bias), "bias") : 0,
+                  out.data_ptr(), cur_stream());
+  check_launch("fp8_linear");
+  return out;
+}
+
+// Batches of tensors of one type for the kernels that take many at once.
+struct Batches {
+  std::vector<std::vector<char>> batch;
+  std::vector<int> type;
+  void add(const Tensor& t) {
+    const int ty = type_of(t, "gradient");
+    if (!t.numel()) return;
+    for (size_t i = 0; i < batch.size(); ++i)
+      if (type[i] == ty && al_norm_batch_add(batch[i].data(), t.data_ptr(), t.numel())) return;
+    batch.emplace_back(al_norm_batch_bytes());
+    type.push_back(ty);
+    al_norm_batch_clear(batch.back().data());
+    al_norm_batch_add(batch.back().data(), t.data_ptr(), t.numel());
+  }
+};
+
+// what the values of a tensor occupy, without gaps and each once, in any order
+bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+
+// [norm, factor] of all tensors; max_dev, where given, holds the bound on the device
+Tensor grad_norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptTensor& max_dev) {
+  TORCH_CHECK(!grads.empty(), "no gradients");
+  const Tensor& first = grads[0];
+  c10::OptionalDeviceGuard guard(first.device());
+  Batches all;
+  std::vector<Tensor> kept;  // copies of what is not dense
+  for (const Tensor& g : grads) {
+    TORCH_CHECK(g.is_cuda() && g.device() == first.device(), "gradients must be on one GPU");
+    TORCH_CHECK(!g.is_sparse(), "sparse gradients have no norm here");
+    if (dense(g)) { all.add(g); continue; }
+    kept.push_back(g.contiguous());
+    all.add(kept.back());
+  }
+  int parts = 0;
+  for (auto& b : all.batch) parts += al_norm_blocks(b.data());
+  Tensor part = torch::empty({std::max(parts, 1)}, first.options().dtype(torch::kFloat64));
+  Tensor out = torch::empty({2}, first.options().dtype(torch::kFloat32));
+  int at = 0;
+  for (size_t i = 0; i < all.batch.size(); ++i) {
+    al_sq_sum(all.type[i], all.batch[i].data(), part.data_ptr<double>() + at, cur_stream());
+    at += al_norm_blocks(all.batch[i].data());
+  }
+  al_norm_factor(part.data_ptr<double>(), parts, (float)max_norm,
+                 max_dev ? value(max_dev).data_ptr<float>() : nullptr, out.data_ptr<float>(), cur_stream());
+  check_launch("grad_norm");
+  return out;
+}
+
+void scale_by_factor(const std::vector<Tensor>& grads, const Tensor& norm_factor) {
+  if (grads.empty()) return;
+  c10::OptionalDeviceGuard guard(norm_factor.device());
+  TORCH_CHECK(norm_factor.is_cuda() && norm_factor.numel() == 2 && norm_factor.scalar_type() == torch::kFloat32 &&
+                  norm_factor.is_contiguous(), "norm and factor");
+  Batches all;
+  std::vector<std::pair<Tensor, Tensor>> copies;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (const Tensor& g : grads) {
+    TORCH_CHECK(g.is_cuda() && g.device() == norm_factor.device(), "gradients must be on one GPU");
+    Tensor at = g;
+    if (!dense(g)) {
+      copies.emplace_back(g, g.contiguous());
+      at = copies.back().second;
+    } else if (g.numel()) {
+      const uintptr_t p = (uintptr_t)g.data_ptr();
+      spans.emplace_back(p, p + g.numel() * g.element_size());
+    }
+    all.add(at);
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i].first >= spans[i - 1].second, "gradients that share memory cannot be scaled in place");
+  for (size_t i = 0; i < all.batch.size(); ++i)
+    al_scale_by_factor(all.type[i], all.batch[i].data(), norm_factor.data_ptr<float>(), cur_stream());
+  check_launch("clip_grad_norm_");
+  for (auto& c : copies) c.first.copy_(c.second);
+}
+
+const float* hyper_of(const OptTensor& h) {
+  if (!h) return nullptr;
+  TORCH_CHECK(value(h).is_cuda() && value(h).numel() >= 3 && value(h).scalar_type() == torch::kFloat32, "hyper");
+  return value(h).data_ptr<float>();
+}
+
+const float* factor_of(const Tensor& f) {
+  TORCH_CHECK(f.is_cuda() && f.numel() == 2 && f.scalar_type() == torch::kFloat32 && f.is_contiguous(),
+              "norm and factor must be two floats on the GPU");
+  return f.data_ptr<float>();
+}
+
+void sgd_step_multi_clip(const Tensor& table, int64_t nchunks, double lr, double momentum, double wd,
+                         const OptTensor& hyper, const Tensor& norm_factor, bool zero_grad) {
+  TORCH_CHECK(table.is_cuda() && table.scalar_type() == torch::kInt64 && table.is_contiguous(), "chunk table");
+  c10::OptionalDeviceGuard guard(table.device());
+  al_sgd_step_multi_clip(table.data_ptr<int64_t>(), (int)nchunks, (float)lr, (float)momentum, (float)wd,
+                         hyper_of(hyper), factor_of(norm_factor), zero_grad, cur_stream());
+  check_launch("SGD step");
+}
+
+void check_update(const Tensor& p, const Tensor& g, const char* what) {
+  TORCH_CHECK(p.is_cuda() && p.scalar_type() == torch::kFloat32 && p.is_contiguous() &&
+                  g.scalar_type() == torch::kFloat32 && g.is_contiguous() && g.numel() == p.numel() &&
+                  g.device() == p.device(), what, ": float32 parameters and gradients, dense");
+}
+
+void sgd_step_clip(Tensor& p, const Tensor& g, Tensor& buf, double lr, double momentum, double wd,
+                   const OptTensor& hyper, Tensor& shadow, const Tensor& norm_factor) {
+  check_update(p, g, "SGD step");
+  if (!p.numel()) return;
+  c10::OptionalDeviceGuard guard(p.device());
+  al_sgd_step_clip(p.data_ptr<float>(), g.data_ptr<float>(), buf.numel() ? buf.data_ptr<float>() : nullptr,
+                   (float)lr, buf.numel() ? (float)momentum : 0.f, (float)wd, hyper_of(hyper), p.numel(),
+                   shadow.numel() ? shadow.data_ptr() : nullptr, factor_of(norm_factor), cur_stream());
+  check_launch("SGD step");
+}
+
+void adam_step_clip(Tensor& p, const Tensor& g, Tensor& m, Tensor& v, double lr, double b1, double b2,
+                    double eps, double wd, double bc1, double bc2, const Tensor& norm_factor) {
+  check_update(p, g, "Adam step");
+  if (!p.numel()) return;
+  c10::OptionalDeviceGuard guard(p.device());
+  al_adam_step_clip(p.data_ptr<float>(), g.data_ptr<float>(), m.data_ptr<float>(), v.data_ptr<float>(),
+                    (float)lr, (float)b1, (float)b2, (float)eps, (float)wd, (float)bc1, (float)bc2, p.numel(),
+                    factor_of(norm_factor), cur_stream());
+  check_launch("Adam step");
+}
+
+}  // namespace
+
+void register_head_ops(py::module_& m) {
+  m.def("rms_norm_fwd", &rms_norm_fwd);
+  m.def("rms_norm_quant", &rms_norm_quant);
+  m.def("rms_norm_bwd", &rms_norm_bwd);
+  m.def("fp8_quant_rows", &fp8_quant_rows);
+  m.def("fp8_quant_tile", &fp8_quant_tile);
+  m.def("fp8_gemm", &fp8_gemm);
+  m.def("fp8_few_rows", &fp8_few_rows);
+  m.def("grad_norm_factor", &grad_norm_factor);
+  m.def("scale_by_factor", &scale_by_factor);
+  m.def("sgd_step_multi_clip", &sgd_step_multi_clip);
+  m.def("sgd_step_clip", &sgd_step_clip);
+  m.def("adam_step_clip", &adam_step_clip);
+}

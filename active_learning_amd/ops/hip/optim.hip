@@ -3,7 +3,9 @@
 // (reference reaches torch.optim.SGD, arg_pools/default.py:39-40).
 // Adam for VAAL's VAE/discriminator (vaal_sampler.py:139-140).
 
-#include "al_common.h"
+#include "al_fp8.h"
+
+#include <algorithm>
 
 template <bool SHADOW>
 __global__ void sgd_kernel(float* __restrict__ p, const float* __restrict__ g,
@@ -195,4 +197,230 @@ extern "C" void al_adam_step(float* p, const float* g, float* m, float* v, float
   int blocks = (int)min((n + 255) / 256, (long)2048);
   hipLaunchKernelGGL(adam_kernel, dim3(blocks), dim3(256), 0, stream, p, g, m, v, lr,
                      b1, b2, eps, wd, bc1, bc2, n);
+}
+
+// ---------------------------------------------------------------------------
+// Norm of all gradients together, and the factor that clips them:
+//   norm = sqrt(sum over all tensors of g^2),  factor = min(1, max / (norm + 1e-6))
+// The tensors' addresses travel in the kernel's arguments: no table to copy, and
+// a captured launch keeps its own. Squares are summed in 64 bits, so that neither
+// large nor tiny values leave the range, first by thread, then by block, then
+// over the blocks' partial sums, each in a fixed order. Bound by one read of the
+// gradients.
+
+constexpr int kNormTensors = 160;  // 24 bytes each: the arguments stay under 4 KB
+constexpr int kNormChunk = 16384;  // values a block takes at a time
+
+struct NormTensor {
+  void* p;
+  long n;
+  long first;  // its first chunk among the batch's
+};
+struct NormBatch {
+  NormTensor t[kNormTensors];
+  long chunks;
+  int count;
+};
+
+// the values of chunk c: [p, p + n)
+template <typename T> AL_DEV T* norm_chunk(const NormBatch& b, long c, int& n) {
+  int lo = 0, hi = b.count - 1;  // the last tensor whose first chunk is not after c
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (b.t[mid].first <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  const long off = (c - b.t[lo].first) * kNormChunk, left = b.t[lo].n - off;
+  n = (int)(left < kNormChunk ? left : kNormChunk);
+  return (T*)b.t[lo].p + off;
+}
+
+template <typename T>
+__launch_bounds__(256)
+__global__ void sq_sum_kernel(NormBatch b, double* __restrict__ part) {
+  __shared__ double lds[4];
+  double s = 0;
+  for (long c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    int n;
+    const T* p = norm_chunk<T>(b, c, n);
+    int i = threadIdx.x * 8;
+    for (; i + 8 <= n; i += 256 * 8) {
+      const f32x8 f = load8(p + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += (double)f[j] * (double)f[j];
+    }
+    for (; i < n; ++i) {  // the last, shorter vector: one thread's
+      const double v = (float)p[i];
+      s += v * v;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = lds[0] + lds[1] + lds[2] + lds[3];
+}
+
+// out[0] = norm, out[1] = the clipping factor
+__launch_bounds__(256)
+__global__ void norm_factor_kernel(const double* __restrict__ part, int parts, float max_norm,
+                                   const float* __restrict__ max_dev, float* __restrict__ out) {
+  __shared__ double lds[4];
+  double s = 0;
+  for (int i = threadIdx.x; i < parts; i += 256) s += part[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(lds[0] + lds[1] + lds[2] + lds[3]);
+    const double f = (double)(max_dev ? *max_dev : max_norm) / (norm + 1e-6);
+    out[0] = (float)norm;
+    out[1] = f < 1.0 ? (float)f : f >= 1.0 ? 1.f : __builtin_nanf("");
+  }
+}
+
+// g *= factor in place; nothing is touched where the factor is one
+template <typename T>
+__launch_bounds__(256)
+__global__ void scale_kernel(NormBatch b, const float* __restrict__ norm_factor) {
+  const float f = norm_factor[1];
+  if (f == 1.f) return;
+  for (long c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    int n;
+    T* p = norm_chunk<T>(b, c, n);
+    int i = threadIdx.x * 8;
+    for (; i + 8 <= n; i += 256 * 8) store8(p + i, load8(p + i) * f);
+    for (; i < n; ++i) p[i] = (T)((float)p[i] * f);
+  }
+}
+
+// The multi-tensor SGD step with clipped gradients: the factor is applied as the
+// gradient is read, which costs no pass of its own, and p.grad keeps its values.
+// Four blocks share a table row, so that a small network fills the chip.
+constexpr int kSgdSub = 4;
+template <bool ZG>
+__launch_bounds__(256)
+__global__ void sgd_mt_clip_kernel(const SgdChunk* __restrict__ table, float lr, float momentum,
+                                   float wd, const float* __restrict__ hyper,
+                                   const float* __restrict__ norm_factor) {
+  if (hyper) { lr = hyper[0]; momentum = hyper[1]; wd = hyper[2]; }
+  const float factor = norm_factor[1];
+  const SgdChunk e = table[blockIdx.x / kSgdSub];
+  const int part = (((int)e.n + kSgdSub - 1) / kSgdSub + 7) & ~7;
+  const int begin = part * (int)(blockIdx.x % kSgdSub), end = min(begin + part, (int)e.n);
+  float* p = e.p + e.off;
+  float* g = const_cast<float*>(e.g) + e.off;
+  float* buf = e.buf ? e.buf + e.off : nullptr;
+  bf16* sh = e.shadow ? e.shadow + e.off : nullptr;
+  for (int i = begin + threadIdx.x * 8; i < end; i += 256 * 8) {
+    const int left = end - i;
+    f32x8 w = load8_upto(p + i, left);
+    f32x8 grad = load8_upto(g + i, left) * factor + wd * w;
+    if (ZG) store8_upto(g + i, f32x8{0, 0, 0, 0, 0, 0, 0, 0}, left);
+    if (momentum != 0.f) {
+      grad = load8_upto(buf + i, left) * momentum + grad;
+      store8_upto(buf + i, grad, left);
+    }
+    w -= lr * grad;
+    store8_upto(p + i, w, left);
+    if (sh) store8_upto((__bf16*)sh + i, w, left);
+  }
+}
+
+// The per-tensor updates with a clipping factor (null: none)
+__global__ void sgd_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
+                                float* __restrict__ buf, float lr, float momentum, float wd,
+                                const float* __restrict__ hyper, long n,
+                                bf16* __restrict__ shadow, const float* __restrict__ norm_factor) {
+  if (hyper) { lr = hyper[0]; momentum = hyper[1]; wd = hyper[2]; }
+  const float factor = norm_factor[1];
+  for (long i = grid_stride_begin(); i < n; i += grid_stride_step()) {
+    float grad = g[i] * factor + wd * p[i];
+    if (momentum != 0.f) {
+      grad = buf[i] * momentum + grad;
+      buf[i] = grad;
+    }
+    const float np = p[i] - lr * grad;
+    p[i] = np;
+    if (shadow) shadow[i] = f2bf(np);
+  }
+}
+
+__global__ void adam_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
+                                 float* __restrict__ m, float* __restrict__ v, float lr,
+                                 float b1, float b2, float eps, float wd, float bc1, float bc2,
+                                 long n, const float* __restrict__ norm_factor) {
+  const float factor = norm_factor[1];
+  for (long i = grid_stride_begin(); i < n; i += grid_stride_step()) {
+    const float grad = g[i] * factor + wd * p[i];
+    const float mi = m[i] * b1 + (1.f - b1) * grad;
+    const float vi = v[i] * b2 + (1.f - b2) * grad * grad;
+    m[i] = mi;
+    v[i] = vi;
+    p[i] -= lr * (mi / bc1) / (sqrtf(vi / bc2) + eps);
+  }
+}
+
+// batch: built by norm_batch_add; part: one double a block
+extern "C" int al_norm_batch_bytes() { return (int)sizeof(NormBatch); }
+extern "C" void al_norm_batch_clear(void* batch) {
+  ((NormBatch*)batch)->chunks = 0;
+  ((NormBatch*)batch)->count = 0;
+}
+// false where the batch is full
+extern "C" int al_norm_batch_add(void* batch, void* p, long n) {
+  NormBatch* b = (NormBatch*)batch;
+  if (b->count == kNormTensors) return 0;
+  b->t[b->count++] = NormTensor{p, n, b->chunks};
+  b->chunks += (n + kNormChunk - 1) / kNormChunk;
+  return 1;
+}
+extern "C" int al_norm_blocks(const void* batch) {
+  return (int)std::min(((const NormBatch*)batch)->chunks, 1024l);
+}
+extern "C" void al_sq_sum(int type, const void* batch, double* part, hipStream_t stream) {
+  const NormBatch& b = *(const NormBatch*)batch;
+  const dim3 grid(al_norm_blocks(batch)), block(256);
+  if (type == kTypeF32) hipLaunchKernelGGL(sq_sum_kernel<float>, grid, block, 0, stream, b, part);
+  else if (type == kTypeBF16) hipLaunchKernelGGL(sq_sum_kernel<__bf16>, grid, block, 0, stream, b, part);
+  else hipLaunchKernelGGL(sq_sum_kernel<_Float16>, grid, block, 0, stream, b, part);
+}
+extern "C" void al_norm_factor(const double* part, int parts, float max_norm, const float* max_dev,
+                               float* out, hipStream_t stream) {
+  hipLaunchKernelGGL(norm_factor_kernel, dim3(1), dim3(256), 0, stream, part, parts, max_norm,
+                     max_dev, out);
+}
+extern "C" void al_scale_by_factor(int type, const void* batch, const float* norm_factor,
+                                   hipStream_t stream) {
+  const NormBatch& b = *(const NormBatch*)batch;
+  const dim3 grid(al_norm_blocks(batch)), block(256);
+  if (type == kTypeF32) hipLaunchKernelGGL(scale_kernel<float>, grid, block, 0, stream, b, norm_factor);
+  else if (type == kTypeBF16) hipLaunchKernelGGL(scale_kernel<__bf16>, grid, block, 0, stream, b, norm_factor);
+  else hipLaunchKernelGGL(scale_kernel<_Float16>, grid, block, 0, stream, b, norm_factor);
+}
+extern "C" void al_sgd_step_multi_clip(const void* table, int nchunks, float lr, float momentum,
+                                       float wd, const float* hyper, const float* norm_factor,
+                                       int zero_grad, hipStream_t stream) {
+  const dim3 grid(nchunks * kSgdSub), block(256);
+  if (zero_grad)
+    hipLaunchKernelGGL((sgd_mt_clip_kernel<true>), grid, block, 0, stream, (const SgdChunk*)table,
+                       lr, momentum, wd, hyper, norm_factor);
+  else
+    hipLaunchKernelGGL((sgd_mt_clip_kernel<false>), grid, block, 0, stream, (const SgdChunk*)table,
+                       lr, momentum, wd, hyper, norm_factor);
+}
+extern "C" void al_sgd_step_clip(float* p, const float* g, float* buf, float lr, float momentum,
+                                 float wd, const float* hyper, long n, void* shadow,
+                                 const float* norm_factor, hipStream_t stream) {
+  const int blocks = (int)std::min((n + 255) / 256, 2048l);
+  hipLaunchKernelGGL(sgd_clip_kernel, dim3(blocks), dim3(256), 0, stream, p, g, buf, lr, momentum,
+                     wd, hyper, n, (bf16*)shadow, norm_factor);
+}
+extern "C" void al_adam_step_clip(float* p, const float* g, float* m, float* v, float lr, float b1,
+                                  float b2, float eps, float wd, float bc1, float bc2, long n,
+                                  const float* norm_factor, hipStream_t stream) {
+  const int blocks = (int)std::min((n + 255) / 256, 2048l);
+  hipLaunchKernelGGL(adam_clip_kernel, dim3(blocks), dim3(256), 0, stream, p, g, m, v, lr, b1, b2,
+                     eps, wd, bc1, bc2, n, norm_factor);
 }

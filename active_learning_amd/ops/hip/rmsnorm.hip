@@ -1,0 +1,345 @@
+// Root-mean-square norm over the last axis, with an optional residual's
+// addition in front of it and an optional output in e4m3 blocks.
+//
+//   s = x + r (rounded to their type, stored)      rstd = 1 / sqrt(mean(s^2) + eps)
+//   y = s * rstd * w
+//   ds = rstd * (w dy - u * mean(w dy u)) + ds_out,   u = s * rstd
+//   dw = sum over rows of dy * u
+//
+// The norm is that of the stored, rounded sum: the backward pass reads the same
+// numbers and differentiates what the forward pass computed. All arithmetic is
+// in 32 bits and rounded once, on the store.
+
+#include "al_fp8.h"
+
+namespace {
+
+enum { kOutPlain = 0, kOutE8M0 = 1, kOutF32 = 2 };
+
+// sum over the TPR threads of a row; every thread gets it
+template <int TPR> AL_DEV float row_sum(float v, float* lds) {
+  v = wave_allsum(v);
+  if (TPR == 64) return v;
+  constexpr int W = TPR / 64;
+  __syncthreads();  // the last row's sums have been read
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) s += lds[i];
+  return s;
+}
+
+constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// One row per TPR threads, VPT vectors of eight values each, rows strided over
+// the grid so that the weight stays in registers. VPT == 0: rows of any length,
+// read twice.
+template <typename T, typename W, int TPR, int VPT, bool RES, int OUT>
+__launch_bounds__(block_of(TPR))
+__global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
+                               const T* __restrict__ res, long res_stride,
+                               const W* __restrict__ w, T* __restrict__ y,
+                               T* __restrict__ total, float* __restrict__ rstd_out,
+                               unsigned char* __restrict__ q, void* __restrict__ scale,
+                               long rows, int dim, int pitch, int scale_stride,
+                               float eps) {
+  __shared__ float lds[16];
+  constexpr int RPB = block_of(TPR) / TPR;
+  constexpr int N = VPT ? VPT : 1;
+  const int t = threadIdx.x % TPR;
+  const int sweeps = VPT ? VPT : (max(dim, pitch) + TPR * 8 - 1) / (TPR * 8);
+  f32x8 wv[N];
+  if (VPT) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) wv[i] = load8_upto(w + (i * TPR + t) * 8, dim - (i * TPR + t) * 8);
+  }
+  const long first = (long)blockIdx.x * RPB;
+  for (long r0 = first; r0 < rows; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + threadIdx.x / TPR;
+    if (RPB > 1 && r >= rows) break;  // whole waves; no barrier when RPB > 1
+    f32x8 v[N];
+    float ss = 0.f;
+    auto take = [&](int c) {
+      f32x8 f = load8_upto(x + r * x_stride + c, dim - c);
+      if (RES) {
+        f += load8_upto(res + r * res_stride + c, dim - c);
+        if (c < dim) store8_upto(total + r * dim + c, f, dim - c);
+        f = __builtin_convertvector(__builtin_convertvector(f, typename Vec8<T>::V), f32x8);
+      }
+      return f;
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      for (int k = i; k < sweeps; k += N) {
+        v[i] = take((k * TPR + t) * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+      }
+    }
+    ss = row_sum<TPR>(ss, lds);
+    const float rstd = 1.f / sqrtf(ss / (float)dim + eps);
+    if (rstd_out && t == 0) rstd_out[r] = rstd;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      for (int k = i; k < sweeps; k += N) {
+        const int c = (k * TPR + t) * 8;
+        f32x8 f, ww;
+        if (VPT) { f = v[i]; ww = wv[i]; }
+        else {
+          ww = load8_upto(w + c, dim - c);
+          // the stored sum, where there is one: this thread wrote it
+          f = RES ? load8_upto(total + r * dim + c, dim - c)
+                  : load8_upto(x + r * x_stride + c, dim - c);
+        }
+        f = f * rstd * ww;
+        if (OUT == kOutPlain) {
+          if (c < dim) store8_upto(y + r * dim + c, f, dim - c);
+        } else {
+          constexpr int KIND = OUT == kOutE8M0 ? kE8M0 : kF32;
+          const BlockScale b = block_scale<KIND>(max_over_16(amax8(f)));
+          if (c < pitch) {
+            *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8(f, b.inv), dim - c);
+            if ((t & 15) == 0 && c < dim)
+              store_scale<KIND>(scale, r * scale_stride + c / kQB, b.code);
+          }
+        }
+      }
+    }
+  }
+}
+
+// The same walk over the rows; dw is summed in registers over a block's rows,
+// joined over its waves in order, and written as one partial row for each block.
+template <typename T, typename W, int TPR, int VPT, bool DSUM>
+__launch_bounds__(block_of(TPR))
+__global__ void rms_bwd_kernel(const T* __restrict__ s, long s_stride,
+                               const T* __restrict__ dy, const T* __restrict__ dsum,
+                               const W* __restrict__ w, const float* __restrict__ rstd_in,
+                               T* __restrict__ dx, float* __restrict__ part,
+                               long rows, int dim) {
+  __shared__ float lds[16];
+  extern __shared__ float dw_lds[];
+  constexpr int RPB = block_of(TPR) / TPR;
+  constexpr int N = VPT ? VPT : 1;
+  const int t = threadIdx.x % TPR;
+  const int sweeps = VPT ? VPT : (dim + TPR * 8 - 1) / (TPR * 8);
+  f32x8 wv[N], dw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    dw[i] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (VPT) wv[i] = load8_upto(w + (i * TPR + t) * 8, dim - (i * TPR + t) * 8);
+  }
+  for (long r0 = (long)blockIdx.x * RPB; r0 < rows; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + threadIdx.x / TPR;
+    if (RPB > 1 && r >= rows) break;
+    const float rstd = rstd_in[r];
+    f32x8 u[N], g[N];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      for (int k = i; k < sweeps; k += N) {
+        const int c = (k * TPR + t) * 8;
+        u[i] = load8_upto(s + r * s_stride + c, dim - c) * rstd;
+        g[i] = load8_upto(dy + r * dim + c, dim - c);
+        if (VPT) dw[i] += g[i] * u[i];
+        g[i] *= VPT ? wv[i] : load8_upto(w + c, dim - c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot += g[i][j] * u[i][j];
+      }
+    }
+    dot = row_sum<TPR>(dot, lds) / (float)dim;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      for (int k = i; k < sweeps; k += N) {
+        const int c = (k * TPR + t) * 8;
+        if (!VPT) {
+          u[i] = load8_upto(s + r * s_stride + c, dim - c) * rstd;
+          g[i] = load8_upto(dy + r * dim + c, dim - c) * load8_upto(w + c, dim - c);
+        }
+        f32x8 d = (g[i] - u[i] * dot) * rstd;
+        if (DSUM) d += load8_upto(dsum + r * dim + c, dim - c);
+        if (c < dim) store8_upto(dx + r * dim + c, d, dim - c);
+      }
+    }
+  }
+  if (!VPT || !part) return;
+  if (RPB == 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * TPR + t) * 8;
+      if (c < dim) store8_upto(part + (long)blockIdx.x * dim + c, dw[i], dim - c);
+    }
+  } else {
+    for (int wave = 0; wave < RPB; ++wave) {
+      if ((int)(threadIdx.x / TPR) == wave) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int c = (i * TPR + t) * 8 + j;
+            if (c < dim) {
+              const float v = (wave ? dw_lds[c] : 0.f) + dw[i][j];
+              if (wave == RPB - 1) part[(long)blockIdx.x * dim + c] = v;
+              else dw_lds[c] = v;
+            }
+          }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// dw's partial rows for lengths that do not fit in registers: one column a
+// thread, a strip of rows a block
+template <typename T>
+__global__ void rms_dw_kernel(const T* __restrict__ s, long s_stride,
+                              const T* __restrict__ dy, const float* __restrict__ rstd,
+                              float* __restrict__ part, long rows, int dim) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= dim) return;
+  float sum = 0.f;
+  for (long r = blockIdx.y; r < rows; r += gridDim.y)
+    sum += (float)dy[r * dim + c] * ((float)s[r * s_stride + c] * rstd[r]);
+  part[(long)blockIdx.y * dim + c] = sum;
+}
+
+// out[c] = sum over p of part[p][c]: 64 columns a block, the partial rows over
+// 16 waves, joined in order
+template <typename W>
+__launch_bounds__(1024)
+__global__ void col_sum_kernel(const float* __restrict__ part, W* __restrict__ out,
+                               int parts, int dim) {
+  __shared__ float lds[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < dim)
+    for (int p = wave; p < parts; p += 16) s += part[(long)p * dim + c];
+  lds[wave][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (wave == 0 && c < dim) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+    out[c] = (W)s;
+  }
+}
+
+struct Shape { int tpr, vpt; };
+
+// The narrowest group of threads that holds a row in registers. A wave for each
+// row needs no barrier; beyond 32768 values a row is read twice instead.
+Shape shape_for(int dim) {
+  if (dim <= 512) return {64, 1};
+  if (dim <= 1024) return {64, 2};
+  if (dim <= 2048) return {64, 4};
+  if (dim <= 4096) return {256, 2};
+  if (dim <= 8192) return {256, 4};
+  if (dim <= 16384) return {1024, 2};
+  if (dim <= 32768) return {1024, 4};
+  return {1024, 0};
+}
+
+template <typename F> void with_shape(int dim, F f) {
+  const Shape s = shape_for(dim);
+  if (s.tpr == 64) {
+    if (s.vpt == 1) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (s.vpt == 2) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  } else if (s.tpr == 256) {
+    if (s.vpt == 2) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  } else {
+    if (s.vpt == 2) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+    else if (s.vpt == 4) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
+  }
+}
+
+int rms_blocks(long rows, int dim, long most) {
+  const int tpr = shape_for(dim).tpr, rpb = tpr < 256 ? 256 / tpr : 1;
+  return (int)std::min((rows + rpb - 1) / rpb, most);
+}
+
+template <typename T, typename W>
+void fwd(const void* x, long x_stride, const void* res, long res_stride, const void* w,
+         void* y, void* total, float* rstd, void* q, void* scale, int out, long rows,
+         int dim, int pitch, int scale_stride, float eps, hipStream_t stream) {
+  const int blocks = rms_blocks(rows, dim, 2048);
+  with_shape(dim, [&](auto tpr, auto vpt) {
+    constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(blocks), dim3(block_of(TPR)), 0, stream, (const T*)x,
+                         x_stride, (const T*)res, res_stride, (const W*)w, (T*)y, (T*)total,
+                         rstd, (unsigned char*)q, scale, rows, dim, pitch, scale_stride, eps);
+    };
+    if (out == kOutPlain) res ? go(rms_fwd_kernel<T, W, TPR, VPT, true, kOutPlain>) : go(rms_fwd_kernel<T, W, TPR, VPT, false, kOutPlain>);
+    else if (out == kOutE8M0) res ? go(rms_fwd_kernel<T, W, TPR, VPT, true, kOutE8M0>) : go(rms_fwd_kernel<T, W, TPR, VPT, false, kOutE8M0>);
+    else res ? go(rms_fwd_kernel<T, W, TPR, VPT, true, kOutF32>) : go(rms_fwd_kernel<T, W, TPR, VPT, false, kOutF32>);
+  });
+}
+
+template <typename T, typename W>
+void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const void* w,
+         const float* rstd, void* dx, float* part, void* dw, int parts, long rows, int dim,
+         hipStream_t stream) {
+  with_shape(dim, [&](auto tpr, auto vpt) {
+    constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(parts), dim3(block_of(TPR)), TPR < 256 ? dim * 4 : 0,
+                         stream, (const T*)s, s_stride, (const T*)dy, (const T*)dsum,
+                         (const W*)w, rstd, (T*)dx, part, rows, dim);
+    };
+    dsum ? go(rms_bwd_kernel<T, W, TPR, VPT, true>) : go(rms_bwd_kernel<T, W, TPR, VPT, false>);
+    if (VPT == 0 && part)
+      hipLaunchKernelGGL(rms_dw_kernel<T>, dim3((dim + 255) / 256, parts), dim3(256), 0, stream,
+                         (const T*)s, s_stride, (const T*)dy, rstd, part, rows, dim);
+  });
+  if (dw)
+    hipLaunchKernelGGL(col_sum_kernel<W>, dim3((dim + 63) / 64), dim3(1024), 0, stream, part,
+                       (W*)dw, parts, dim);
+}
+
+template <typename F> void with_types(int type, int wtype, F f) {
+  // the weight has 32 bits, or the input's type
+  if (type == kTypeF32) f((float*)0, (float*)0);
+  else if (type == kTypeBF16) wtype == kTypeF32 ? f((__bf16*)0, (float*)0) : f((__bf16*)0, (__bf16*)0);
+  else wtype == kTypeF32 ? f((_Float16*)0, (float*)0) : f((_Float16*)0, (_Float16*)0);
+}
+
+}  // namespace
+
+extern "C" void al_rms_fwd(int type, int wtype, const void* x, long x_stride,
+                           const void* res, long res_stride, const void* w, void* y,
+                           void* total, float* rstd, void* q, void* scale, int out,
+                           long rows, int dim, int pitch, int scale_stride, float eps,
+                           hipStream_t stream) {
+  with_types(type, wtype, [&](auto* t, auto* wt) {
+    fwd<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(wt)>>(
+        x, x_stride, res, res_stride, w, y, total, rstd, q, scale, out, rows, dim, pitch,
+        scale_stride, eps, stream);
+  });
+}
+
+// how many partial rows of dw the backward pass writes
+extern "C" int al_rms_bwd_parts(long rows, int dim) { return rms_blocks(rows, dim, 512); }
+
+extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,
+                           const void* dy, const void* dsum, const void* w,
+                           const float* rstd, void* dx, float* part, void* dw, int parts,
+                           long rows, int dim, hipStream_t stream) {
+  with_types(type, wtype, [&](auto* t, auto* wt) {
+    bwd<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(wt)>>(
+        s, s_stride, dy, dsum, w, rstd, dx, part, dw, parts, rows, dim, stream);
+  });
+}
+
+extern "C" void al_col_sum(const float* part, void* out, int type, int parts, int dim,
+                           hipStream_t stream) {
+  const dim3 grid((dim + 63) / 64), block(1024);
+  if (type == kTypeF32)
+    hipLaunchKernelGGL(col_sum_kernel<float>, grid, block, 0, stream, part, (float*)out, parts, dim);
+  else if (type == kTypeBF16)
+    hipLaunchKernelGGL(col_sum_kernel<__bf16>, grid, block, 0, stream, part, (__bf16*)out, parts, dim);
+  else
+    hipLaunchKernelGGL(col_sum_kernel<_Float16>, grid, block, 0, stream, part, (_Float16*)out, parts, dim);
+}

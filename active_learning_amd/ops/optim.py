@@ -17,6 +17,7 @@ import torch
 
 from .extension import extension_available, load_extension
 from .functional import bump_tick
+from .grad_clip import _distinct, _norm_factor
 
 
 def _invalidate(p):
@@ -26,11 +27,29 @@ def _invalidate(p):
         p._al_cast = None
 
 
+def _check_max_norm(max_grad_norm):
+    if max_grad_norm is not None and not float(max_grad_norm) >= 0:
+        raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+    return max_grad_norm
+
+
+def _group_grads(optimizer):
+    return _distinct(p.grad for group in optimizer.param_groups for p in group["params"])
+
+
 class FusedSGD(torch.optim.Optimizer):
+    """SGD with momentum and weight decay.
+
+    ``max_grad_norm``: the step uses gradients scaled so that their norm over all
+    parameters is at most this (ops/grad_clip.py). The scaling happens as the
+    update reads them: ``p.grad`` keeps its values, and the norm they had is in
+    ``last_grad_norm``, a 0-d tensor on the device.
+    """
+
     _CHUNK = 32768  # elements per workgroup in the multi-tensor kernel
 
     def __init__(self, params, lr, momentum=0.0, weight_decay=0.0, dampening=0.0,
-                 nesterov=False):
+                 nesterov=False, max_grad_norm=None):
         if nesterov:
             raise ValueError("nesterov not supported")
         if dampening != 0:
@@ -44,6 +63,9 @@ class FusedSGD(torch.optim.Optimizer):
         self._hyper_dev = None   # device (lr, momentum, wd); graph-capture mode
         self._hyper_host = None
         self._persistent = False  # grads kept in stable storage, zeroed in-kernel
+        self.max_grad_norm = _check_max_norm(max_grad_norm)
+        self.last_grad_norm = None
+        self._clip_dev = None    # device max_grad_norm; graph-capture mode
 
     def enable_persistent_grads(self):
         """Persistent-grad mode for hipGraph capture: the caller must NOT call
@@ -68,11 +90,33 @@ class FusedSGD(torch.optim.Optimizer):
         if tuple(self._hyper_host.tolist()) != vals:
             self._hyper_host.copy_(torch.tensor(vals))
             self._hyper_dev.copy_(self._hyper_host, non_blocking=True)
+        if self.max_grad_norm is not None:
+            if self._clip_dev is None:
+                self._clip_dev = torch.full((1,), float(self.max_grad_norm),
+                                            device=self._hyper_dev.device)
+                self._clip_host = self.max_grad_norm
+            elif self._clip_host != self.max_grad_norm:
+                self._clip_dev.fill_(float(self.max_grad_norm))
+                self._clip_host = self.max_grad_norm
+
+    def _clip(self):
+        """(norm, factor) of this step's gradients on their device; None without
+        max_grad_norm or gradients."""
+        if self.max_grad_norm is None:
+            return None
+        grads = _group_grads(self)
+        if not grads:
+            return None
+        both = _norm_factor(grads, float(self.max_grad_norm),
+                            self._clip_dev if grads[0].is_cuda else None)
+        self.last_grad_norm = both[0]
+        return both
 
     @torch.no_grad()
     def step(self, closure=None):
         loss = closure() if closure is not None else None
         ext = load_extension() if extension_available() else None
+        clip = self._clip()
         for gi, group in enumerate(self.param_groups):
             lr = group["lr"]
             momentum = group["momentum"]
@@ -98,9 +142,8 @@ class FusedSGD(torch.optim.Optimizer):
                               and cache[1].numel() == p.numel()
                               and cache[1].dtype == torch.bfloat16
                               else p.new_empty(0, dtype=torch.bfloat16))
-                    ext.sgd_step(p, g.to(torch.float32),
-                                 buf if buf is not None else p.new_empty(0),
-                                 lr, momentum, wd, shadow)
+                    self._sgd_step(ext, p, g.to(torch.float32), buf, lr, momentum, wd,
+                                   shadow, clip)
                     if shadow.numel():
                         # the kernel refreshed the bf16 copy in-pass; derived
                         # caches (bwd-data permute) must be recomputed
@@ -112,6 +155,8 @@ class FusedSGD(torch.optim.Optimizer):
                     bump_tick(p)  # in-kernel update: no _version bump
                 else:
                     gf = g.float()
+                    if clip is not None:
+                        gf = gf * clip[1]
                     if wd != 0:
                         gf = gf.add(p, alpha=wd)
                     if momentum != 0:
@@ -121,10 +166,19 @@ class FusedSGD(torch.optim.Optimizer):
                     if self._persistent:
                         g.zero_()
             if fused:
-                self._multi_tensor_step(ext, gi, fused, lr, momentum, wd)
+                self._multi_tensor_step(ext, gi, fused, lr, momentum, wd, clip)
         return loss
 
-    def _multi_tensor_step(self, ext, gi, params, lr, momentum, wd):
+    def _sgd_step(self, ext, p, g, buf, lr, momentum, wd, shadow, clip):
+        if buf is None:
+            buf = p.new_empty(0)
+        if clip is None:
+            ext.sgd_step(p, g, buf, lr, momentum, wd, shadow)
+        else:
+            ext.sgd_step_clip(p, g.contiguous(), buf, lr, momentum, wd, self._hyper_dev,
+                              shadow, clip)
+
+    def _multi_tensor_step(self, ext, gi, params, lr, momentum, wd, clip):
         """ONE kernel launch for the whole parameter set (the per-tensor path
         cost 161 launches/step on ResNet-50). Packs a chunk table of
         (p, grad, momentum-buf, bf16-shadow, offset, count) int64 rows; the
@@ -155,7 +209,7 @@ class FusedSGD(torch.optim.Optimizer):
                 # hipGraph capture — fall back to per-tensor launches for
                 # this (captured) step. With persistent grads the
                 # fingerprint is stable and this path never triggers.
-                self._per_tensor_fallback(ext, params, lr, momentum, wd)
+                self._per_tensor_fallback(ext, params, lr, momentum, wd, clip)
                 return
             rows = []
             for pp, gp, bp, sp, n in fp:
@@ -169,7 +223,10 @@ class FusedSGD(torch.optim.Optimizer):
             self._mt_keepalive.append((host, dev))
             entry = (fp, dev, len(rows))
             self._mt_cache[gi] = entry
-        if self._hyper_dev is not None:
+        if clip is not None:
+            ext.sgd_step_multi_clip(entry[1], entry[2], lr, momentum, wd,
+                                    self._hyper_dev, clip, self._persistent)
+        elif self._hyper_dev is not None:
             ext.sgd_step_multi_dev(entry[1], entry[2], self._hyper_dev,
                                    self._persistent)
         else:
@@ -224,7 +281,7 @@ class FusedSGD(torch.optim.Optimizer):
             self._wt_cache[gi] = entry
         ext.wt_refresh_multi(entry[1], entry[2])
 
-    def _per_tensor_fallback(self, ext, params, lr, momentum, wd):
+    def _per_tensor_fallback(self, ext, params, lr, momentum, wd, clip):
         for p in params:
             buf = self.state[p].get("momentum_buffer")
             cache = getattr(p, "_al_cast", None)
@@ -232,8 +289,7 @@ class FusedSGD(torch.optim.Optimizer):
                       and cache[1].numel() == p.numel()
                       and cache[1].dtype == torch.bfloat16
                       else p.new_empty(0, dtype=torch.bfloat16))
-            ext.sgd_step(p, p.grad, buf if buf is not None else p.new_empty(0),
-                         lr, momentum, wd, shadow)
+            self._sgd_step(ext, p, p.grad, buf, lr, momentum, wd, shadow, clip)
             if self._persistent:
                 p.grad.zero_()
             if shadow.numel():
@@ -246,14 +302,30 @@ class FusedSGD(torch.optim.Optimizer):
 
 
 class FusedAdam(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0):
+    """Adam; ``max_grad_norm`` and ``last_grad_norm`` as in FusedSGD."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
+                 max_grad_norm=None):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
+        self.max_grad_norm = _check_max_norm(max_grad_norm)
+        self.last_grad_norm = None
+
+    def _clip(self):
+        if self.max_grad_norm is None:
+            return None
+        grads = _group_grads(self)
+        if not grads:
+            return None
+        both = _norm_factor(grads, float(self.max_grad_norm))
+        self.last_grad_norm = both[0]
+        return both
 
     @torch.no_grad()
     def step(self, closure=None):
         loss = closure() if closure is not None else None
         ext = load_extension() if extension_available() else None
+        clip = self._clip()
         for group in self.param_groups:
             lr = group["lr"]
             beta1, beta2 = group["betas"]
@@ -272,12 +344,20 @@ class FusedAdam(torch.optim.Optimizer):
                 bc1 = 1 - beta1 ** t
                 bc2 = 1 - beta2 ** t
                 if p.is_cuda and ext is not None:
-                    ext.adam_step(p, p.grad.to(torch.float32), state["exp_avg"],
-                                  state["exp_avg_sq"], lr, beta1, beta2, eps, wd, bc1, bc2)
+                    if clip is not None:
+                        ext.adam_step_clip(p, p.grad.to(torch.float32).contiguous(),
+                                           state["exp_avg"], state["exp_avg_sq"], lr, beta1,
+                                           beta2, eps, wd, bc1, bc2, clip)
+                    else:
+                        ext.adam_step(p, p.grad.to(torch.float32), state["exp_avg"],
+                                      state["exp_avg_sq"], lr, beta1, beta2, eps, wd,
+                                      bc1, bc2)
                     _invalidate(p)
                     bump_tick(p)  # in-kernel update: no _version bump
                 else:
                     gf = p.grad.float()
+                    if clip is not None:
+                        gf = gf * clip[1]
                     if wd != 0:
                         gf = gf.add(p, alpha=wd)
                     state["exp_avg"].mul_(beta1).add_(gf, alpha=1 - beta1)
