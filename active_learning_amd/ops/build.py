@@ -15,7 +15,8 @@ import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HIP_SOURCES = ["bn.hip", "pool.hip", "scoring.hip", "optim.hip", "igemm.hip",
-               "wgrad.hip", "kcenter.hip", "linear.hip", "rmsnorm.hip", "fp8.hip"]
+               "wgrad.hip", "kcenter.hip", "linear.hip", "rmsnorm.hip", "fp8.hip",
+               "fp8_gemm.hip"]
 BINDINGS = ["bindings.cpp", "head_bindings.cpp"]
 HEADERS = ["al_common.h", "al_fp8.h"]
 

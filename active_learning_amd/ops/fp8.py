@@ -51,7 +51,7 @@ class Fp8Blocks:
 
     ``values`` (rows, cols) are the codes, ``scale`` the factors: (rows, blocks)
     of 1x128 blocks, or with ``tile`` (row blocks, blocks) of 128x128 tiles.
-    Kernels read whole blocks and, of e8m0, whole words, so the storage is padded
+    Kernels read whole blocks and four scales at a time, so the storage is padded
     (zero behind the last column). The constructor copies into that layout what
     does not have it already: build it once and keep it, as a program keeps its
     weights.
@@ -81,14 +81,13 @@ class Fp8Blocks:
                                 device=values.device)
             codes[:, :cols] = values.view(torch.uint8)
             values = codes.view(torch.float8_e4m3fn)
-        if scale.dtype == torch.float32:
-            scale = scale.contiguous()
-        elif (want[1] % 4 or not scale.is_contiguous()
-              or (scale.is_cuda and scale.data_ptr() % 4)):
-            words = torch.zeros(want[0], -(-want[1] // 4) * 4, dtype=torch.uint8,
+        size = scale.element_size()
+        if (want[1] % 4 or not scale.is_contiguous()
+                or (scale.is_cuda and scale.data_ptr() % (4 * size))):
+            fours = torch.zeros(want[0], -(-want[1] // 4) * 4 * size, dtype=torch.uint8,
                                 device=scale.device)
-            words[:, :want[1]] = scale.view(torch.uint8)
-            scale = words.view(torch.float8_e8m0fnu)
+            fours[:, :want[1] * size] = scale.contiguous().view(torch.uint8)
+            scale = fours.view(scale.dtype)
         self._codes, self._scales = values, scale
         self.shape, self.tile = torch.Size((rows, cols)), bool(tile)
 

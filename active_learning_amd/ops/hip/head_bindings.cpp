@@ -93,11 +93,10 @@ long blocks_of(long n) { return (n + kBlock - 1) / kBlock; }
 Tensor new_codes(const Tensor& like, long rows, long cols) {
   return torch::empty({rows, blocks_of(cols) * kBlock}, like.options().dtype(torch::kFloat8_e4m3fn));
 }
-// storage of scales: e8m0 rows are whole 4-byte words, since kernels read them so
+// storage of scales: rows of whole fours, since the products read them four at a time
 Tensor new_scales(const Tensor& like, long rows, long cols, long kind) {
-  const long n = blocks_of(cols);
-  return kind == 0 ? torch::empty({rows, (n + 3) / 4 * 4}, like.options().dtype(torch::kFloat8_e8m0fnu))
-                   : torch::empty({rows, n}, like.options().dtype(torch::kFloat32));
+  return torch::empty({rows, (blocks_of(cols) + 3) / 4 * 4},
+                      like.options().dtype(kind == 0 ? torch::kFloat8_e8m0fnu : torch::kFloat32));
 }
 
 const Tensor& value(const OptTensor& t) { return *t; }
@@ -253,9 +252,10 @@ void check_codes(const Tensor& q, const Tensor& s, long rows, long cols, bool ti
   TORCH_CHECK(s.device() == q.device() && s.is_contiguous() && s.dim() == 2 &&
                   (s.scalar_type() == torch::kFloat32 || s.scalar_type() == torch::kFloat8_e8m0fnu) &&
                   s.size(0) == (tile ? blocks_of(rows) : rows) && s.size(1) >= blocks_of(cols) &&
-                  (kind_of(s) || s.size(1) % 4 == 0) && (uintptr_t)s.data_ptr() % 4 == 0,
+                  s.size(1) % 4 == 0 && (uintptr_t)s.data_ptr() % (kind_of(s) ? 16 : 4) == 0,
               name, " scales are not laid out as blocks");
-  TORCH_CHECK(rows <= INT_MAX && cols <= INT_MAX - kBlock, name, " is too large");
+  // a workgroup addresses its 256 rows with 32 bits
+  TORCH_CHECK(rows <= INT_MAX && cols <= (1 << 23), name, " matrix has too many rows or too long ones");
 }
 
 void check_bias(const OptTensor& bias, long n, const Tensor& like) {
