@@ -214,15 +214,16 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   const int first = (int)((long)words * blockIdx.y / g.splits) * 4;
   const int steps = min((int)((long)words * (blockIdx.y + 1) / g.splits) * 4, g.blocks) - first;
 
-  // a wave's load brings 8 rows of 128 bytes; the chunk that lands at slot s of row
-  // r is s ^ (r & 7), so that fragments are read from different banks
+  // A wave's load brings 8 rows of 128 bytes; the chunk that lands at slot s of row
+  // r is s ^ (r >> 1 & 7). A read of 16 bytes a lane takes 16 lanes at a time, of
+  // rows 0-3, 12-15, 20-23 and 24-27 first: this way they fall on different banks.
   const int rows_a = min(256, g.m - m0), rows_b = min(256, g.n - n0);
   const Rsrc a = rsrc_of(g.a + (long)m0 * g.lda + (long)first * kQB, (long)rows_a * g.lda - (long)first * kQB);
   const Rsrc b = rsrc_of(g.b + (long)n0 * g.ldb + (long)first * kQB, (long)rows_b * g.ldb - (long)first * kQB);
   unsigned off_a[4], off_b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 64 + wid * 8 + (lane >> 3), chunk = (lane & 7) ^ (lane >> 3);
+    const int r = i * 64 + wid * 8 + (lane >> 3), chunk = (lane & 7) ^ (r >> 1 & 7);
     off_a[i] = (unsigned)min(r, rows_a - 1) * (unsigned)g.lda + chunk * 16;
     off_b[i] = (unsigned)min(r, rows_b - 1) * (unsigned)g.ldb + chunk * 16;
   }
@@ -268,7 +269,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   int at[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
-    at[c] = l31 * 128 + (((((c >> 1) * 4) + l5 * 2 + (c & 1)) ^ (lane & 7)) << 4);
+    at[c] = l31 * 128 + (((((c >> 1) * 4) + l5 * 2 + (c & 1)) ^ (l31 >> 1 & 7)) << 4);
   auto fragment = [&](const unsigned char* p, int half) {
     const i32x4 lo = *(const i32x4*)(p + at[2 * half]), hi = *(const i32x4*)(p + at[2 * half + 1]);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
