@@ -31,9 +31,6 @@ _AMAX_FLOOR = 2.0 ** -110
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _KINDS = {"e8m0": 0, "fp32": 1}
 _SCALE_TYPES = {torch.float8_e8m0fnu: "e8m0", torch.float32: "fp32"}
-#: the most rows that are multiplied straight from their values, without a
-#: quantised copy between
-FEW_ROWS = 16
 
 
 def check_scale_kind(scale):
@@ -171,15 +168,8 @@ def _dense_rows(x):
 
 
 def _pair(x, kind, tile, plain, transposed, sums=None):
-    """(blocks, blocks of the transpose, column sums) of ``x`` in one read of it,
-    each None where it is not asked for."""
-    rows, cols = x.shape
-    if x.is_cuda:
-        q, s, qt, st, total = require_extension().fp8_quant_tile(
-            _dense_rows(x), kind, tile, plain, transposed, sums)
-        return (Fp8Blocks._of(q, s, (rows, cols), tile) if plain else None,
-                Fp8Blocks._of(qt, st, (cols, rows), tile) if transposed else None,
-                total if sums is not None else None)
+    """(blocks, blocks of the transpose, column sums) of ``x``, each None where it
+    is not asked for."""
     x = x.float()
     return (_quantize_cpu(x, kind, tile) if plain else None,
             _quantize_cpu(x.t(), kind, tile) if transposed else None,
@@ -196,13 +186,15 @@ def quantize_fp8(x, tile=False, scale="e8m0"):
     x = _matrix(x, "x")
     if not x.is_cuda:
         return _quantize_cpu(x.float(), kind, tile)
-    across = x.stride(1) != 1 and x.stride(0) == 1 and x.shape[0] > 0
-    if across:  # the transpose of a matrix with dense rows
-        return _pair(x.t(), kind, tile, False, True)[1]
-    if tile:
-        return _pair(x, kind, True, True, False)[0]
-    codes, scales = require_extension().fp8_quant_rows(x, kind)
-    return Fp8Blocks._of(codes, scales, x.shape, False)
+    ext = require_extension()
+    if x.stride(1) != 1 and x.stride(0) == 1 and x.shape[0] > 0:
+        # the transpose of a matrix with dense rows
+        _, _, codes, scales, _ = ext.fp8_quant_tile(x.t(), kind, tile, False, True, None)
+    elif tile:
+        codes, scales, _, _, _ = ext.fp8_quant_tile(_dense_rows(x), kind, True, True, False, None)
+    else:
+        codes, scales = ext.fp8_quant_rows(x, kind)
+    return Fp8Blocks._of(codes, scales, x.shape, tile)
 
 
 def _check_product(a_kind, a_cols, a_device, b, bias):
@@ -249,14 +241,7 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     return _product(a, b, bias if bias is None else bias.detach().contiguous(), out_dtype)
 
 
-def _linear_blocks(x, weight, bias):
-    if x.is_cuda and x.shape[0] <= FEW_ROWS:
-        return require_extension().fp8_few_rows(
-            _dense_rows(x), weight._codes, weight._scales, weight.tile, weight.shape[0], bias)
-    return _product(quantize_fp8(x, scale=weight.scale_kind), weight, bias, x.dtype)
-
-
-class _Fp8Linear(Function):
+class _Fp8LinearCPU(Function):
     """y = Q(x) Q(w)^T + b,  dx = Q(dy) Q(w),  dw = Q(dy^T) Q(x^T)^T: each
     operand in blocks along its product's contraction. The weight's tiles are the
     same for both of its products."""
@@ -297,6 +282,11 @@ def fp8_linear(x, weight, bias=None, scale="e8m0"):
     and bias: both of the gradients' products are e4m3 products too.
     """
     kept = isinstance(weight, Fp8Blocks)
+    if x.is_cuda:  # checked, and differentiated, by the extension
+        if kept:
+            return require_extension().fp8_linear_kept(
+                x, weight._codes, weight._scales, weight.tile, *weight.shape, bias)
+        return require_extension().fp8_linear(x, weight, bias, check_scale_kind(scale))
     kind = check_scale_kind(weight.scale_kind if kept else scale)
     if x.dtype not in _TYPES:
         raise TypeError(f"x must be bfloat16, float16 or float32, got {x.dtype}")
@@ -310,7 +300,7 @@ def fp8_linear(x, weight, bias=None, scale="e8m0"):
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("a weight kept in Fp8Blocks has no gradient: pass the weight "
                                "itself to train, or use torch.no_grad()")
-        y = _linear_blocks(flat.detach(), weight, bias)
+        y = _product(quantize_fp8(flat, scale=weight.scale_kind), weight, bias, x.dtype)
     else:
         if weight.dim() != 2 or weight.dtype not in _TYPES:
             raise TypeError("weight must be Fp8Blocks or a bfloat16, float16 or float32 matrix")
@@ -322,7 +312,7 @@ def fp8_linear(x, weight, bias=None, scale="e8m0"):
         if bias is not None and (bias.shape != weight.shape[:1] or bias.dtype not in _TYPES
                                  or bias.device != x.device):
             raise ValueError(f"bias must be a vector of {weight.shape[0]} values on {x.device}")
-        y = _Fp8Linear.apply(flat, weight, bias, kind)
+        y = _Fp8LinearCPU.apply(flat, weight, bias, kind)
     return y.view(*x.shape[:-1], y.shape[1])
 
 

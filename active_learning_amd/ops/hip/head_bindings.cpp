@@ -4,6 +4,7 @@
 // that neither streams nor captured graphs share any.
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -60,7 +61,8 @@ void al_adam_step_clip(float* p, const float* g, float* m, float* v, float lr, f
 
 namespace {
 
-constexpr long kBlock = 128;  // values that share a scale
+constexpr long kBlock = 128;    // values that share a scale
+constexpr long kFewRows = 16;   // the most rows that need no quantised copy
 
 void* cur_stream() { return (void*)c10::hip::getCurrentHIPStream().stream(); }
 
@@ -74,7 +76,7 @@ int type_of(const Tensor& t, const char* name) {
     case torch::kBFloat16: return 0;
     case torch::kFloat16: return 1;
     case torch::kFloat32: return 2;
-    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
+    default: TORCH_CHECK_TYPE(false, name, " must be bfloat16, float16 or float32, got ", t.scalar_type());
   }
 }
 
@@ -101,92 +103,157 @@ Tensor new_scales(const Tensor& like, long rows, long cols, long kind) {
 
 const Tensor& value(const OptTensor& t) { return *t; }
 
-void check_norm(const Tensor& x, const Tensor& w, const OptTensor& res) {
-  check_rows(x, "input", x);
-  TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous(),
-              "weight must be a dense vector of the last axis' length on the input's device");
-  TORCH_CHECK(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(),
-              "weight must be float32 or of the input's type");
+void check_norm(const Tensor& x, const Tensor& w, const OptTensor& res, double eps) {
+  type_of(x, "input");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "the norm needs a last axis of at least one value");
+  TORCH_CHECK_VALUE(x.size(-1) <= INT_MAX - kBlock, "the last axis is too long");
+  TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == x.size(-1), "weight has shape ", w.sizes(), ", not [",
+                    x.size(-1), "]");
+  TORCH_CHECK_TYPE(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(),
+                   "weight must be float32 or ", x.scalar_type(), ", got ", w.scalar_type());
+  TORCH_CHECK_VALUE(w.device() == x.device(), "weight is on ", w.device(), ", the input on ", x.device());
   if (res) {
-    check_rows(value(res), "residual", x);
-    TORCH_CHECK(value(res).sizes() == x.sizes() && value(res).scalar_type() == x.scalar_type(),
-                "residual must have the input's shape and type");
+    TORCH_CHECK_VALUE(value(res).sizes() == x.sizes() && value(res).scalar_type() == x.scalar_type(),
+                      "residual must have the input's shape and type: ", value(res).sizes(), " ",
+                      value(res).scalar_type(), ", not ", x.sizes(), " ", x.scalar_type());
+    TORCH_CHECK_VALUE(value(res).device() == x.device(), "residual is on ", value(res).device(),
+                      ", the input on ", x.device());
   }
+  TORCH_CHECK_VALUE(eps > 0, "eps must be positive, got ", eps);
 }
 
-// (y, stored sum or x, 1 / root)
-std::vector<Tensor> rms_norm_fwd(const Tensor& x, const Tensor& w, const OptTensor& res,
-                                 double eps, bool need_rstd) {
-  check_norm(x, w, res);
-  const int type = type_of(x, "input"), wtype = type_of(w, "weight");
-  c10::OptionalDeviceGuard guard(x.device());
+// (rows, last axis) with a dense last axis; a view wherever there is one
+Tensor as_rows(const Tensor& t) {
+  if (t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1)) return t;
+  const Tensor r = t.reshape({-1, t.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+// Gradients that have none of their own: a second backward pass raises, as
+// once_differentiable does for a function in Python.
+torch::autograd::variable_list once(torch::autograd::variable_list grads,
+                                    const torch::autograd::variable_list& outer, const char* name) {
+  if (!torch::GradMode::is_enabled() ||
+      !std::any_of(outer.begin(), outer.end(), [](const Tensor& t) { return wants_grad(t); }))
+    return grads;
+  torch::autograd::variable_list fake;
+  for (auto& g : grads) fake.push_back(g.defined() ? g.detach().requires_grad_() : g);
+  auto stop = std::make_shared<torch::autograd::DelayedError>(
+      std::string(name) + " is differentiable once: its backward pass has no gradient", (int)fake.size());
+  return (*stop)(std::move(fake));
+}
+
+struct NormOut {
+  Tensor y, total, rstd;
+};
+
+// rows of a checked input; rstd only where it is asked for
+NormOut norm_rows(const Tensor& x, const Tensor& w, const OptTensor& res, double eps, bool need_rstd) {
   const long rows = x.size(0), dim = x.size(1);
-  Tensor y = torch::empty({rows, dim}, x.options());
-  Tensor total = res ? torch::empty({rows, dim}, x.options()) : x;
-  Tensor rstd = need_rstd ? torch::empty({rows}, x.options().dtype(torch::kFloat32)) : Tensor();
-  if (rows && dim) {
-    al_rms_fwd(type, wtype, x.data_ptr(), row_stride(x), res ? value(res).data_ptr() : nullptr,
-               res ? row_stride(value(res)) : 0, w.data_ptr(), y.data_ptr(),
-               res ? total.data_ptr() : nullptr, need_rstd ? rstd.data_ptr<float>() : nullptr,
-               nullptr, nullptr, 0, rows, (int)dim, 0, 0, (float)eps, cur_stream());
+  NormOut o;
+  o.y = torch::empty({rows, dim}, x.options());
+  o.total = res ? torch::empty({rows, dim}, x.options()) : x;
+  if (need_rstd) o.rstd = torch::empty({rows}, x.options().dtype(torch::kFloat32));
+  if (rows) {
+    al_rms_fwd(type_of(x, "input"), type_of(w, "weight"), x.data_ptr(), row_stride(x),
+               res ? value(res).data_ptr() : nullptr, res ? row_stride(value(res)) : 0, w.data_ptr(),
+               o.y.data_ptr(), res ? o.total.data_ptr() : nullptr,
+               need_rstd ? o.rstd.data_ptr<float>() : nullptr, nullptr, nullptr, 0, rows, (int)dim, 0, 0,
+               (float)eps, cur_stream());
     check_launch("rms_norm");
   }
-  return {y, total, need_rstd ? rstd : torch::empty({0}, w.options().dtype(torch::kFloat32))};
+  return o;
 }
 
-// (codes, scales, stored sum)
-std::vector<Tensor> rms_norm_quant(const Tensor& x, const Tensor& w, const OptTensor& res,
-                                   double eps, long kind) {
-  check_norm(x, w, res);
-  const int type = type_of(x, "input"), wtype = type_of(w, "weight");
-  c10::OptionalDeviceGuard guard(x.device());
-  const long rows = x.size(0), dim = x.size(1);
-  Tensor q = new_codes(x, rows, dim), scale = new_scales(x, rows, dim, kind);
-  Tensor total = res ? torch::empty({rows, dim}, x.options()) : x;
-  if (rows && dim) {
-    al_rms_fwd(type, wtype, x.data_ptr(), row_stride(x), res ? value(res).data_ptr() : nullptr,
-               res ? row_stride(value(res)) : 0, w.data_ptr(), nullptr,
-               res ? total.data_ptr() : nullptr, nullptr, q.data_ptr(), scale.data_ptr(),
-               kind == 0 ? 1 : 2, rows, (int)dim, (int)q.size(1), (int)scale.size(1), (float)eps,
-               cur_stream());
-    check_launch("rms_norm_fp8");
-  }
-  return {q, scale, total};
-}
-
-// (dx, dw): dw is empty where it is not asked for
-std::vector<Tensor> rms_norm_bwd(const Tensor& s, const Tensor& w, const Tensor& rstd,
-                                 const Tensor& dy_in, const OptTensor& dsum_in, bool need_dw) {
-  check_norm(s, w, std::nullopt);
-  const int type = type_of(s, "input"), wtype = type_of(w, "weight");
-  TORCH_CHECK(dy_in.sizes() == s.sizes() && dy_in.scalar_type() == s.scalar_type() &&
-                  dy_in.device() == s.device(), "gradient must match the output");
-  c10::OptionalDeviceGuard guard(s.device());
-  const Tensor dy = dy_in.contiguous();
-  Tensor dsum;
-  if (dsum_in) {
-    TORCH_CHECK(value(dsum_in).sizes() == s.sizes() && value(dsum_in).scalar_type() == s.scalar_type() &&
-                    value(dsum_in).device() == s.device(), "gradient must match the sum");
-    dsum = value(dsum_in).contiguous();
-  }
+// (dx, dw): dw is undefined where it is not asked for
+std::pair<Tensor, Tensor> norm_rows_bwd(const Tensor& s, const Tensor& w, const Tensor& rstd,
+                                        const Tensor& dy, const Tensor& dsum, bool need_dw) {
   const long rows = s.size(0), dim = s.size(1);
-  TORCH_CHECK(rstd.numel() == rows && rstd.scalar_type() == torch::kFloat32 && rstd.is_contiguous() &&
-                  rstd.device() == s.device(), "rstd must hold one float a row");
-  Tensor dx = torch::empty({rows, dim}, s.options());
-  Tensor dw = need_dw ? torch::empty({dim}, w.options()) : torch::empty({0}, w.options());
-  if (!rows || !dim) {
-    if (need_dw) dw.zero_();
-    return {dx, dw};
-  }
+  Tensor dx = torch::empty({rows, dim}, s.options()), dw, part;
+  if (need_dw) dw = rows ? torch::empty({dim}, w.options()) : torch::zeros({dim}, w.options());
+  if (!rows) return {dx, dw};
   const int parts = al_rms_bwd_parts(rows, (int)dim);
-  Tensor part;
   if (need_dw) part = torch::empty({parts, dim}, s.options().dtype(torch::kFloat32));
-  al_rms_bwd(type, wtype, s.data_ptr(), row_stride(s), dy.data_ptr(),
+  al_rms_bwd(type_of(s, "input"), type_of(w, "weight"), s.data_ptr(), row_stride(s), dy.data_ptr(),
              dsum.defined() ? dsum.data_ptr() : nullptr, w.data_ptr(), rstd.data_ptr<float>(),
              dx.data_ptr(), need_dw ? part.data_ptr<float>() : nullptr,
              need_dw ? dw.data_ptr() : nullptr, parts, rows, (int)dim, cur_stream());
   check_launch("rms_norm backward");
   return {dx, dw};
+}
+
+struct RmsNorm : public torch::autograd::Function<RmsNorm> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
+                                                const Tensor& w, const OptTensor& res, double eps) {
+    ctx->set_materialize_grads(false);
+    c10::OptionalDeviceGuard guard(x.device());
+    const NormOut o = norm_rows(as_rows(x), w, res ? OptTensor(as_rows(*res)) : res, eps, true);
+    ctx->save_for_backward({o.total, w, o.rstd});
+    ctx->saved_data["residual"] = res.has_value();
+    if (!res) return {o.y.view(x.sizes())};
+    return {o.y.view(x.sizes()), o.total.view(x.sizes())};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &total = saved[0], &w = saved[1], &rstd = saved[2];
+    const bool res = ctx->saved_data["residual"].toBool();
+    const bool need_w = ctx->needs_input_grad(1);
+    Tensor dy = grads[0], dsum = res ? grads[1] : Tensor();
+    c10::OptionalDeviceGuard guard(total.device());
+    Tensor dx, dw;
+    if (!dy.defined()) {  // only the sum was used
+      dx = dsum;
+      if (need_w) dw = torch::zeros_like(w);
+    } else {
+      const auto shape = dy.sizes().vec();
+      dy = dy.reshape(total.sizes()).contiguous();
+      if (dsum.defined()) dsum = dsum.reshape(total.sizes()).contiguous();
+      std::tie(dx, dw) = norm_rows_bwd(total, w, rstd, dy, dsum, need_w);
+      dx = dx.view(shape);
+    }
+    return once({ctx->needs_input_grad(0) ? dx : Tensor(), dw,
+                 res && ctx->needs_input_grad(2) ? dx : Tensor(), Tensor()}, grads, "rms_norm");
+  }
+};
+
+// y, or y and the stored sum where there is a residual
+std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& w_in, const OptTensor& res, double eps) {
+  check_norm(x, w_in, res, eps);
+  const Tensor w = w_in.contiguous();
+  if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || (res && wants_grad(*res))))
+    return RmsNorm::apply(x, w, res, eps);
+  c10::OptionalDeviceGuard guard(x.device());
+  const NormOut o = norm_rows(as_rows(x), w, res ? OptTensor(as_rows(*res)) : res, eps, false);
+  if (!res) return {o.y.view(x.sizes())};
+  return {o.y.view(x.sizes()), o.total.view(x.sizes())};
+}
+
+// (codes, scales, stored sum)
+std::vector<Tensor> rms_norm_quant(const Tensor& x_in, const Tensor& w_in, const OptTensor& res_in,
+                                   double eps, long kind) {
+  check_norm(x_in, w_in, res_in, eps);
+  TORCH_CHECK(!torch::GradMode::is_enabled() ||
+                  !(wants_grad(x_in) || wants_grad(w_in) || (res_in && wants_grad(*res_in))),
+              "rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to train, or torch.no_grad()");
+  c10::OptionalDeviceGuard guard(x_in.device());
+  const Tensor x = as_rows(x_in), w = w_in.contiguous();
+  const OptTensor res = res_in ? OptTensor(as_rows(*res_in)) : res_in;
+  const long rows = x.size(0), dim = x.size(1);
+  Tensor q = new_codes(x, rows, dim), scale = new_scales(x, rows, dim, kind);
+  Tensor total = res ? torch::empty({rows, dim}, x.options()) : x;
+  if (rows) {
+    al_rms_fwd(type_of(x, "input"), type_of(w, "weight"), x.data_ptr(), row_stride(x),
+               res ? value(res).data_ptr() : nullptr, res ? row_stride(value(res)) : 0, w.data_ptr(),
+               nullptr, res ? total.data_ptr() : nullptr, nullptr, q.data_ptr(), scale.data_ptr(),
+               kind == 0 ? 1 : 2, rows, (int)dim, (int)q.size(1), (int)scale.size(1), (float)eps,
+               cur_stream());
+    check_launch("rms_norm_fp8");
+  }
+  return {q, scale, res ? total.view(x_in.sizes()) : total};
 }
 
 // (codes, scales) of 1x128 blocks; any strides
@@ -261,7 +328,7 @@ void check_codes(const Tensor& q, const Tensor& s, long rows, long cols, bool ti
 void check_bias(const OptTensor& bias, long n, const Tensor& like) {
   if (!bias) return;
   type_of(value(bias), "bias");
-  TORCH_CHECK(value(bias).device() == like.device() && value(bias).dim() == 1 && value(bias).size(0) == n &&
+  TORCH_CHECK_VALUE(value(bias).device() == like.device() && value(bias).dim() == 1 && value(bias).size(0) == n &&
                   value(bias).is_contiguous(),
               "bias must be a dense vector of one value for each output column, on the operands' device");
 }
@@ -306,6 +373,100 @@ Tensor fp8_few_rows(const Tensor& x, const Tensor& b, const Tensor& sb, bool b_t
                   out.data_ptr(), cur_stream());
   check_launch("fp8_linear");
   return out;
+}
+
+// y = Q(x) Q(w)^T + b,  dx = Q(dy) Q(w),  dw = Q(dy^T) Q(x^T)^T: each operand in
+// blocks along its product's contraction. The weight's tiles are the same for both
+// of its products.
+struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const OptTensor& bias, long kind, bool need_x, bool need_w) {
+    c10::OptionalDeviceGuard guard(x.device());
+    const Tensor rows = as_rows(x), wr = as_rows(w);
+    const long m = rows.size(0), k = rows.size(1), n = wr.size(0);
+    const auto xq = fp8_quant_tile(rows, kind, false, true, need_w, std::nullopt);
+    const auto wq = fp8_quant_tile(wr, kind, true, true, need_x, std::nullopt);
+    ctx->save_for_backward({xq[2], xq[3], wq[2], wq[3]});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["w"] = (int64_t)w.scalar_type();
+    ctx->saved_data["x"] = (int64_t)x.scalar_type();
+    ctx->saved_data["bias"] = bias ? (int64_t)value(bias).scalar_type() : -1;
+    auto shape = x.sizes().vec();
+    shape.back() = n;
+    return fp8_gemm(xq[0], xq[1], wq[0], wq[1], true, m, n, k, bias, x.scalar_type()).view(shape);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const long k = ctx->saved_data["k"].toInt(), kind = ctx->saved_data["kind"].toInt();
+    const int64_t bias = ctx->saved_data["bias"].toInt();
+    const bool need_b = bias >= 0 && ctx->needs_input_grad(2);
+    c10::OptionalDeviceGuard guard(grads[0].device());
+    const Tensor dy = as_rows(grads[0]);
+    const long m = dy.size(0), n = dy.size(1);
+    const auto dq = fp8_quant_tile(dy, kind, false, need_x, need_w,
+                                   need_b ? std::optional((torch::ScalarType)bias) : std::nullopt);
+    Tensor dx, dw;
+    if (need_x) {
+      auto shape = grads[0].sizes().vec();
+      shape.back() = k;
+      dx = fp8_gemm(dq[0], dq[1], saved[2], saved[3], true, m, k, n, std::nullopt,
+                    (torch::ScalarType)ctx->saved_data["x"].toInt()).view(shape);
+    }
+    if (need_w)
+      dw = fp8_gemm(dq[2], dq[3], saved[0], saved[1], false, n, k, m, std::nullopt,
+                    (torch::ScalarType)ctx->saved_data["w"].toInt());
+    return once({dx, dw, need_b ? dq[4] : Tensor(), Tensor(), Tensor(), Tensor()}, grads, "fp8_linear");
+  }
+};
+
+void check_linear(const Tensor& x, long n, long k, const OptTensor& bias, const Tensor& like) {
+  type_of(x, "x");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x needs a last axis of at least one value");
+  TORCH_CHECK_VALUE(x.size(-1) == k, "the operands' rows are ", x.size(-1), " and ", k, " values long");
+  TORCH_CHECK_VALUE(x.device() == like.device(), "the operands are on ", x.device(), " and ", like.device());
+  check_bias(bias, n, like);
+}
+
+// x times a weight, quantised here
+Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& bias_in, long kind) {
+  type_of(w, "weight");
+  TORCH_CHECK_TYPE(w.dim() == 2, "weight must be a matrix");
+  const OptTensor bias = bias_in ? OptTensor(bias_in->contiguous()) : bias_in;
+  check_linear(x, w.size(0), w.size(1), bias, w);
+  TORCH_CHECK_VALUE(x.is_cuda(), "x must be on the GPU");
+  const bool grad = torch::GradMode::is_enabled();
+  const bool need_x = grad && x.requires_grad(), need_w = grad && w.requires_grad();
+  if (need_x || need_w || (grad && bias && bias->requires_grad()))
+    return Fp8Linear::apply(x, w, bias, kind, need_x, need_w);
+  c10::OptionalDeviceGuard guard(x.device());
+  const Tensor rows = as_rows(x);
+  const auto xq = fp8_quant_rows(rows, kind);
+  const auto wq = fp8_quant_tile(as_rows(w), kind, true, true, false, std::nullopt);
+  auto shape = x.sizes().vec();
+  shape.back() = w.size(0);
+  return fp8_gemm(xq[0], xq[1], wq[0], wq[1], true, rows.size(0), w.size(0), w.size(1), bias,
+                  x.scalar_type()).view(shape);
+}
+
+// x times a weight that is kept in blocks
+Tensor fp8_linear_kept(const Tensor& x, const Tensor& b, const Tensor& sb, bool b_tile, long n, long k,
+                       const OptTensor& bias_in) {
+  const OptTensor bias = bias_in ? OptTensor(bias_in->contiguous()) : bias_in;
+  check_linear(x, n, k, bias, b);
+  TORCH_CHECK(!torch::GradMode::is_enabled() || !(x.requires_grad() || (bias && bias->requires_grad())),
+              "a weight kept in Fp8Blocks has no gradient: pass the weight itself to train, or use "
+              "torch.no_grad()");
+  c10::OptionalDeviceGuard guard(x.device());
+  const Tensor rows = as_rows(x);
+  auto shape = x.sizes().vec();
+  shape.back() = n;
+  if (rows.size(0) <= kFewRows) return fp8_few_rows(rows, b, sb, b_tile, n, bias).view(shape);
+  const auto xq = fp8_quant_rows(rows, kind_of(sb));
+  return fp8_gemm(xq[0], xq[1], b, sb, b_tile, rows.size(0), n, k, bias, x.scalar_type()).view(shape);
 }
 
 // Batches of tensors of one type for the kernels that take many at once.
@@ -437,13 +598,13 @@ void adam_step_clip(Tensor& p, const Tensor& g, Tensor& m, Tensor& v, double lr,
 }  // namespace
 
 void register_head_ops(py::module_& m) {
-  m.def("rms_norm_fwd", &rms_norm_fwd);
+  m.def("rms_norm", &rms_norm);
   m.def("rms_norm_quant", &rms_norm_quant);
-  m.def("rms_norm_bwd", &rms_norm_bwd);
   m.def("fp8_quant_rows", &fp8_quant_rows);
   m.def("fp8_quant_tile", &fp8_quant_tile);
   m.def("fp8_gemm", &fp8_gemm);
-  m.def("fp8_few_rows", &fp8_few_rows);
+  m.def("fp8_linear", &fp8_linear);
+  m.def("fp8_linear_kept", &fp8_linear_kept);
   m.def("grad_norm_factor", &grad_norm_factor);
   m.def("scale_by_factor", &scale_by_factor);
   m.def("sgd_step_multi_clip", &sgd_step_multi_clip);

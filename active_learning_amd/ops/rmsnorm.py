@@ -58,7 +58,7 @@ def _forward_cpu(x, weight, residual, eps):
     return s * rstd * weight.float(), total, rstd[..., 0]
 
 
-class _RMSNorm(Function):
+class _RMSNormCPU(Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.set_materialize_grads(False)
@@ -67,12 +67,8 @@ class _RMSNorm(Function):
         if residual is not None:
             residual = _rows(residual)
         weight = weight.contiguous()
-        if x.is_cuda:
-            y, total, rstd = require_extension().rms_norm_fwd(
-                x, weight, residual, eps, any(ctx.needs_input_grad))
-        else:
-            y, total, rstd = _forward_cpu(x, weight, residual, eps)
-            y = y.to(x.dtype)
+        y, total, rstd = _forward_cpu(x, weight, residual, eps)
+        y = y.to(x.dtype)
         ctx.save_for_backward(total, weight, rstd)
         if residual is None:
             return y.view(shape)
@@ -90,17 +86,13 @@ class _RMSNorm(Function):
         dy = dy.reshape(total.shape)
         if dsum is not None:
             dsum = dsum.reshape(total.shape)
-        if total.is_cuda:
-            dx, dw = require_extension().rms_norm_bwd(total, weight, rstd, dy, dsum, need_w)
-        else:
-            u = total.float() * rstd[:, None]
-            g = dy.float() * weight.float()
-            dx = (g - u * (g * u).mean(-1, keepdim=True)) * rstd[:, None]
-            if dsum is not None:
-                dx = dx + dsum.float()
-            dx = dx.to(total.dtype)
-            dw = (dy.float() * u).sum(0).to(weight.dtype)
-        dx = dx.view(shape)
+        u = total.float() * rstd[:, None]
+        g = dy.float() * weight.float()
+        dx = (g - u * (g * u).mean(-1, keepdim=True)) * rstd[:, None]
+        if dsum is not None:
+            dx = dx + dsum.float()
+        dx = dx.to(total.dtype).view(shape)
+        dw = (dy.float() * u).sum(0).to(weight.dtype)
         return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
 
 
@@ -111,8 +103,11 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     shape and type; ``weight``: (dim,) in float32 or x's type. Returns y, or
     (y, sum) where a residual is given. Differentiable in all three.
     """
+    if x.is_cuda:  # checked, and differentiated, by the extension
+        out = require_extension().rms_norm(x, weight, residual, eps)
+        return out[0] if residual is None else tuple(out)
     _check(x, weight, residual, eps)
-    return _RMSNorm.apply(x, weight, residual, eps)
+    return _RMSNormCPU.apply(x, weight, residual, eps)
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
@@ -123,8 +118,12 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
     rounding to x's type between. For inference: it has no gradient, and inputs
     that ask for one are refused.
     """
-    _check(x, weight, residual, eps)
     kind = check_scale_kind(scale)
+    if x.is_cuda:
+        codes, scales, total = require_extension().rms_norm_quant(x, weight, residual, eps, kind)
+        blocks = Fp8Blocks._of(codes, scales, (codes.shape[0], x.shape[-1]), False)
+        return blocks if residual is None else (blocks, total)
+    _check(x, weight, residual, eps)
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to "
@@ -133,13 +132,8 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
     x = _rows(x)
     if residual is not None:
         residual = _rows(residual)
-    if x.is_cuda:
-        codes, scales, total = require_extension().rms_norm_quant(
-            x, weight.contiguous(), residual, eps, kind)
-        blocks = Fp8Blocks._of(codes, scales, x.shape, False)
-    else:
-        y, total, _ = _forward_cpu(x, weight, residual, eps)
-        blocks = quantize_fp8(y, scale=scale)
+    y, total, _ = _forward_cpu(x, weight, residual, eps)
+    blocks = quantize_fp8(y, scale=scale)
     return blocks if residual is None else (blocks, total.view(shape))
 
 

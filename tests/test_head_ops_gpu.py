@@ -611,3 +611,40 @@ def test_blocks_move_between_devices():
 def test_refuses_two_devices(bad):
     with pytest.raises((ValueError, RuntimeError)):
         bad()
+
+
+@pytest.mark.parametrize("bad,error", [
+    (lambda: rms_norm(randn(2, 4).double(), randn(4)), TypeError),
+    (lambda: rms_norm(randn(2, 4), randn(5)), ValueError),
+    (lambda: rms_norm(randn(2, 4), randn(4).half()), TypeError),
+    (lambda: rms_norm(randn(2, 4), randn(4), residual=randn(1, 4)), ValueError),
+    (lambda: rms_norm(randn(2, 4), randn(4), residual=randn(2, 4).bfloat16()), ValueError),
+    (lambda: rms_norm(randn(2, 0), randn(0)), ValueError),
+    (lambda: rms_norm(randn(2, 4), randn(4), eps=0.0), ValueError),
+    (lambda: rms_norm_fp8(randn(2, 4), randn(4), scale="bf16"), ValueError),
+    (lambda: rms_norm_fp8(randn(2, 4).requires_grad_(), randn(4)), RuntimeError),
+    (lambda: quantize_fp8(randn(4, 4).double()), TypeError),
+    (lambda: fp8_linear(randn(2, 5), randn(3, 4)), ValueError),
+    (lambda: fp8_linear(randn(2, 4), randn(3, 4), randn(4)), ValueError),
+    (lambda: fp8_linear(randn(2, 4).double(), randn(3, 4)), TypeError),
+    (lambda: fp8_linear(randn(2, 5), quantize_fp8(randn(3, 4), tile=True)), ValueError),
+    (lambda: fp8_linear(randn(2, 4).requires_grad_(), quantize_fp8(randn(3, 4), tile=True)), RuntimeError),
+    (lambda: fp8_linear(randn(2, 4), quantize_fp8(randn(3, 4)), randn(3).requires_grad_()), RuntimeError),
+    (lambda: fp8_matmul(quantize_fp8(randn(4, 4)), quantize_fp8(randn(4, 4), scale="fp32")), ValueError),
+])
+def test_refusals(bad, error):
+    with pytest.raises(error):
+        bad()
+
+
+@pytest.mark.parametrize("what", ["norm", "linear"])
+def test_no_second_gradient(what):
+    """A gradient that is asked to be differentiable is given, and refuses to be differentiated."""
+    x, w = randn(4, 8).requires_grad_(), randn(8 if what == "norm" else 3, 8)[0 if what == "norm" else slice(None)]
+    y = rms_norm(x, w) if what == "norm" else fp8_linear(x, w)
+    dy = torch.ones_like(y).requires_grad_()
+    plain = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)[0]
+    dx = torch.autograd.grad(y, x, dy, create_graph=True)[0]
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), dy)
