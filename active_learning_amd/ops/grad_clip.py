@@ -32,13 +32,22 @@ def _distinct(tensors):
     return kept
 
 
-def _norm_factor(grads, max_norm, max_dev=None):
-    """Two floats on the gradients' device: norm, factor."""
-    if grads[0].is_cuda:
-        return require_extension().grad_norm_factor(grads, max_norm, max_dev)
+def _norm_factor(grads, max_norm):
+    """Norm and factor of gradients on the CPU."""
     norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
     factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
     return torch.stack([norm, factor]).float()
+
+
+def _params_norm_factor(params, max_norm, max_dev=None):
+    """Two floats on the device of the parameters' gradients, or None where there
+    are no gradients."""
+    on_gpu = next((p.is_cuda for p in params if p.grad is not None), None)
+    if on_gpu:
+        return require_extension().params_norm_factor(params, max_norm, max_dev)
+    if on_gpu is None:
+        return None
+    return _norm_factor(_distinct(p.grad for p in params), max_norm)
 
 
 def grad_norm(tensors):
@@ -46,34 +55,33 @@ def grad_norm(tensors):
     device. None is skipped; a tensor that is listed twice counts once."""
     if isinstance(tensors, torch.Tensor):
         tensors = [tensors]
-    grads = _distinct(tensors)
-    if not grads:
+    tensors = [t for t in tensors if t is not None]
+    if not tensors:
         return torch.zeros(())
-    return _norm_factor(grads, float("inf"))[0]
+    if tensors[0].is_cuda:
+        return require_extension().grad_norm_factor(tensors, float("inf"), None)[0]
+    return _norm_factor(_distinct(tensors), float("inf"))[0]
 
 
 def clip_grad_norm_(parameters, max_norm):
     """Scales the parameters' gradients in place so that their norm is at most
     ``max_norm``, and returns the norm they had.
 
-    A gradient with a NaN makes all of them NaN; an infinity makes its own tensor
-    NaN where it stands and the others zero. Gradients that share memory are refused.
+    A NaN makes all gradients NaN; an infinity makes the factor zero, so that it
+    becomes NaN itself and everything else zero. Gradients that share memory are
+    refused.
     """
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    seen = {id(p): p for p in parameters}
-    grads = _distinct(p.grad for p in seen.values())
-    if not grads:
+    both = _params_norm_factor(parameters, max_norm)
+    if both is None:
         return torch.zeros(())
-    both = _norm_factor(grads, max_norm)
     with torch.no_grad():
-        if grads[0].is_cuda:
-            require_extension().scale_by_factor(grads, both)
-            torch.autograd.graph.increment_version(grads)
+        if both.is_cuda:
+            require_extension().scale_grads(parameters, both)
         else:
-            for g in grads:
+            for g in _distinct(p.grad for p in parameters):
                 g.mul_(both[1])
     return both[0]

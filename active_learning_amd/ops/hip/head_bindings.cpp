@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <climits>
 #include <optional>
+#include <unordered_set>
 #include <vector>
 
 using torch::Tensor;
@@ -488,16 +489,33 @@ struct Batches {
 // what the values of a tensor occupy, without gaps and each once, in any order
 bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 
-// [norm, factor] of all tensors; max_dev, where given, holds the bound on the device
-Tensor grad_norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptTensor& max_dev) {
-  TORCH_CHECK(!grads.empty(), "no gradients");
+// each tensor once, however often it is listed
+std::vector<Tensor> distinct(const std::vector<Tensor>& tensors) {
+  std::vector<Tensor> kept;
+  std::unordered_set<const void*> seen;
+  seen.reserve(tensors.size() * 2);
+  for (const Tensor& t : tensors)
+    if (t.defined() && seen.insert(t.unsafeGetTensorImpl()).second) kept.push_back(t);
+  return kept;
+}
+
+std::vector<Tensor> grads_of(const std::vector<Tensor>& params) {
+  std::vector<Tensor> grads;
+  grads.reserve(params.size());
+  for (const Tensor& p : params) grads.push_back(p.grad());
+  return distinct(grads);
+}
+
+// [norm, factor] of distinct tensors; max_dev, where given, holds the bound on the device
+Tensor norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptTensor& max_dev) {
   const Tensor& first = grads[0];
   c10::OptionalDeviceGuard guard(first.device());
   Batches all;
   std::vector<Tensor> kept;  // copies of what is not dense
   for (const Tensor& g : grads) {
-    TORCH_CHECK(g.is_cuda() && g.device() == first.device(), "gradients must be on one GPU");
-    TORCH_CHECK(!g.is_sparse(), "sparse gradients have no norm here");
+    TORCH_CHECK_VALUE(g.is_cuda() && g.device() == first.device(), "gradients are on ", first.device(),
+                      " and ", g.device());
+    TORCH_CHECK_TYPE(g.layout() == torch::kStrided, "sparse gradients have no norm here");
     if (dense(g)) { all.add(g); continue; }
     kept.push_back(g.contiguous());
     all.add(kept.back());
@@ -517,14 +535,23 @@ Tensor grad_norm_factor(const std::vector<Tensor>& grads, double max_norm, const
   return out;
 }
 
-void scale_by_factor(const std::vector<Tensor>& grads, const Tensor& norm_factor) {
-  if (grads.empty()) return;
-  c10::OptionalDeviceGuard guard(norm_factor.device());
+Tensor grad_norm_factor(const std::vector<Tensor>& tensors, double max_norm, const OptTensor& max_dev) {
+  return norm_factor(distinct(tensors), max_norm, max_dev);
+}
+
+Tensor params_norm_factor(const std::vector<Tensor>& params, double max_norm, const OptTensor& max_dev) {
+  return norm_factor(grads_of(params), max_norm, max_dev);
+}
+
+// the parameters' gradients times the factor, in place
+void scale_grads(const std::vector<Tensor>& params, const Tensor& norm_factor) {
   TORCH_CHECK(norm_factor.is_cuda() && norm_factor.numel() == 2 && norm_factor.scalar_type() == torch::kFloat32 &&
                   norm_factor.is_contiguous(), "norm and factor");
+  c10::OptionalDeviceGuard guard(norm_factor.device());
   Batches all;
   std::vector<std::pair<Tensor, Tensor>> copies;
   std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  const std::vector<Tensor> grads = grads_of(params);
   for (const Tensor& g : grads) {
     TORCH_CHECK(g.is_cuda() && g.device() == norm_factor.device(), "gradients must be on one GPU");
     Tensor at = g;
@@ -544,6 +571,35 @@ void scale_by_factor(const std::vector<Tensor>& grads, const Tensor& norm_factor
     al_scale_by_factor(all.type[i], all.batch[i].data(), norm_factor.data_ptr<float>(), cur_stream());
   check_launch("clip_grad_norm_");
   for (auto& c : copies) c.first.copy_(c.second);
+  for (const Tensor& g : grads) g.unsafeGetTensorImpl()->bump_version();
+}
+
+// whether the multi-tensor step can take all of these parameters
+bool sgd_fusable(const std::vector<Tensor>& params) {
+  for (const Tensor& p : params) {
+    const Tensor& g = p.grad();
+    if (!p.is_cuda() || p.scalar_type() != torch::kFloat32 || !p.is_contiguous() || !g.defined() ||
+        g.scalar_type() != torch::kFloat32 || !g.is_contiguous() || g.device() != p.device())
+      return false;
+  }
+  return true;
+}
+
+// five words a parameter: the addresses of its values, gradient, momentum and bf16
+// copy (0: none), and its length
+py::bytes sgd_addresses(const std::vector<Tensor>& params, const std::vector<OptTensor>& bufs,
+                        const std::vector<OptTensor>& shadows) {
+  TORCH_CHECK(bufs.size() == params.size() && shadows.size() == params.size(), "one of each a parameter");
+  std::vector<int64_t> words;
+  words.reserve(params.size() * 5);
+  for (size_t i = 0; i < params.size(); ++i) {
+    words.push_back((int64_t)params[i].data_ptr());
+    words.push_back((int64_t)params[i].grad().data_ptr());
+    words.push_back(bufs[i] ? (int64_t)bufs[i]->data_ptr() : 0);
+    words.push_back(shadows[i] ? (int64_t)shadows[i]->data_ptr() : 0);
+    words.push_back(params[i].numel());
+  }
+  return py::bytes((const char*)words.data(), words.size() * 8);
 }
 
 const float* hyper_of(const OptTensor& h) {
@@ -606,7 +662,10 @@ void register_head_ops(py::module_& m) {
   m.def("fp8_linear", &fp8_linear);
   m.def("fp8_linear_kept", &fp8_linear_kept);
   m.def("grad_norm_factor", &grad_norm_factor);
-  m.def("scale_by_factor", &scale_by_factor);
+  m.def("params_norm_factor", &params_norm_factor);
+  m.def("scale_grads", &scale_grads);
+  m.def("sgd_fusable", &sgd_fusable);
+  m.def("sgd_addresses", &sgd_addresses);
   m.def("sgd_step_multi_clip", &sgd_step_multi_clip);
   m.def("sgd_step_clip", &sgd_step_clip);
   m.def("adam_step_clip", &adam_step_clip);

@@ -244,6 +244,16 @@ __global__ void sq_sum_kernel(NormBatch b, double* __restrict__ part) {
     int n;
     const T* p = norm_chunk<T>(b, c, n);
     int i = threadIdx.x * 8;
+    // four vectors in flight: at one the loads' latency is the bound (4.3 TB/s)
+    for (; i + 3 * 256 * 8 + 8 <= n; i += 4 * 256 * 8) {
+      f32x8 f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f[u] = load8(p + i + u * 256 * 8);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += (double)f[u][j] * (double)f[u][j];
+    }
     for (; i + 8 <= n; i += 256 * 8) {
       const f32x8 f = load8(p + i);
 #pragma unroll
@@ -306,9 +316,12 @@ __global__ void sgd_mt_clip_kernel(const SgdChunk* __restrict__ table, float lr,
                                    const float* __restrict__ norm_factor) {
   if (hyper) { lr = hyper[0]; momentum = hyper[1]; wd = hyper[2]; }
   const float factor = norm_factor[1];
-  const SgdChunk e = table[blockIdx.x / kSgdSub];
+  // from the last row to the first: the norm's pass read the last gradients last,
+  // and some of them are still in the cache
+  const int at = gridDim.x - 1 - blockIdx.x;
+  const SgdChunk e = table[at / kSgdSub];
   const int part = (((int)e.n + kSgdSub - 1) / kSgdSub + 7) & ~7;
-  const int begin = part * (int)(blockIdx.x % kSgdSub), end = min(begin + part, (int)e.n);
+  const int begin = part * (at % kSgdSub), end = min(begin + part, (int)e.n);
   float* p = e.p + e.off;
   float* g = const_cast<float*>(e.g) + e.off;
   float* buf = e.buf ? e.buf + e.off : nullptr;
@@ -377,7 +390,7 @@ extern "C" int al_norm_batch_add(void* batch, void* p, long n) {
   return 1;
 }
 extern "C" int al_norm_blocks(const void* batch) {
-  return (int)std::min(((const NormBatch*)batch)->chunks, 1024l);
+  return (int)std::min(((const NormBatch*)batch)->chunks, 2048l);
 }
 extern "C" void al_sq_sum(int type, const void* batch, double* part, hipStream_t stream) {
   const NormBatch& b = *(const NormBatch*)batch;

@@ -12,12 +12,13 @@ unchanged; the trainer maps names through OPTIMIZERS.
 """
 
 import math
+import struct
 
 import torch
 
 from .extension import extension_available, load_extension
 from .functional import bump_tick
-from .grad_clip import _distinct, _norm_factor
+from .grad_clip import _params_norm_factor
 
 
 def _invalidate(p):
@@ -33,8 +34,8 @@ def _check_max_norm(max_grad_norm):
     return max_grad_norm
 
 
-def _group_grads(optimizer):
-    return _distinct(p.grad for group in optimizer.param_groups for p in group["params"])
+def _all_params(optimizer):
+    return [p for group in optimizer.param_groups for p in group["params"]]
 
 
 class FusedSGD(torch.optim.Optimizer):
@@ -104,12 +105,10 @@ class FusedSGD(torch.optim.Optimizer):
         max_grad_norm or gradients."""
         if self.max_grad_norm is None:
             return None
-        grads = _group_grads(self)
-        if not grads:
-            return None
-        both = _norm_factor(grads, float(self.max_grad_norm),
-                            self._clip_dev if grads[0].is_cuda else None)
-        self.last_grad_norm = both[0]
+        both = _params_norm_factor(_all_params(self), float(self.max_grad_norm),
+                                   self._clip_dev)
+        if both is not None:
+            self.last_grad_norm = both[0]
         return both
 
     @torch.no_grad()
@@ -122,9 +121,10 @@ class FusedSGD(torch.optim.Optimizer):
             momentum = group["momentum"]
             wd = group["weight_decay"]
             fused = []
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
+            params = [p for p in group["params"] if p.grad is not None]
+            if ext is not None and params and ext.sgd_fusable(params):
+                fused, params = params, []  # all of them: no look at each in Python
+            for p in params:
                 if (ext is not None and p.is_cuda
                         and p.dtype == torch.float32 and p.is_contiguous()
                         and p.grad.dtype == torch.float32
@@ -185,23 +185,21 @@ class FusedSGD(torch.optim.Optimizer):
         device copy is cached and only refreshed when any pointer moves, so
         steady-state steps (and hipGraph captures) launch with no H2D
         traffic."""
-        fp = []
-        post = []
+        state = self.state
+        if momentum != 0:
+            for p in params:
+                if "momentum_buffer" not in state[p]:
+                    state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+        bufs = [state[p].get("momentum_buffer") for p in params]
+        shadows = []
         for p in params:
-            state = self.state[p]
-            if momentum != 0 and "momentum_buffer" not in state:
-                state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
-            buf = state.get("momentum_buffer")
             cache = getattr(p, "_al_cast", None)
-            shadow = (cache[1] if cache is not None
-                      and cache[1].numel() == p.numel()
-                      and cache[1].dtype == torch.bfloat16 else None)
-            fp.append((p.data_ptr(), p.grad.data_ptr(),
-                       buf.data_ptr() if buf is not None else 0,
-                       shadow.data_ptr() if shadow is not None else 0,
-                       p.numel()))
-            post.append((p, shadow))
-        fp = tuple(fp)
+            shadows.append(cache[1] if cache is not None
+                           and cache[1].numel() == p.numel()
+                           and cache[1].dtype == torch.bfloat16 else None)
+        # five words a parameter: its address, its gradient's, momentum's and
+        # shadow's (0: none), and its length
+        fp = ext.sgd_addresses(params, bufs, shadows)
         entry = self._mt_cache.get(gi)
         if entry is None or entry[0] != fp:
             if torch.cuda.is_current_stream_capturing():
@@ -212,7 +210,7 @@ class FusedSGD(torch.optim.Optimizer):
                 self._per_tensor_fallback(ext, params, lr, momentum, wd, clip)
                 return
             rows = []
-            for pp, gp, bp, sp, n in fp:
+            for pp, gp, bp, sp, n in struct.iter_unpack("5q", fp):
                 off = 0
                 while off < n:
                     rows.append((pp, gp, bp, sp, off, min(self._CHUNK, n - off)))
@@ -233,7 +231,7 @@ class FusedSGD(torch.optim.Optimizer):
             ext.sgd_step_multi(entry[1], entry[2], lr, momentum, wd,
                                self._persistent)
         wt_fp, wt_entries = [], []
-        for p, shadow in post:
+        for p, shadow in zip(params, shadows):
             if shadow is not None:
                 wt = getattr(shadow, "_al_wt", None)
                 if wt is not None:
@@ -314,11 +312,9 @@ class FusedAdam(torch.optim.Optimizer):
     def _clip(self):
         if self.max_grad_norm is None:
             return None
-        grads = _group_grads(self)
-        if not grads:
-            return None
-        both = _norm_factor(grads, float(self.max_grad_norm))
-        self.last_grad_norm = both[0]
+        both = _params_norm_factor(_all_params(self), float(self.max_grad_norm))
+        if both is not None:
+            self.last_grad_norm = both[0]
         return both
 
     @torch.no_grad()
