@@ -62,85 +62,160 @@ template <bool EXACT> AL_DEV f32x4 block_product(i32x8 x, i32x8 y) {
   return d;
 }
 
-// 128x128 outputs a workgroup, four waves of 64x64, one block of 128 a step
-// through 32 KB of LDS. Rows of b are the first operand, so that a lane holds
-// four neighbouring columns of an output row.
-template <bool EXACT, int KIND>
-__launch_bounds__(256)
-__global__ void gemm_kernel(Gemm g) {
-  __shared__ __align__(16) unsigned char lds_a[128 * 128], lds_b[128 * 128];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int l15 = lane & 15, l4 = lane >> 4;
-  const int m0 = blockIdx.x * 128, n0 = blockIdx.y * 128;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+AL_DEV float scale_value(int kind, unsigned code) {
+  return __uint_as_float(kind == kF32 ? code : code == 255u ? 0x7fc00000u : code << 23);
+}
+template <int KIND> AL_DEV unsigned scale_code(const void* p, long at) {
+  return KIND == kF32 ? ((const unsigned*)p)[at] : ((const unsigned char*)p)[at];
+}
 
-  // chunk c of a row lies at c ^ ((row >> 1) & 7): 16 rows' chunks fall on
-  // different banks
-  const int lrow = t >> 3, lchunk = t & 7;
-  const int first = (int)((long)g.blocks * blockIdx.z / g.splits);
-  const int last = (int)((long)g.blocks * (blockIdx.z + 1) / g.splits);
-  for (int kb = first; kb < last; ++kb) {
-    __syncthreads();
+// --------------------------------------------------------------------------
+// few outputs: (16 MT) x (16 NT) a workgroup, straight from memory
+// --------------------------------------------------------------------------
+//
+// Each wave takes every WAVES-th block of the contraction, with fragments read
+// into registers a block ahead, so that no wave waits for another; the waves'
+// sums meet in LDS and are joined in order. With T a float type a's rows come as
+// values, at most 16 of them, and each wave quantises the blocks that it reads:
+// a launch less, and b's bytes are what it costs. With T unsigned char they come
+// as codes.
+template <typename T, bool EXACT, int KIND, bool BTILE, int MT, int NT, int WAVES>
+__launch_bounds__(WAVES * 64)
+__global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g) {
+  constexpr bool VALUES = !std::is_same<T, unsigned char>::value;
+  constexpr bool HW = KIND == kE8M0 && !EXACT;  // the matrix instruction applies the scales
+  static_assert(!VALUES || MT == 1, "values: one tile of rows");
+  __shared__ f32x4 lds[WAVES][MT * NT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l15 = lane & 15, l4 = lane >> 4;
+  const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+
+  // rows behind the last are the last one again; their outputs are not stored
+  const unsigned char *a[MT], *b[NT];
+  long sa[MT], sb[NT];  // where the first block's scales are
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = lrow + i * 32;
-      const long ra = min(m0 + r, g.m - 1), rb = min(n0 + r, g.n - 1);
-      const int at = r * 128 + ((lchunk ^ ((r >> 1) & 7)) << 4);
-      *(i32x4*)(lds_a + at) = *(const i32x4*)(g.a + ra * g.lda + (long)kb * kQB + lchunk * 16);
-      *(i32x4*)(lds_b + at) = *(const i32x4*)(g.b + rb * g.ldb + (long)kb * kQB + lchunk * 16);
-    }
-    __syncthreads();
-    auto fragment = [&](const unsigned char* lds, int r) {
-      const int s = (r >> 1) & 7;
-      const i32x4 lo = *(const i32x4*)(lds + r * 128 + (((2 * l4) ^ s) << 4));
-      const i32x4 hi = *(const i32x4*)(lds + r * 128 + (((2 * l4 + 1) ^ s) << 4));
-      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    };
-    i32x8 fa[4];
-    float sa[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[i] = fragment(lds_a, wm + i * 16 + l15);
-      sa[i] = load_scale<KIND>(g.sa, (long)min(m0 + wm + i * 16 + l15, g.m - 1) * g.sa_stride + kb);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const i32x8 fb = fragment(lds_b, wn + j * 16 + l15);
-      f32x4 sb;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = min(n0 + wn + j * 16 + l4 * 4 + r, g.n - 1);
-        sb[r] = load_scale<KIND>(g.sb, (long)(g.b_tile ? n / kQB : n) * g.sb_stride + kb);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 d = block_product<EXACT>(fb, fa[i]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(d[r], sa[i] * sb[r], acc[i][j][r]);
-      }
-    }
+  for (int i = 0; i < MT; ++i) {
+    const long m = min(m0 + i * 16 + l15, g.m - 1);
+    a[i] = VALUES ? (const unsigned char*)(x + m * x_stride + l4 * 32) : g.a + m * g.lda + l4 * 32;
+    sa[i] = m * g.sa_stride;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + wm + i * 16 + l15;
+  for (int j = 0; j < NT; ++j) {
+    const int n = min(n0 + j * 16 + l15, g.n - 1);
+    b[j] = g.b + (long)n * g.ldb + l4 * 32;
+    sb[j] = (long)(BTILE ? n / kQB : n) * g.sb_stride;
+  }
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  struct Raw {
+    i32x8 a[VALUES ? 1 : MT], b[NT];
+    typename std::conditional<VALUES, T, float>::type v[VALUES ? 32 : 1];
+    unsigned sa[MT], sb[NT];
+  };
+  auto load32 = [](const unsigned char* p) {
+    const i32x4 lo = *(const i32x4*)p, hi = *(const i32x4*)(p + 16);
+    return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto load = [&](Raw& r, int kb) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      r.b[j] = load32(b[j] + (long)kb * kQB);
+      r.sb[j] = scale_code<KIND>(g.sb, sb[j] + kb);
+    }
+    if (VALUES) {
+      const int left = dim - kb * kQB - l4 * 32;  // a block's tail is masked where it is quantised
+      const T* p = (const T*)a[0] + (long)kb * kQB;
+      if ((kb + 1) * kQB <= dim) __builtin_memcpy(&r.v, p, sizeof(T) * 32);
+      else
+        for (int i = 0; i < 32; ++i) r.v[VALUES ? i : 0] = i < left ? p[i] : (T)0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        r.a[VALUES ? 0 : i] = load32(a[i] + (long)kb * kQB);
+        r.sa[i] = scale_code<KIND>(g.sa, sa[i] + kb);
+      }
+    }
+  };
+  auto compute = [&](Raw& r, int kb) {
+    if (VALUES) {
+      f32x8 f[4];
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = (float)r.v[VALUES ? i * 8 + e : 0];
+        top = max(top, amax8(f[i]));
+      }
+      top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+      top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+      const BlockScale s = block_scale<KIND>(top);
+      r.sa[0] = s.code;
+      const int left = dim - kb * kQB - l4 * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const i32x2 codes = keep_upto(to_fp8(f[i], s.inv), left - i * 8);
+        r.a[0][2 * i] = codes[0];
+        r.a[0][2 * i + 1] = codes[1];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      f32x4 by;
+      if (!HW) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          by[e] = scale_value(KIND, BTILE ? r.sb[j]
+                                          : (unsigned)__shfl((int)r.sb[j], l4 * 4 + e, 64));
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const i32x8 fa = r.a[VALUES ? 0 : i];
+        if (HW) {
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.b[j], fa, acc[i][j], 0, 0, 0,
+                                                                      (int)r.sb[j], 0, (int)r.sa[i]);
+        } else {
+          const f32x4 d = block_product<EXACT>(r.b[j], fa);
+          const float s = scale_value(KIND, r.sa[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s * by[e], acc[i][j][e]);
+        }
+      }
+    }
+  };
+  Raw r[2];
+  if (wave < g.blocks) load(r[0], wave);
+  for (int kb = wave; kb < g.blocks; kb += 2 * WAVES) {
+    if (kb + WAVES < g.blocks) load(r[1], kb + WAVES);
+    compute(r[0], kb);
+    if (kb + WAVES >= g.blocks) break;
+    if (kb + 2 * WAVES < g.blocks) load(r[0], kb + 2 * WAVES);
+    compute(r[1], kb + WAVES);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) lds[wave][i * NT + j][lane] = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int f = 0; f < MT * NT; f += WAVES) {
+    if (f + wave >= MT * NT) break;
+    const int i = (f + wave) / NT, j = (f + wave) % NT;
+    f32x4 v = lds[0][f + wave][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += lds[w][f + wave][lane];
+    const int m = m0 + i * 16 + l15;
     if (m >= g.m) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = n0 + wn + j * 16 + l4 * 4 + r;
-        if (n >= g.n) continue;
-        if (g.splits > 1)
-          g.split_out[((long)blockIdx.z * g.m + m) * g.n + n] = acc[i][j][r];
-        else
-          store_out(g.out, g.out_type, (long)m * g.n + n,
-                    acc[i][j][r] + (g.bias ? bias_at(g.bias, g.bias_type, n) : 0.f));
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + j * 16 + l4 * 4 + e;
+      if (n < g.n)
+        store_out(g.out, g.out_type, (long)m * g.n + n,
+                  v[e] + (g.bias ? bias_at(g.bias, g.bias_type, n) : 0.f));
+    }
   }
 }
 
@@ -485,65 +560,6 @@ __global__ void gemm_join_kernel(Gemm g) {
   }
 }
 
-// Up to 16 rows, straight from the values: a workgroup computes 16 columns, its
-// eight waves take every eighth block of the contraction, quantise x's block as
-// they read it, and join through LDS in order. What it costs is b's bytes.
-template <typename T, bool EXACT, int KIND>
-__launch_bounds__(512)
-__global__ void few_rows_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g) {
-  __shared__ f32x4 lds[8][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int l15 = lane & 15, l4 = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const unsigned char* b = g.b + (long)min(n0 + l15, g.n - 1) * g.ldb + l4 * 32;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int kb = wave; kb < g.blocks; kb += 8) {
-    const i32x4 lo = *(const i32x4*)(b + (long)kb * kQB), hi = *(const i32x4*)(b + (long)kb * kQB + 16);
-    const i32x8 fb = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    const int c = kb * kQB + l4 * 32;
-    f32x8 f[4];
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (l15 < g.m) f[i] = load8_upto(x + l15 * x_stride + c + i * 8, dim - c - i * 8);
-      top = max(top, amax8(f[i]));
-    }
-    top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
-    top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
-    const BlockScale s = block_scale<KIND>(top);
-    i32x8 fa;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const i32x2 codes = keep_upto(to_fp8(f[i], s.inv), dim - c - i * 8);
-      fa[2 * i] = codes[0];
-      fa[2 * i + 1] = codes[1];
-    }
-    const float sa = KIND == kF32 ? __uint_as_float(s.code)
-                                  : __uint_as_float(s.code == 255u ? 0x7fc00000u : s.code << 23);
-    const f32x4 d = block_product<EXACT>(fb, fa);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = min(n0 + l4 * 4 + r, g.n - 1);
-      const float sb = load_scale<KIND>(g.sb, (long)(g.b_tile ? n / kQB : n) * g.sb_stride + kb);
-      acc[r] = fmaf(d[r], sa * sb, acc[r]);
-    }
-  }
-  lds[wave][lane] = acc;
-  __syncthreads();
-  if (wave) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) acc += lds[w][lane];
-  if (l15 >= g.m) return;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = n0 + l4 * 4 + r;
-    if (n < g.n)
-      store_out(g.out, g.out_type, (long)l15 * g.n + n,
-                acc[r] + (g.bias ? bias_at(g.bias, g.bias_type, n) : 0.f));
-  }
-}
-
 template <typename F> void with_type(int type, F f) {
   if (type == kTypeF32) f((float*)0);
   else if (type == kTypeBF16) f((__bf16*)0);
@@ -556,9 +572,17 @@ template <typename F> void with_kind(int kind, F f) {
 
 }  // namespace
 
+// Whether few workgroups of 256x256 outputs would run, fewer than half the chip
+// even with the contraction split: 64x64 tiles then.
+static bool few_outputs(int m, int n, int blocks) {
+  const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
+  return tiles * std::max(1, std::min(blocks / 8, 16)) < 128;
+}
+
 // how many parts the contraction is split into; the caller gives that many
 // [m][n] matrices of floats where there are more than one
 extern "C" int al_fp8_gemm_splits(int m, int n, int blocks) {
+  if (few_outputs(m, n, blocks)) return 1;
   const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
   int s = (int)std::min((long)blocks / 8, 256 / std::max(tiles, 1l));
   return std::max(1, std::min(s, 16));
@@ -570,9 +594,19 @@ extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, i
                             int out_type, float* split_out, int splits, hipStream_t stream) {
   Gemm g = {(const unsigned char*)a, (const unsigned char*)b, sa, sb, lda, ldb, sa_stride,
             sb_stride, m, n, blocks, b_tile, bias, bias_type, out, out_type, split_out, splits};
-  const int tiles_m = (m + 255) / 256, tiles_n = (n + 255) / 256;
   with_kind(kind, [&](auto k) {
     constexpr int KIND = decltype(k)::value;
+    if (splits == 1 && few_outputs(m, n, blocks)) {
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0, stream,
+                           (const unsigned char*)nullptr, 0l, 0, g);
+      };
+      typedef unsigned char C;
+      if (out_type == kTypeF32) b_tile ? go(direct_kernel<C, true, KIND, true, 4, 4, 4>) : go(direct_kernel<C, true, KIND, false, 4, 4, 4>);
+      else b_tile ? go(direct_kernel<C, false, KIND, true, 4, 4, 4>) : go(direct_kernel<C, false, KIND, false, 4, 4, 4>);
+      return;
+    }
+    const int tiles_m = (m + 255) / 256, tiles_n = (n + 255) / 256;
     constexpr int bytes = kRingS + 2 * 512 * (KIND == kE8M0 ? 4 : 16);
     auto go = [&](auto kernel) {
       static bool allowed[64];  // by device: more than 64 KB of LDS is asked for once
@@ -603,8 +637,16 @@ extern "C" void al_fp8_few_rows(int kind, int type, const void* x, long x_stride
     with_kind(kind, [&](auto k) {
       typedef std::remove_pointer_t<decltype(t)> T;
       constexpr int KIND = decltype(k)::value;
-      hipLaunchKernelGGL((few_rows_kernel<T, std::is_same<T, float>::value, KIND>),
-                         dim3((n + 15) / 16), dim3(512), 0, stream, (const T*)x, x_stride, dim, g);
+      constexpr bool EXACT = std::is_same<T, float>::value;
+      auto go = [&](auto kernel, int columns) {
+        hipLaunchKernelGGL(kernel, dim3((n + columns - 1) / columns), dim3(512), 0, stream,
+                           (const T*)x, x_stride, dim, g);
+      };
+      // as many columns as still give each compute unit a workgroup: the more of
+      // them share the quantisation of x the better
+      if (n >= 64 * 256) b_tile ? go(direct_kernel<T, EXACT, KIND, true, 1, 4, 8>, 64) : go(direct_kernel<T, EXACT, KIND, false, 1, 4, 8>, 64);
+      else if (n >= 32 * 256) b_tile ? go(direct_kernel<T, EXACT, KIND, true, 1, 2, 8>, 32) : go(direct_kernel<T, EXACT, KIND, false, 1, 2, 8>, 32);
+      else b_tile ? go(direct_kernel<T, EXACT, KIND, true, 1, 1, 8>, 16) : go(direct_kernel<T, EXACT, KIND, false, 1, 1, 8>, 16);
     });
   });
 }

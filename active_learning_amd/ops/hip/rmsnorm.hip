@@ -134,7 +134,7 @@ __global__ void rms_bwd_kernel(const T* __restrict__ s, long s_stride,
     const long r = r0 + threadIdx.x / TPR;
     if (RPB > 1 && r >= rows) break;
     const float rstd = rstd_in[r];
-    f32x8 u[N], g[N];
+    f32x8 u[N], g[N], add[N];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -142,6 +142,7 @@ __global__ void rms_bwd_kernel(const T* __restrict__ s, long s_stride,
         const int c = (k * TPR + t) * 8;
         u[i] = load8_upto(s + r * s_stride + c, dim - c) * rstd;
         g[i] = load8_upto(dy + r * dim + c, dim - c);
+        if (DSUM && VPT) add[i] = load8_upto(dsum + r * dim + c, dim - c);
         if (VPT) dw[i] += g[i] * u[i];
         g[i] *= VPT ? wv[i] : load8_upto(w + c, dim - c);
 #pragma unroll
@@ -158,7 +159,7 @@ __global__ void rms_bwd_kernel(const T* __restrict__ s, long s_stride,
           g[i] = load8_upto(dy + r * dim + c, dim - c) * load8_upto(w + c, dim - c);
         }
         f32x8 d = (g[i] - u[i] * dot) * rstd;
-        if (DSUM) d += load8_upto(dsum + r * dim + c, dim - c);
+        if (DSUM) d += VPT ? add[i] : load8_upto(dsum + r * dim + c, dim - c);
         if (c < dim) store8_upto(dx + r * dim + c, d, dim - c);
       }
     }
@@ -204,31 +205,32 @@ __global__ void rms_dw_kernel(const T* __restrict__ s, long s_stride,
   part[(long)blockIdx.y * dim + c] = sum;
 }
 
-// out[c] = sum over p of part[p][c]: 64 columns a block, the partial rows over
-// 16 waves, joined in order
+// out[c] = sum over p of part[p][c]: 16 columns a block, the partial rows over 64
+// threads each, joined in order
 template <typename W>
 __launch_bounds__(1024)
 __global__ void col_sum_kernel(const float* __restrict__ part, W* __restrict__ out,
                                int parts, int dim) {
-  __shared__ float lds[16][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), wave = threadIdx.x >> 6;
+  __shared__ float lds[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
   float s = 0.f;
   if (c < dim)
-    for (int p = wave; p < parts; p += 16) s += part[(long)p * dim + c];
-  lds[wave][threadIdx.x & 63] = s;
+    for (int p = y; p < parts; p += 64) s += part[(long)p * dim + c];
+  lds[y][x] = s;
   __syncthreads();
-  if (wave == 0 && c < dim) {
-#pragma unroll
-    for (int i = 1; i < 16; ++i) s += lds[i][threadIdx.x];
+  if (threadIdx.x < 16 && c < dim) {
+    for (int i = 1; i < 64; ++i) s += lds[i][x];
     out[c] = (W)s;
   }
 }
 
 struct Shape { int tpr, vpt; };
 
-// The narrowest group of threads that holds a row in registers. A wave for each
-// row needs no barrier; beyond 32768 values a row is read twice instead.
-Shape shape_for(int dim) {
+// The forward pass: the narrowest group of threads that holds a row in registers,
+// since a wave for each row needs no barrier; where that leaves compute units
+// without a workgroup, four waves. Beyond 32768 values a row is read twice.
+Shape fwd_shape(long rows, int dim) {
+  if (rows < 1024 && dim > 512 && dim <= 2048) return {256, 1};
   if (dim <= 512) return {64, 1};
   if (dim <= 1024) return {64, 2};
   if (dim <= 2048) return {64, 4};
@@ -238,25 +240,33 @@ Shape shape_for(int dim) {
   if (dim <= 32768) return {1024, 4};
   return {1024, 0};
 }
-
-template <typename F> void with_shape(int dim, F f) {
-  const Shape s = shape_for(dim);
-  if (s.tpr == 64) {
-    if (s.vpt == 1) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    else if (s.vpt == 2) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-  } else if (s.tpr == 256) {
-    if (s.vpt == 2) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-  } else {
-    if (s.vpt == 2) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
-    else if (s.vpt == 4) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 4>{});
-    else f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
-  }
+// The backward pass holds four times as much for each value: one vector a thread.
+Shape bwd_shape(long, int dim) {
+  if (dim <= 512) return {64, 1};
+  if (dim <= 2048) return {256, 1};
+  if (dim <= 4096) return {512, 1};
+  if (dim <= 8192) return {1024, 1};
+  if (dim <= 16384) return {1024, 2};
+  return {1024, 0};
 }
 
-int rms_blocks(long rows, int dim, long most) {
-  const int tpr = shape_for(dim).tpr, rpb = tpr < 256 ? 256 / tpr : 1;
+template <int N> using Int = std::integral_constant<int, N>;
+template <typename F> void with_fwd_shape(long rows, int dim, F f) {
+  const Shape s = fwd_shape(rows, dim);
+  if (s.tpr == 64) s.vpt == 1 ? f(Int<64>{}, Int<1>{}) : s.vpt == 2 ? f(Int<64>{}, Int<2>{}) : f(Int<64>{}, Int<4>{});
+  else if (s.tpr == 256) s.vpt == 1 ? f(Int<256>{}, Int<1>{}) : s.vpt == 2 ? f(Int<256>{}, Int<2>{}) : f(Int<256>{}, Int<4>{});
+  else s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : s.vpt == 4 ? f(Int<1024>{}, Int<4>{}) : f(Int<1024>{}, Int<0>{});
+}
+template <typename F> void with_bwd_shape(long rows, int dim, F f) {
+  const Shape s = bwd_shape(rows, dim);
+  if (s.tpr == 64) f(Int<64>{}, Int<1>{});
+  else if (s.tpr == 256) f(Int<256>{}, Int<1>{});
+  else if (s.tpr == 512) f(Int<512>{}, Int<1>{});
+  else s.vpt == 1 ? f(Int<1024>{}, Int<1>{}) : s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : f(Int<1024>{}, Int<0>{});
+}
+
+int blocks_for(Shape s, long rows, long most) {
+  const int rpb = block_of(s.tpr) / s.tpr;
   return (int)std::min((rows + rpb - 1) / rpb, most);
 }
 
@@ -264,8 +274,8 @@ template <typename T, typename W>
 void fwd(const void* x, long x_stride, const void* res, long res_stride, const void* w,
          void* y, void* total, float* rstd, void* q, void* scale, int out, long rows,
          int dim, int pitch, int scale_stride, float eps, hipStream_t stream) {
-  const int blocks = rms_blocks(rows, dim, 2048);
-  with_shape(dim, [&](auto tpr, auto vpt) {
+  const int blocks = blocks_for(fwd_shape(rows, dim), rows, 2048);
+  with_fwd_shape(rows, dim, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(blocks), dim3(block_of(TPR)), 0, stream, (const T*)x,
@@ -282,7 +292,7 @@ template <typename T, typename W>
 void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const void* w,
          const float* rstd, void* dx, float* part, void* dw, int parts, long rows, int dim,
          hipStream_t stream) {
-  with_shape(dim, [&](auto tpr, auto vpt) {
+  with_bwd_shape(rows, dim, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(parts), dim3(block_of(TPR)), TPR < 256 ? dim * 4 : 0,
@@ -295,7 +305,7 @@ void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const v
                          (const T*)s, s_stride, (const T*)dy, rstd, part, rows, dim);
   });
   if (dw)
-    hipLaunchKernelGGL(col_sum_kernel<W>, dim3((dim + 63) / 64), dim3(1024), 0, stream, part,
+    hipLaunchKernelGGL(col_sum_kernel<W>, dim3((dim + 15) / 16), dim3(1024), 0, stream, part,
                        (W*)dw, parts, dim);
 }
 
@@ -321,7 +331,9 @@ extern "C" void al_rms_fwd(int type, int wtype, const void* x, long x_stride,
 }
 
 // how many partial rows of dw the backward pass writes
-extern "C" int al_rms_bwd_parts(long rows, int dim) { return rms_blocks(rows, dim, 512); }
+extern "C" int al_rms_bwd_parts(long rows, int dim) {
+  return blocks_for(bwd_shape(rows, dim), rows, 1024);
+}
 
 extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,
                            const void* dy, const void* dsum, const void* w,
@@ -335,7 +347,7 @@ extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,
 
 extern "C" void al_col_sum(const float* part, void* out, int type, int parts, int dim,
                            hipStream_t stream) {
-  const dim3 grid((dim + 63) / 64), block(1024);
+  const dim3 grid((dim + 15) / 16), block(1024);
   if (type == kTypeF32)
     hipLaunchKernelGGL(col_sum_kernel<float>, grid, block, 0, stream, part, (float*)out, parts, dim);
   else if (type == kTypeBF16)
