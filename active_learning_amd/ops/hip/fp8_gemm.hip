@@ -253,6 +253,10 @@ template <int BYTES> AL_DEV void lds_load(Rsrc from, unsigned off, int step, uns
   else __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Lds)to, 4, off, step, 0, 0);
 }
 
+// all but the COUNT newest of this wave's loads are done, and all its LDS reads
+template <int COUNT> AL_DEV void wait_but() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(COUNT) : "memory");
+}
 AL_DEV void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_barrier" ::: "memory");
@@ -275,6 +279,7 @@ AL_DEV void tile_of(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
 template <int KIND, bool EXACT, bool BTILE>
 __launch_bounds__(512, 2)
 __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
+  static_assert(KIND == kE8M0 || !EXACT, "32-bit scales and results: the direct kernel");
   constexpr bool HW = KIND == kE8M0 && !EXACT;
   constexpr int SB = KIND == kE8M0 ? 4 : 16;  // bytes of four steps' scales
   extern __shared__ __align__(16) unsigned char smem[];
@@ -295,13 +300,13 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   const int rows_a = min(256, g.m - m0), rows_b = min(256, g.n - n0);
   const Rsrc a = rsrc_of(g.a + (long)m0 * g.lda + (long)first * kQB, (long)rows_a * g.lda - (long)first * kQB);
   const Rsrc b = rsrc_of(g.b + (long)n0 * g.ldb + (long)first * kQB, (long)rows_b * g.ldb - (long)first * kQB);
-  unsigned off_a[4], off_b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 64 + wid * 8 + (lane >> 3), chunk = (lane & 7) ^ (r >> 1 & 7);
-    off_a[i] = (unsigned)min(r, rows_a - 1) * (unsigned)g.lda + chunk * 16;
-    off_b[i] = (unsigned)min(r, rows_b - 1) * (unsigned)g.ldb + chunk * 16;
-  }
+  // Rows behind the operand's last are the last one again, and no output of theirs is
+  // stored.
+  const int r = wid * 8 + (lane >> 3);  // and 64 rows on, and on
+  const unsigned chunk = ((lane & 7) ^ (r >> 1 & 7)) * 16;
+  const unsigned off_a = (unsigned)r * (unsigned)g.lda, off_b = (unsigned)r * (unsigned)g.ldb;
+  const unsigned step_a = 64 * (unsigned)g.lda, step_b = 64 * (unsigned)g.ldb;
+  const unsigned last_a = (unsigned)(rows_a - 1) * (unsigned)g.lda, last_b = (unsigned)(rows_b - 1) * (unsigned)g.ldb;
   // scales: the first four waves bring those of a's rows, the others those of b's
   const int sr = (wid & 3) * 64 + lane;
   const int scale_row = wid < 4 ? g.sa_stride * (SB / 4) : g.sb_stride * (SB / 4);  // bytes
@@ -316,17 +321,18 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   // what lies behind the last step is asked for at the last one: every wave has
   // the same loads in flight in every step
   const int last = steps - 1;
-  auto load_a = [&](int k, int h, int ring) {
+  auto load_a = [&](int k, int h, int ring) __attribute__((always_inline)) {
     unsigned char* to = smem + ring + wid * 1024;
-    lds_load<16>(a, off_a[2 * h], min(k, last) * kQB, to);
-    lds_load<16>(a, off_a[2 * h + 1], min(k, last) * kQB, to + 8192);
+    lds_load<16>(a, min(off_a + 2 * h * step_a, last_a) + chunk, min(k, last) * kQB, to);
+    lds_load<16>(a, min(off_a + (2 * h + 1) * step_a, last_a) + chunk, min(k, last) * kQB, to + 8192);
   };
-  auto load_b = [&](int k) {
+  auto load_b = [&](int k) __attribute__((always_inline)) {
     unsigned char* to = smem + kRingB + (k & 1) * 2 * kHalf + wid * 1024;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds_load<16>(b, off_b[i], min(k, last) * kQB, to + i * 8192);
+    for (int i = 0; i < 4; ++i)
+      lds_load<16>(b, min(off_b + i * step_b, last_b) + chunk, min(k, last) * kQB, to + i * 8192);
   };
-  auto load_scales = [&](int word) {
+  auto load_scales = [&](int word) __attribute__((always_inline)) {
     lds_load<SB>(scale, off_s, min(word, last >> 2) * SB, smem + kRingS + ((word & 1) * 512 + wid * 64) * SB);
   };
 
@@ -340,25 +346,35 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[h][i][j][r] = 0.f;
 
-  // the four 16-byte chunks of a lane's row: two for each half of the block
-  int at[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    at[c] = l31 * 128 + (((((c >> 1) * 4) + l5 * 2 + (c & 1)) ^ (l31 >> 1 & 7)) << 4);
-  auto fragment = [&](const unsigned char* p, int half) {
-    const i32x4 lo = *(const i32x4*)(p + at[2 * half]), hi = *(const i32x4*)(p + at[2 * half + 1]);
+  // A lane's row has four 16-byte chunks, two for each half of the block; the other
+  // three lie where bits 4 and 6 of the first one's address are turned over. Where
+  // registers are short these addresses are computed again for each use.
+  auto this_lane = [&]() __attribute__((always_inline)) {
+    if (HW) return lane;
+    int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(l));
+    return l;
+  };
+  auto first_chunk = [&](int l) __attribute__((always_inline)) {
+    return (l & 31) * 128 + (((l >> 5) * 2 ^ (l >> 1 & 7)) << 4);
+  };
+  auto fragment = [&](unsigned first, int half) __attribute__((always_inline)) {
+    typedef const __attribute__((address_space(3))) i32x4* Chunk;
+    const i32x4 lo = *(Chunk)(first ^ (half * 64)), hi = *(Chunk)(first ^ (half * 64 + 16));
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
+  const unsigned lds = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
 
   i32x8 fa[2][2], fb[2][2];
   int sa[2], sb[2];  // e8m0: this step's scales, in the lowest byte; else a float's bits
   // where the scales of step k (the s-th of its four) are
-  auto scale_of = [&](int row, int k, int s) {
+  auto scale_of = [&](int row, int k, int s) __attribute__((always_inline)) {
     const unsigned char* p = smem + kRingS + ((k >> 2 & 1) * 512 + row) * SB;
     return KIND == kF32 ? ((const int*)p)[s] : (int)(*(const unsigned*)p >> (8 * s));
   };
-  auto read_a = [&](int k, int s, int h, int ring) {
-    const unsigned char* p = smem + ring + wr * 64 * 128;
+  auto read_a = [&](int k, int s, int h, int ring) __attribute__((always_inline)) {
+    const int l = this_lane(), l31 = l & 31;
+    const unsigned p = lds + ring + wr * 64 * 128 + first_chunk(l);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       fa[i][0] = fragment(p + i * 32 * 128, 0);
@@ -366,8 +382,9 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
       sa[i] = scale_of(h * 128 + wr * 64 + i * 32 + l31, k, s);
     }
   };
-  auto read_b = [&](int k, int s) {
-    const unsigned char* p = smem + kRingB + (k & 1) * 2 * kHalf + wc * 64 * 128;
+  auto read_b = [&](int k, int s) __attribute__((always_inline)) {
+    const int l = this_lane(), l31 = l & 31;
+    const unsigned p = lds + kRingB + (k & 1) * 2 * kHalf + wc * 64 * 128 + first_chunk(l);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       fb[j][0] = fragment(p + j * 32 * 128, 0);
@@ -375,7 +392,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
       if (KIND == kE8M0 || BTILE) sb[j] = scale_of(256 + wc * 64 + j * 32 + l31, k, s);
     }
   };
-  auto multiply = [&](int k, int s, f32x16 (&c)[2][2]) {
+  auto multiply = [&](int k, int s, f32x16 (&c)[2][2]) __attribute__((always_inline)) {
     __builtin_amdgcn_s_setprio(1);
     if (HW) {
 #pragma unroll
@@ -412,17 +429,8 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) d[r] = 0.f;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (!EXACT) {
-              d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][half], fa[i][half], d, 0, 0, 0, 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int q = 0; q < 8; q += 2)
-                d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    to_bf16(fb[j][half][q], fb[j][half][q + 1], 1.f),
-                    to_bf16(fa[i][half][q], fa[i][half][q + 1], 1.f), d, 0, 0, 0);
-            }
-          }
+          for (int half = 0; half < 2; ++half)
+            d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][half], fa[i][half], d, 0, 0, 0, 0, 0, 0);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int by = BTILE ? sb[j] : scale_of(256 + wc * 64 + j * 32 + (r >> 2) * 8 + l5 * 4 + (r & 3), k, s);
@@ -445,82 +453,94 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   if (wr) phase_barrier();
   int read = 0, write = 4 * kHalf;  // places in a's ring
   auto next = [](int at) { return at == 4 * kHalf ? 0 : at + kHalf; };
-  // Four steps a turn, without a branch between a phase's parts: the compiler would
+  // The s-th of four steps, without a branch between its parts: the compiler would
   // move matrix instructions over it.
-  for (int k = 0;; k += 4) {
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      read_b(k + s, s);
-      read_a(k + s, s, 0, read);
-      load_a(k + s + 2, 0, write);
-      // not before the second group's last phase of the words' last user is over
-      if (s == 1) load_scales((k >> 2) + 1);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      phase_barrier();
-      multiply(k + s, s, acc[0]);
-      phase_barrier();
-      read = next(read);
-      write = next(write);
-      read_a(k + s, s, 1, read);
-      load_a(k + s + 2, 1, write);
-      load_b(k + s + 2);
-      // The next step's tiles are there, in every wave's part: the eight newest
-      // loads are those of the step after it.
-      asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
-      phase_barrier();
-      multiply(k + s, s, acc[1]);
-      phase_barrier();
-      read = next(read);
-      write = next(write);
-      if (k + s == last) goto done;
+  auto one_step = [&](auto s_, int k) __attribute__((always_inline)) {
+    constexpr int s = decltype(s_)::value;
+    read_b(k, s);
+    read_a(k, s, 0, read);
+    load_a(k + 2, 0, write);
+    // not before the second group's last phase of the words' last user is over
+    if (s == 1) load_scales((k >> 2) + 1);
+    wait_but<63>();
+    phase_barrier();
+    multiply(k, s, acc[0]);
+    phase_barrier();
+    read = next(read);
+    write = next(write);
+    read_a(k, s, 1, read);
+    load_a(k + 2, 1, write);
+    load_b(k + 2);
+    // The next step's tiles are there, in every wave's part: newer are the loads of
+    // the step after it.
+    wait_but<s == 1 ? 9 : 8>();
+    phase_barrier();
+    multiply(k, s, acc[1]);
+    phase_barrier();
+    read = next(read);
+    write = next(write);
+  };
+  int k = 0;
+  for (; k + 4 <= steps; k += 4) {
+    one_step(std::integral_constant<int, 0>{}, k);
+    one_step(std::integral_constant<int, 1>{}, k + 1);
+    one_step(std::integral_constant<int, 2>{}, k + 2);
+    one_step(std::integral_constant<int, 3>{}, k + 3);
+  }
+  if (k < steps) {
+    one_step(std::integral_constant<int, 0>{}, k);
+    if (k + 1 < steps) {
+      one_step(std::integral_constant<int, 1>{}, k + 1);
+      if (k + 2 < steps) one_step(std::integral_constant<int, 2>{}, k + 2);
     }
   }
-done:
   if (!wr) phase_barrier();
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   phase_barrier();
+
+  // computed anew: kept until here they would take registers from the loop
+  int own = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(own));
+  const int e31 = own & 31, e5 = own >> 5, thread = wid * 64 + own;
 
   // Through LDS, so that rows are written in whole lines; 16-byte chunks again
   // spread over the banks by their row.
   const bool split = g.splits > 1;
   float* bias = (float*)(smem + kRingS);  // the scales' place: 256 floats
-  if (threadIdx.x < 256)
-    bias[threadIdx.x] = g.bias && !split && n0 + (int)threadIdx.x < g.n
-                            ? bias_at(g.bias, g.bias_type, n0 + threadIdx.x) : 0.f;
+  if (thread < 256)
+    bias[thread] = g.bias && !split && n0 + thread < g.n
+                            ? bias_at(g.bias, g.bias_type, n0 + thread) : 0.f;
   __syncthreads();
-  auto each_four = [&](int h, auto put) {
+  auto each_four = [&](int h, auto put) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int n = wc * 64 + j * 32 + q * 8 + l5 * 4;
+        const int n = wc * 64 + j * 32 + q * 8 + e5 * 4;
         const f32x4 add = *(const f32x4*)(bias + n);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           f32x4 v;
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = acc[h][i][j][q * 4 + r] + add[r];
-          put(h * 128 + wr * 64 + i * 32 + l31, n, v);
+          put(h * 128 + wr * 64 + i * 32 + e31, n, v);
         }
       }
   };
   if (!EXACT && !split) {
-    auto put_all = [&](auto convert) {
+    const bool halves = g.out_type == kTypeF16;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        each_four(h, [&](int m, int n, f32x4 v) {
-          *(s16x4*)(smem + m * 512 + (((n >> 3) ^ l31) << 4) + (n & 4) * 2) = convert(v);
-        });
-    };
-    if (g.out_type == kTypeF16)
-      put_all([](f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4v)); });
-    else
-      put_all([](f32x4 v) { return __builtin_bit_cast(s16x4, __builtin_convertvector(v, bf16x4v)); });
+    for (int h = 0; h < 2; ++h)
+      each_four(h, [&](int m, int n, f32x4 v) {
+        *(s16x4*)(smem + m * 512 + (((n >> 3) ^ e31) << 4) + (n & 4) * 2) =
+            halves ? __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4v))
+                   : __builtin_bit_cast(s16x4, __builtin_convertvector(v, bf16x4v));
+      });
     __syncthreads();
-    const int c = threadIdx.x & 31, left = g.n - n0 - c * 8;
+    const int c = thread & 31, left = g.n - n0 - c * 8;
     const int high = left > 0 ? min(256, g.m - m0) : 0;
     short* out = (short*)g.out + (long)m0 * g.n + n0 + c * 8;
-    for (int m = threadIdx.x >> 5; m < high; m += 16) {
+    for (int m = thread >> 5; m < high; m += 16) {
       const s16x8 v = *(const s16x8*)(smem + m * 512 + ((c ^ (m & 31)) << 4));
       short* to = out + (long)m * g.n;
       if (left >= 8) __builtin_memcpy(to, &v, 16);
@@ -534,12 +554,12 @@ done:
   for (int h = 0; h < 2; ++h) {
     if (h) __syncthreads();
     each_four(h, [&](int m, int n, f32x4 v) {
-      *(f32x4*)(smem + (m & 127) * 1024 + (((n >> 2) ^ l31) << 4)) = v;
+      *(f32x4*)(smem + (m & 127) * 1024 + (((n >> 2) ^ e31) << 4)) = v;
     });
     __syncthreads();
-    const int c = threadIdx.x & 63, left = g.n - n0 - c * 4;
+    const int c = thread & 63, left = g.n - n0 - c * 4;
     const int high = left > 0 ? min(128, g.m - m0 - h * 128) : 0;
-    for (int m = threadIdx.x >> 6; m < high; m += 8) {
+    for (int m = thread >> 6; m < high; m += 8) {
       const float* from = (const float*)(smem + m * 1024 + ((c ^ (m & 31)) << 4));
       float* to = out + (long)(h * 128 + m) * g.n + c * 4;
       if (left >= 4) __builtin_memcpy(to, from, 16);
@@ -572,17 +592,19 @@ template <typename F> void with_kind(int kind, F f) {
 
 }  // namespace
 
-// Whether few workgroups of 256x256 outputs would run, fewer than half the chip
-// even with the contraction split: 64x64 tiles then.
-static bool few_outputs(int m, int n, int blocks) {
+// Whether the direct kernel's 64x64 tiles are taken: where few workgroups of 256x256
+// outputs would run, fewer than half the chip even with the contraction split; and
+// for 32-bit results with 32-bit scales, which the large tile has no registers for.
+static bool direct_tiles(int kind, int out_type, int m, int n, int blocks) {
   const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
-  return tiles * std::max(1, std::min(blocks / 8, 16)) < 128;
+  return (kind == kF32 && out_type == kTypeF32) ||
+         tiles * std::max(1, std::min(blocks / 8, 16)) < 128;
 }
 
-// how many parts the contraction is split into; the caller gives that many
-// [m][n] matrices of floats where there are more than one
-extern "C" int al_fp8_gemm_splits(int m, int n, int blocks) {
-  if (few_outputs(m, n, blocks)) return 1;
+// How many parts the contraction is split into; the caller gives that many [m][n]
+// matrices of floats where there are more than one.
+extern "C" int al_fp8_gemm_splits(int kind, int out_type, int m, int n, int blocks) {
+  if (direct_tiles(kind, out_type, m, n, blocks)) return 1;
   const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
   int s = (int)std::min((long)blocks / 8, 256 / std::max(tiles, 1l));
   return std::max(1, std::min(s, 16));
@@ -596,7 +618,7 @@ extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, i
             sb_stride, m, n, blocks, b_tile, bias, bias_type, out, out_type, split_out, splits};
   with_kind(kind, [&](auto k) {
     constexpr int KIND = decltype(k)::value;
-    if (splits == 1 && few_outputs(m, n, blocks)) {
+    if (direct_tiles(kind, out_type, m, n, blocks)) {
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0, stream,
                            (const unsigned char*)nullptr, 0l, 0, g);
@@ -618,8 +640,13 @@ extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, i
       }
       hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n, splits), dim3(512), bytes, stream, g, tiles_m, tiles_n);
     };
-    if (out_type == kTypeF32) b_tile ? go(gemm256_kernel<KIND, true, true>) : go(gemm256_kernel<KIND, true, false>);
-    else b_tile ? go(gemm256_kernel<KIND, false, true>) : go(gemm256_kernel<KIND, false, false>);
+    if constexpr (KIND == kE8M0) {
+      if (out_type == kTypeF32) {
+        b_tile ? go(gemm256_kernel<KIND, true, true>) : go(gemm256_kernel<KIND, true, false>);
+        return;
+      }
+    }
+    b_tile ? go(gemm256_kernel<KIND, false, true>) : go(gemm256_kernel<KIND, false, false>);
   });
   if (splits > 1) {
     const int join = (int)std::min(((long)m * n + 255) / 256, 2048l);

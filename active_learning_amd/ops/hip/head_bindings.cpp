@@ -33,7 +33,7 @@ void al_quant_rows(int type, int kind, const void* x, long row_stride, long col_
 void al_quant_tile(int type, int kind, int tile, const void* x, long row_stride, int rows,
                    int cols, void* q, void* scale, int pitch, int scale_stride, void* qt,
                    void* scale_t, int pitch_t, int scale_t_stride, float* part, void* stream);
-int al_fp8_gemm_splits(int m, int n, int blocks);
+int al_fp8_gemm_splits(int kind, int out_type, int m, int n, int blocks);
 void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, int sa_stride, const void* b,
                  const void* sb, long ldb, int sb_stride, int b_tile, int m, int n, int blocks,
                  const void* bias, int bias_type, void* out, int out_type, float* split_out,
@@ -345,7 +345,7 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor
   Tensor out = torch::empty({m, n}, a.options().dtype(out_type));
   const int ot = type_of(out, "output"), blocks = (int)blocks_of(k);
   if (!m || !n) return out;
-  const int splits = al_fp8_gemm_splits((int)m, (int)n, blocks);
+  const int splits = al_fp8_gemm_splits(kind_of(sa), ot, (int)m, (int)n, blocks);
   Tensor split;
   if (splits > 1) split = torch::empty({splits, m, n}, a.options().dtype(torch::kFloat32));
   al_fp8_gemm(kind_of(sa), a.data_ptr(), sa.data_ptr(), a.size(1), (int)sa.size(1), b.data_ptr(),

@@ -648,3 +648,21 @@ def test_no_second_gradient(what):
     assert torch.equal(dx, plain)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.sum(), dy)
+
+
+# a workgroup computes several of these products' tiles after each other: one step
+# each, two, and counts that end in every place of four; edges at both sides; a split
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m,n,k", [(4096, 4608, 100), (4097, 4500, 256), (4200, 4352, 384), (8000, 2300, 512),
+                                   (2100, 9000, 640), (5000, 4100, 1100), (300, 33000, 900), (2048, 2048, 2176)])
+def test_matmul_many_tiles(m, n, k, kind):
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2)
+    bias = randn(n, seed=3)
+    a = quantize_fp8(x, scale=kind)
+    av = a.dequantize()
+    for tile in (True, False):
+        b = quantize_fp8(w, tile=tile, scale=kind)
+        for out, add in ((torch.bfloat16, bias), (torch.float16, None), (torch.float32, bias)):
+            y = fp8_matmul(a, b, add, out)
+            product_within(y, av, b.dequantize(), add)
+            assert torch.equal(y, fp8_matmul(a, b, add, out))
