@@ -12,6 +12,8 @@
 #include "al_common.h"
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -72,6 +74,9 @@ struct BlockScale {
   float inv;      // codes are value * inv
   unsigned code;  // e8m0 byte, or the bits of the 32-bit scale
 };
+AL_DEV float e8m0_value(unsigned code) {
+  return __uint_as_float(code == 255u ? 0x7fc00000u : code << 23);
+}
 
 template <int KIND> AL_DEV BlockScale block_scale(unsigned amax) {
   BlockScale s;
@@ -103,14 +108,91 @@ template <int KIND> AL_DEV float load_scale(const void* p, long at) {
   return __uint_as_float(c == 255u ? 0x7fc00000u : c << 23);
 }
 
+// Eight values as they are in memory, and the work on them that needs no unpacking:
+// 16-bit magnitudes are compared as whole numbers, two at a time, and the conversion
+// to e4m3 takes them, and a power of two to divide by, directly.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+template <typename T> struct Raw8 { typedef i32x4 V; };
+template <> struct Raw8<float> { typedef f32x8 V; };
+
+template <typename T> AL_DEV typename Raw8<T>::V raw8(const T* p) {
+  typename Raw8<T>::V v;
+  __builtin_memcpy(&v, p, sizeof(T) * 8);
+  return v;
+}
+template <typename T> AL_DEV typename Raw8<T>::V raw8_upto(const T* p, int left) {
+  if (left >= 8) return raw8(p);
+  typename Vec8<T>::V v = (typename Vec8<T>::V)(T)0;
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < left) v[i] = p[i];
+  return __builtin_bit_cast(typename Raw8<T>::V, v);
+}
+template <typename T> AL_DEV f32x8 unpack(typename Raw8<T>::V v) {
+  return __builtin_convertvector(__builtin_bit_cast(typename Vec8<T>::V, v), f32x8);
+}
+
+// the largest magnitude so far
+template <typename T> struct Top {
+  u16x2 m = {0, 0};
+  AL_DEV void add(int two) { m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, two & 0x7fff7fff)); }
+  AL_DEV void add(i32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add(v[i]);
+  }
+  // as the bits of a 32-bit float
+  AL_DEV static unsigned bits(unsigned short v) {
+    return abs_bits((float)__builtin_bit_cast(T, v));
+  }
+  AL_DEV unsigned bits() const { return bits(m[0] > m[1] ? m[0] : m[1]); }
+};
+template <> struct Top<float> {
+  unsigned m = 0;
+  AL_DEV void add(f32x8 v) { m = max(m, amax8(v)); }
+  AL_DEV unsigned bits() const { return m; }
+};
+
+// two values' codes into the lower or upper half of `to`; e8m0: divided by a power of two
+template <bool HIGH> AL_DEV int two_codes(int to, float x, float y, float scale) {
+  return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(__builtin_bit_cast(s16x2, to), x, y, scale, HIGH));
+}
+template <typename T, bool HIGH> AL_DEV int two_codes(int to, int two, float scale) {
+  const s16x2 t = __builtin_bit_cast(s16x2, to);
+  if constexpr (std::is_same<T, __bf16>::value)
+    return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(t, __builtin_bit_cast(bf16x2v, two), scale, HIGH));
+  else
+    return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(t, __builtin_bit_cast(f16x2v, two), scale, HIGH));
+}
+
 // eight values to eight e4m3 codes, rounded to nearest even
-AL_DEV i32x2 to_fp8(f32x8 f, float inv) {
+template <int KIND> AL_DEV i32x2 to_fp8(f32x8 f, BlockScale s) {
   i32x2 r;
-  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, 0, false);
-  r[0] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
-  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, 0, false);
-  r[1] = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
+  if (KIND == kE8M0) {
+    const float by = e8m0_value(s.code);
+    r[0] = two_codes<true>(two_codes<false>(0, f[0], f[1], by), f[2], f[3], by);
+    r[1] = two_codes<true>(two_codes<false>(0, f[4], f[5], by), f[6], f[7], by);
+    return r;
+  }
+  int lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * s.inv, f[1] * s.inv, 0, false);
+  r[0] = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * s.inv, f[3] * s.inv, lo, true);
+  int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * s.inv, f[5] * s.inv, 0, false);
+  r[1] = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * s.inv, f[7] * s.inv, hi, true);
   return r;
+}
+template <typename T, int KIND> AL_DEV i32x2 raw_to_fp8(typename Raw8<T>::V v, BlockScale s) {
+  if constexpr (std::is_same<T, float>::value) {
+    return to_fp8<KIND>(v, s);
+  } else if constexpr (KIND == kF32) {
+    return to_fp8<KIND>(unpack<T>(v), s);
+  } else {
+    const float by = e8m0_value(s.code);
+    i32x2 r;
+    r[0] = two_codes<T, true>(two_codes<T, false>(0, v[0], by), v[1], by);
+    r[1] = two_codes<T, true>(two_codes<T, false>(0, v[2], by), v[3], by);
+    return r;
+  }
 }
 
 // the first `left` of eight codes, zero behind them (also where the codes are NaN)

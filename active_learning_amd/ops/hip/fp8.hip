@@ -20,16 +20,20 @@ __global__ void quant_rows_kernel(const T* __restrict__ x, long row_stride, long
   for (long b = (long)blockIdx.x * 16 + (threadIdx.x >> 4); b < blocks; b += (long)gridDim.x * 16) {
     const long r = b / per_row;
     const int kb = (int)(b - r * per_row), c = kb * kQB + lane * 8;
-    f32x8 f = {0, 0, 0, 0, 0, 0, 0, 0};
+    typename Raw8<T>::V v;
     if (STRIDED) {
+      typename Vec8<T>::V e = (typename Vec8<T>::V)(T)0;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < dim) f[i] = (float)x[r * row_stride + (c + i) * col_stride];
+        if (c + i < dim) e[i] = x[r * row_stride + (c + i) * col_stride];
+      v = __builtin_bit_cast(typename Raw8<T>::V, e);
     } else {
-      f = load8_upto(x + r * row_stride + c, dim - c);
+      v = raw8_upto(x + r * row_stride + c, dim - c);
     }
-    const BlockScale s = block_scale<KIND>(max_over_16(amax8(f)));
-    *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8(f, s.inv), dim - c);
+    Top<T> top;
+    top.add(v);
+    const BlockScale s = block_scale<KIND>(max_over_16(top.bits()));
+    *(i32x2*)(q + r * pitch + c) = keep_upto(raw_to_fp8<T, KIND>(v, s), dim - c);
     if (lane == 0) store_scale<KIND>(scale, r * scale_stride + kb, s.code);
   }
 }
@@ -45,23 +49,32 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
                                   int pitch, int scale_stride,
                                   unsigned char* __restrict__ qt, void* __restrict__ scale_t,
                                   int pitch_t, int scale_t_stride, float* __restrict__ part) {
-  __shared__ unsigned words[16][kQB];  // column maxima or sums of each 8 rows
-  __shared__ float col_inv[kQB];
-  __shared__ __align__(16) unsigned char bytes[kQB][144];
+  constexpr bool WIDE = std::is_same<T, float>::value;
+  // column maxima (16-bit types: of two columns a word) or sums of each 8 rows
+  __shared__ unsigned words[16][kQB];
+  __shared__ unsigned col_code[kQB];
+  // a column's eight bytes of rows 8u .. 8u + 7 lie at u ^ (column >> 3): lanes that
+  // write eight columns apart then fall on different banks
+  __shared__ __align__(16) unsigned char bytes[kQB][kQB];
   const int t = threadIdx.x, c8 = t & 15, rg = t >> 4;
   const int r0 = blockIdx.y * kQB, c0 = blockIdx.x * kQB;
   const int row = r0 + rg * 8, col = c0 + c8 * 8;
-  f32x8 f[8];
+  typename Raw8<T>::V v[8];
+  if (row + 8 <= rows && col + 8 <= cols) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    f[j] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (row + j < rows) f[j] = load8_upto(x + (long)(row + j) * row_stride + col, cols - col);
+    for (int j = 0; j < 8; ++j) v[j] = raw8(x + (long)(row + j) * row_stride + col);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = row + j < rows ? raw8_upto(x + (long)(row + j) * row_stride + col, cols - col)
+                            : (typename Raw8<T>::V)0;
   }
   BlockScale all;
   if (TILE) {
-    unsigned m = 0;
+    Top<T> top;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, amax8(f[j]));
+    for (int j = 0; j < 8; ++j) top.add(v[j]);
+    unsigned m = top.bits();
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
     if ((t & 63) == 0) words[0][t >> 6] = m;
@@ -78,22 +91,24 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       BlockScale s = all;
-      if (!TILE) s = block_scale<KIND>(max_over_16(amax8(f[j])));
+      if (!TILE) {
+        Top<T> top;
+        top.add(v[j]);
+        s = block_scale<KIND>(max_over_16(top.bits()));
+      }
       if (row + j < rows) {
-        *(i32x2*)(q + (long)(row + j) * pitch + col) = keep_upto(to_fp8(f[j], s.inv), cols - col);
+        *(i32x2*)(q + (long)(row + j) * pitch + col) = keep_upto(raw_to_fp8<T, KIND>(v[j], s), cols - col);
         if (!TILE && c8 == 0)
           store_scale<KIND>(scale, (long)(row + j) * scale_stride + blockIdx.x, s.code);
       }
     }
   }
   if (part) {
+    f32x8 s = unpack<T>(v[0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float s = 0.f;
+    for (int j = 1; j < 8; ++j) s += unpack<T>(v[j]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += f[j][i];
-      words[rg][c8 * 8 + i] = __float_as_uint(s);
-    }
+    for (int i = 0; i < 8; ++i) words[rg][c8 * 8 + i] = __float_as_uint(s[i]);
     __syncthreads();
     if (t < kQB && c0 + t < cols) {
       float s = 0.f;
@@ -105,20 +120,38 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
   }
   if (!qt) return;
   if (!TILE) {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned m = 0;
+      for (int i = 0; i < 8; ++i) {
+        unsigned m = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(f[j][i]));
-      words[rg][c8 * 8 + i] = m;
+        for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j][i]));
+        words[rg][c8 * 8 + i] = m;
+      }
+    } else {
+      i32x4 m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        Top<T> top;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top.add(v[j][i]);
+        m[i] = __builtin_bit_cast(int, top.m);
+      }
+      *(i32x4*)&words[rg][c8 * 4] = m;
     }
     __syncthreads();
     if (t < kQB) {
       unsigned m = 0;
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int g = 0; g < 16; ++g) m = max(m, words[g][t]);
+        for (int g = 0; g < 16; ++g) m = max(m, words[g][t]);
+      } else {
+#pragma unroll
+        for (int g = 0; g < 16; ++g) m = max(m, words[g][t >> 1] >> (16 * (t & 1)) & 0xffffu);
+        m = Top<T>::bits((unsigned short)m);
+      }
       const BlockScale s = block_scale<KIND>(m);
-      col_inv[t] = s.inv;
+      col_code[t] = KIND == kE8M0 ? s.code : __float_as_uint(s.inv);
       if (c0 + t < cols)
         store_scale<KIND>(scale_t, (long)(c0 + t) * scale_t_stride + blockIdx.y, s.code);
     }
@@ -126,18 +159,41 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    f32x8 v;
+    BlockScale s = all;
+    if (!TILE) {
+      const unsigned c = col_code[c8 * 8 + i];
+      s.code = c;
+      s.inv = __uint_as_float(c);
+    }
+    i32x2 codes;
+    if constexpr (WIDE || KIND == kF32) {
+      f32x8 f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = f[j][i];
-    const float inv = TILE ? all.inv : col_inv[c8 * 8 + i];
-    *(i32x2*)&bytes[c8 * 8 + i][rg * 8] = keep_upto(to_fp8(v, inv), rows - row);
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (WIDE) f[j] = v[j][i];
+        else f[j] = (float)__builtin_bit_cast(typename Vec8<T>::V, v[j])[i];
+      }
+      codes = to_fp8<KIND>(f, s);
+    } else {
+      // two rows of a column side by side, as the conversion takes them
+      const float by = e8m0_value(s.code);
+      int two[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        two[j] = (int)__builtin_amdgcn_perm((unsigned)v[2 * j + 1][i >> 1], (unsigned)v[2 * j][i >> 1],
+                                            i & 1 ? 0x07060302u : 0x05040100u);
+      codes[0] = two_codes<T, true>(two_codes<T, false>(0, two[0], by), two[1], by);
+      codes[1] = two_codes<T, true>(two_codes<T, false>(0, two[2], by), two[3], by);
+    }
+    *(i32x2*)&bytes[c8 * 8 + i][(rg ^ c8) * 8] = keep_upto(codes, rows - row);
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = (t >> 3) + i * 32, at = (t & 7) * 16;
-    if (c0 + c < cols)
-      *(i32x4*)(qt + (long)(c0 + c) * pitch_t + r0 + at) = *(const i32x4*)&bytes[c][at];
+    const int c = (t >> 3) + i * 32, at = t & 7, turn = c >> 3;
+    i32x4 two = *(const i32x4*)&bytes[c][(at ^ turn >> 1) * 16];
+    if (turn & 1) two = i32x4{two[2], two[3], two[0], two[1]};
+    if (c0 + c < cols) *(i32x4*)(qt + (long)(c0 + c) * pitch_t + r0 + at * 16) = two;
   }
 }
 

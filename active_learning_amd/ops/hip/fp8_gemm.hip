@@ -113,7 +113,7 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 
   struct Raw {
     i32x8 a[VALUES ? 1 : MT], b[NT];
-    typename std::conditional<VALUES, T, float>::type v[VALUES ? 32 : 1];
+    typename Raw8<typename std::conditional<VALUES, T, float>::type>::V v[VALUES ? 4 : 1];
     unsigned sa[MT], sb[NT];
   };
   auto load32 = [](const unsigned char* p) {
@@ -127,11 +127,17 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
       r.sb[j] = scale_code<KIND>(g.sb, sb[j] + kb);
     }
     if (VALUES) {
-      const int left = dim - kb * kQB - l4 * 32;  // a block's tail is masked where it is quantised
+      const int left = dim - kb * kQB - l4 * 32;
       const T* p = (const T*)a[0] + (long)kb * kQB;
-      if ((kb + 1) * kQB <= dim) __builtin_memcpy(&r.v, p, sizeof(T) * 32);
-      else
-        for (int i = 0; i < 32; ++i) r.v[VALUES ? i : 0] = i < left ? p[i] : (T)0;
+      if constexpr (VALUES) {
+        if ((kb + 1) * kQB <= dim) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r.v[i] = raw8(p + i * 8);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r.v[i] = raw8_upto(p + i * 8, left - i * 8);
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -141,15 +147,11 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
     }
   };
   auto compute = [&](Raw& r, int kb) {
-    if (VALUES) {
-      f32x8 f[4];
-      unsigned top = 0;
+    if constexpr (VALUES) {
+      Top<T> most;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[i][e] = (float)r.v[VALUES ? i * 8 + e : 0];
-        top = max(top, amax8(f[i]));
-      }
+      for (int i = 0; i < 4; ++i) most.add(r.v[i]);
+      unsigned top = most.bits();
       top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
       top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
       const BlockScale s = block_scale<KIND>(top);
@@ -157,7 +159,7 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
       const int left = dim - kb * kQB - l4 * 32;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const i32x2 codes = keep_upto(to_fp8(f[i], s.inv), left - i * 8);
+        const i32x2 codes = keep_upto(raw_to_fp8<T, KIND>(r.v[i], s), left - i * 8);
         r.a[0][2 * i] = codes[0];
         r.a[0][2 * i + 1] = codes[1];
       }

@@ -99,7 +99,7 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
           constexpr int KIND = OUT == kOutE8M0 ? kE8M0 : kF32;
           const BlockScale b = block_scale<KIND>(max_over_16(amax8(f)));
           if (c < pitch) {
-            *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8(f, b.inv), dim - c);
+            *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8<KIND>(f, b), dim - c);
             if ((t & 15) == 0 && c < dim)
               store_scale<KIND>(scale, r * scale_stride + c / kQB, b.code);
           }
