@@ -3,6 +3,8 @@
 
 #include "al_fp8.h"
 
+#include <algorithm>
+
 namespace {
 
 // --------------------------------------------------------------------------
@@ -48,7 +50,8 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
                                   unsigned char* __restrict__ q, void* __restrict__ scale,
                                   int pitch, int scale_stride,
                                   unsigned char* __restrict__ qt, void* __restrict__ scale_t,
-                                  int pitch_t, int scale_t_stride, float* __restrict__ part) {
+                                  int pitch_t, int scale_t_stride, float* __restrict__ part,
+                                  int across, int tiles) {
   constexpr bool WIDE = std::is_same<T, float>::value;
   // column maxima (16-bit types: of two columns a word) or sums of each 8 rows
   __shared__ unsigned words[16][kQB];
@@ -57,143 +60,155 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
   // write eight columns apart then fall on different banks
   __shared__ __align__(16) unsigned char bytes[kQB][kQB];
   const int t = threadIdx.x, c8 = t & 15, rg = t >> 4;
-  const int r0 = blockIdx.y * kQB, c0 = blockIdx.x * kQB;
-  const int row = r0 + rg * 8, col = c0 + c8 * 8;
-  typename Raw8<T>::V v[8];
-  if (row + 8 <= rows && col + 8 <= cols) {
+  typedef typename Raw8<T>::V Raw;
+  auto load = [&](Raw (&v)[8], int tile) {
+    const int row = tile / across * kQB + rg * 8, col = tile % across * kQB + c8 * 8;
+    if (row + 8 <= rows && col + 8 <= cols) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = raw8(x + (long)(row + j) * row_stride + col);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[j] = row + j < rows ? raw8_upto(x + (long)(row + j) * row_stride + col, cols - col)
-                            : (typename Raw8<T>::V)0;
-  }
-  BlockScale all;
-  if (TILE) {
-    Top<T> top;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top.add(v[j]);
-    unsigned m = top.bits();
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-    if ((t & 63) == 0) words[0][t >> 6] = m;
-    __syncthreads();
-    m = max(max(words[0][0], words[0][1]), max(words[0][2], words[0][3]));
-    all = block_scale<KIND>(m);
-    if (t == 0) {
-      if (q) store_scale<KIND>(scale, (long)blockIdx.y * scale_stride + blockIdx.x, all.code);
-      if (qt) store_scale<KIND>(scale_t, (long)blockIdx.x * scale_t_stride + blockIdx.y, all.code);
-    }
-    __syncthreads();
-  }
-  if (q) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      BlockScale s = all;
-      if (!TILE) {
-        Top<T> top;
-        top.add(v[j]);
-        s = block_scale<KIND>(max_over_16(top.bits()));
-      }
-      if (row + j < rows) {
-        *(i32x2*)(q + (long)(row + j) * pitch + col) = keep_upto(raw_to_fp8<T, KIND>(v[j], s), cols - col);
-        if (!TILE && c8 == 0)
-          store_scale<KIND>(scale, (long)(row + j) * scale_stride + blockIdx.x, s.code);
-      }
-    }
-  }
-  if (part) {
-    f32x8 s = unpack<T>(v[0]);
-#pragma unroll
-    for (int j = 1; j < 8; ++j) s += unpack<T>(v[j]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) words[rg][c8 * 8 + i] = __float_as_uint(s[i]);
-    __syncthreads();
-    if (t < kQB && c0 + t < cols) {
-      float s = 0.f;
-#pragma unroll
-      for (int g = 0; g < 16; ++g) s += __uint_as_float(words[g][t]);
-      part[(long)blockIdx.y * cols + c0 + t] = s;
-    }
-    __syncthreads();
-  }
-  if (!qt) return;
-  if (!TILE) {
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        unsigned m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j][i]));
-        words[rg][c8 * 8 + i] = m;
-      }
+      for (int j = 0; j < 8; ++j) v[j] = raw8(x + (long)(row + j) * row_stride + col);
     } else {
-      i32x4 m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        Top<T> top;
+      for (int j = 0; j < 8; ++j)
+        v[j] = row + j < rows ? raw8_upto(x + (long)(row + j) * row_stride + col, cols - col) : (Raw)0;
+    }
+  };
+  // the next tile's values are on their way while this one's are worked on
+  Raw v[8], next[8];
+  load(v, blockIdx.x);
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int by = tile / across, bx = tile % across;
+    const int r0 = by * kQB, c0 = bx * kQB, row = r0 + rg * 8, col = c0 + c8 * 8;
+    if (tile + (int)gridDim.x < tiles) load(next, tile + gridDim.x);
+    BlockScale all;
+    if (TILE) {
+      Top<T> top;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top.add(v[j][i]);
-        m[i] = __builtin_bit_cast(int, top.m);
+      for (int j = 0; j < 8; ++j) top.add(v[j]);
+      unsigned m = top.bits();
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+      if ((t & 63) == 0) words[0][t >> 6] = m;
+      __syncthreads();
+      m = max(max(words[0][0], words[0][1]), max(words[0][2], words[0][3]));
+      all = block_scale<KIND>(m);
+      if (t == 0) {
+        if (q) store_scale<KIND>(scale, (long)by * scale_stride + bx, all.code);
+        if (qt) store_scale<KIND>(scale_t, (long)bx * scale_t_stride + by, all.code);
       }
-      *(i32x4*)&words[rg][c8 * 4] = m;
+      __syncthreads();
     }
-    __syncthreads();
-    if (t < kQB) {
-      unsigned m = 0;
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int g = 0; g < 16; ++g) m = max(m, words[g][t]);
-      } else {
-#pragma unroll
-        for (int g = 0; g < 16; ++g) m = max(m, words[g][t >> 1] >> (16 * (t & 1)) & 0xffffu);
-        m = Top<T>::bits((unsigned short)m);
-      }
-      const BlockScale s = block_scale<KIND>(m);
-      col_code[t] = KIND == kE8M0 ? s.code : __float_as_uint(s.inv);
-      if (c0 + t < cols)
-        store_scale<KIND>(scale_t, (long)(c0 + t) * scale_t_stride + blockIdx.y, s.code);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    BlockScale s = all;
-    if (!TILE) {
-      const unsigned c = col_code[c8 * 8 + i];
-      s.code = c;
-      s.inv = __uint_as_float(c);
-    }
-    i32x2 codes;
-    if constexpr (WIDE || KIND == kF32) {
-      f32x8 f;
+    if (q) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if constexpr (WIDE) f[j] = v[j][i];
-        else f[j] = (float)__builtin_bit_cast(typename Vec8<T>::V, v[j])[i];
+        BlockScale s = all;
+        if (!TILE) {
+          Top<T> top;
+          top.add(v[j]);
+          s = block_scale<KIND>(max_over_16(top.bits()));
+        }
+        if (row + j < rows) {
+          *(i32x2*)(q + (long)(row + j) * pitch + col) = keep_upto(raw_to_fp8<T, KIND>(v[j], s), cols - col);
+          if (!TILE && c8 == 0)
+            store_scale<KIND>(scale, (long)(row + j) * scale_stride + bx, s.code);
+        }
       }
-      codes = to_fp8<KIND>(f, s);
-    } else {
-      // two rows of a column side by side, as the conversion takes them
-      const float by = e8m0_value(s.code);
-      int two[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        two[j] = (int)__builtin_amdgcn_perm((unsigned)v[2 * j + 1][i >> 1], (unsigned)v[2 * j][i >> 1],
-                                            i & 1 ? 0x07060302u : 0x05040100u);
-      codes[0] = two_codes<T, true>(two_codes<T, false>(0, two[0], by), two[1], by);
-      codes[1] = two_codes<T, true>(two_codes<T, false>(0, two[2], by), two[3], by);
     }
-    *(i32x2*)&bytes[c8 * 8 + i][(rg ^ c8) * 8] = keep_upto(codes, rows - row);
-  }
-  __syncthreads();
+    if (part) {
+      f32x8 s = unpack<T>(v[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = (t >> 3) + i * 32, at = t & 7, turn = c >> 3;
-    i32x4 two = *(const i32x4*)&bytes[c][(at ^ turn >> 1) * 16];
-    if (turn & 1) two = i32x4{two[2], two[3], two[0], two[1]};
-    if (c0 + c < cols) *(i32x4*)(qt + (long)(c0 + c) * pitch_t + r0 + at * 16) = two;
+      for (int j = 1; j < 8; ++j) s += unpack<T>(v[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) words[rg][c8 * 8 + i] = __float_as_uint(s[i]);
+      __syncthreads();
+      if (t < kQB && c0 + t < cols) {
+        float s = 0.f;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) s += __uint_as_float(words[g][t]);
+        part[(long)by * cols + c0 + t] = s;
+      }
+      __syncthreads();
+    }
+    if (qt) {
+      if (!TILE) {
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            unsigned m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j][i]));
+            words[rg][c8 * 8 + i] = m;
+          }
+        } else {
+          i32x4 m;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            Top<T> top;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top.add(v[j][i]);
+            m[i] = __builtin_bit_cast(int, top.m);
+          }
+          *(i32x4*)&words[rg][c8 * 4] = m;
+        }
+        __syncthreads();
+        if (t < kQB) {
+          unsigned m = 0;
+          if constexpr (WIDE) {
+#pragma unroll
+            for (int g = 0; g < 16; ++g) m = max(m, words[g][t]);
+          } else {
+#pragma unroll
+            for (int g = 0; g < 16; ++g) m = max(m, words[g][t >> 1] >> (16 * (t & 1)) & 0xffffu);
+            m = Top<T>::bits((unsigned short)m);
+          }
+          const BlockScale s = block_scale<KIND>(m);
+          col_code[t] = KIND == kE8M0 ? s.code : __float_as_uint(s.inv);
+          if (c0 + t < cols)
+            store_scale<KIND>(scale_t, (long)(c0 + t) * scale_t_stride + by, s.code);
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        BlockScale s = all;
+        if (!TILE) {
+          const unsigned c = col_code[c8 * 8 + i];
+          s.code = c;
+          s.inv = __uint_as_float(c);
+        }
+        i32x2 codes;
+        if constexpr (WIDE || KIND == kF32) {
+          f32x8 f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (WIDE) f[j] = v[j][i];
+            else f[j] = (float)__builtin_bit_cast(typename Vec8<T>::V, v[j])[i];
+          }
+          codes = to_fp8<KIND>(f, s);
+        } else {
+          // two rows of a column side by side, as the conversion takes them
+          const float scale_by = e8m0_value(s.code);
+          int two[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            two[j] = (int)__builtin_amdgcn_perm((unsigned)v[2 * j + 1][i >> 1], (unsigned)v[2 * j][i >> 1],
+                                                i & 1 ? 0x07060302u : 0x05040100u);
+          codes[0] = two_codes<T, true>(two_codes<T, false>(0, two[0], scale_by), two[1], scale_by);
+          codes[1] = two_codes<T, true>(two_codes<T, false>(0, two[2], scale_by), two[3], scale_by);
+        }
+        *(i32x2*)&bytes[c8 * 8 + i][(rg ^ c8) * 8] = keep_upto(codes, rows - row);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = (t >> 3) + i * 32, at = t & 7, turn = c >> 3;
+        i32x4 two = *(const i32x4*)&bytes[c][(at ^ turn >> 1) * 16];
+        if (turn & 1) two = i32x4{two[2], two[3], two[0], two[1]};
+        if (c0 + c < cols) *(i32x4*)(qt + (long)(c0 + c) * pitch_t + r0 + at * 16) = two;
+      }
+      __syncthreads();  // the bytes have been read
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = next[j];
   }
 }
 
@@ -231,7 +246,8 @@ extern "C" void al_quant_tile(int type, int kind, int tile, const void* x, long 
                               int rows, int cols, void* q, void* scale, int pitch,
                               int scale_stride, void* qt, void* scale_t, int pitch_t,
                               int scale_t_stride, float* part, hipStream_t stream) {
-  const dim3 grid((cols + kQB - 1) / kQB, (rows + kQB - 1) / kQB);
+  const int across = (cols + kQB - 1) / kQB, tiles = across * ((rows + kQB - 1) / kQB);
+  const dim3 grid(std::min(tiles, 1024));
   with_type(type, [&](auto* t) {
     with_kind(kind, [&](auto k) {
       typedef std::remove_pointer_t<decltype(t)> T;
@@ -239,7 +255,7 @@ extern "C" void al_quant_tile(int type, int kind, int tile, const void* x, long 
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const T*)x, row_stride, rows, cols,
                            (unsigned char*)q, scale, pitch, scale_stride, (unsigned char*)qt,
-                           scale_t, pitch_t, scale_t_stride, part);
+                           scale_t, pitch_t, scale_t_stride, part, across, tiles);
       };
       tile ? go(quant_tile_kernel<T, KIND, true>) : go(quant_tile_kernel<T, KIND, false>);
     });

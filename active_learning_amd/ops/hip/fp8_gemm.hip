@@ -41,6 +41,21 @@ AL_DEV void store_out(void* p, int type, long at, float v) {
   else ((_Float16*)p)[at] = (_Float16)v;
 }
 
+AL_DEV void store_four(void* p, int type, long at, f32x4 v, int left) {
+  if (left >= 4) {
+    if (type == kTypeF32) __builtin_memcpy((float*)p + at, &v, 16);
+    else if (type == kTypeBF16) {
+      const bf16x4v r = __builtin_convertvector(v, bf16x4v);
+      __builtin_memcpy((__bf16*)p + at, &r, 8);
+    } else {
+      const f16x4v r = __builtin_convertvector(v, f16x4v);
+      __builtin_memcpy((_Float16*)p + at, &r, 8);
+    }
+    return;
+  }
+  for (int e = 0; e < left; ++e) store_out(p, type, at + e, v[e]);
+}
+
 // eight codes times a power of two as bf16, which holds them exactly
 AL_DEV bf16x8v to_bf16(int lo, int hi, float scale) {
   const bf16x2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
@@ -81,14 +96,14 @@ template <int KIND> AL_DEV unsigned scale_code(const void* p, long at) {
 // as codes.
 template <typename T, bool EXACT, int KIND, bool BTILE, int MT, int NT, int WAVES>
 __launch_bounds__(WAVES * 64)
-__global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g) {
+__global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g, int across) {
   constexpr bool VALUES = !std::is_same<T, unsigned char>::value;
   constexpr bool HW = KIND == kE8M0 && !EXACT;  // the matrix instruction applies the scales
   static_assert(!VALUES || MT == 1, "values: one tile of rows");
   __shared__ f32x4 lds[WAVES][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l15 = lane & 15, l4 = lane >> 4;
-  const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+  const int n0 = blockIdx.x % across * (16 * NT), m0 = blockIdx.x / across * (16 * MT);
 
   // rows behind the last are the last one again; their outputs are not stored
   const unsigned char *a[MT], *b[NT];
@@ -96,13 +111,13 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const long m = min(m0 + i * 16 + l15, g.m - 1);
-    a[i] = VALUES ? (const unsigned char*)(x + m * x_stride + l4 * 32) : g.a + m * g.lda + l4 * 32;
+    a[i] = VALUES ? (const unsigned char*)(x + m * x_stride + l4 * 16) : g.a + m * g.lda + l4 * 16;
     sa[i] = m * g.sa_stride;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int n = min(n0 + j * 16 + l15, g.n - 1);
-    b[j] = g.b + (long)n * g.ldb + l4 * 32;
+    b[j] = g.b + (long)n * g.ldb + l4 * 16;
     sb[j] = (long)(BTILE ? n / kQB : n) * g.sb_stride;
   }
   f32x4 acc[MT][NT];
@@ -116,10 +131,14 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
     typename Raw8<typename std::conditional<VALUES, T, float>::type>::V v[VALUES ? 4 : 1];
     unsigned sa[MT], sb[NT];
   };
+  // A lane has 16 values of each half of the block, so that a load takes 64
+  // neighbouring bytes of a row: the order within a block is the same on both sides
+  // and means nothing to the sum.
   auto load32 = [](const unsigned char* p) {
-    const i32x4 lo = *(const i32x4*)p, hi = *(const i32x4*)(p + 16);
+    const i32x4 lo = *(const i32x4*)p, hi = *(const i32x4*)(p + 64);
     return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
+  auto place = [](int i) { return (i >> 1) * 64 + (i & 1) * 8; };  // of a lane's i-th eight
   auto load = [&](Raw& r, int kb) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -127,15 +146,15 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
       r.sb[j] = scale_code<KIND>(g.sb, sb[j] + kb);
     }
     if (VALUES) {
-      const int left = dim - kb * kQB - l4 * 32;
+      const int left = dim - kb * kQB - l4 * 16;
       const T* p = (const T*)a[0] + (long)kb * kQB;
       if constexpr (VALUES) {
         if ((kb + 1) * kQB <= dim) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) r.v[i] = raw8(p + i * 8);
+          for (int i = 0; i < 4; ++i) r.v[i] = raw8(p + place(i));
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) r.v[i] = raw8_upto(p + i * 8, left - i * 8);
+          for (int i = 0; i < 4; ++i) r.v[i] = raw8_upto(p + place(i), left - place(i));
         }
       }
     } else {
@@ -156,10 +175,10 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
       top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
       const BlockScale s = block_scale<KIND>(top);
       r.sa[0] = s.code;
-      const int left = dim - kb * kQB - l4 * 32;
+      const int left = dim - kb * kQB - l4 * 16;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const i32x2 codes = keep_upto(raw_to_fp8<T, KIND>(r.v[i], s), left - i * 8);
+        const i32x2 codes = keep_upto(raw_to_fp8<T, KIND>(r.v[i], s), left - place(i));
         r.a[0][2 * i] = codes[0];
         r.a[0][2 * i + 1] = codes[1];
       }
@@ -291,17 +310,14 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * 256, n0 = tn * 256;
 
-  // a split's steps begin at multiples of four, where its scales' words do
-  const int words = (g.blocks + 3) / 4;
-  const int first = (int)((long)words * blockIdx.y / g.splits) * 4;
-  const int steps = min((int)((long)words * (blockIdx.y + 1) / g.splits) * 4, g.blocks) - first;
+  const int steps = g.blocks;
 
   // A wave's load brings 8 rows of 128 bytes; the chunk that lands at slot s of row
   // r is s ^ (r >> 1 & 7). A read of 16 bytes a lane takes 16 lanes at a time, of
   // rows 0-3, 12-15, 20-23 and 24-27 first: this way they fall on different banks.
   const int rows_a = min(256, g.m - m0), rows_b = min(256, g.n - n0);
-  const Rsrc a = rsrc_of(g.a + (long)m0 * g.lda + (long)first * kQB, (long)rows_a * g.lda - (long)first * kQB);
-  const Rsrc b = rsrc_of(g.b + (long)n0 * g.ldb + (long)first * kQB, (long)rows_b * g.ldb - (long)first * kQB);
+  const Rsrc a = rsrc_of(g.a + (long)m0 * g.lda, (long)rows_a * g.lda);
+  const Rsrc b = rsrc_of(g.b + (long)n0 * g.ldb, (long)rows_b * g.ldb);
   // Rows behind the operand's last are the last one again, and no output of theirs is
   // stored.
   const int r = wid * 8 + (lane >> 3);  // and 64 rows on, and on
@@ -315,8 +331,8 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   const int scale_rows = wid < 4 ? rows_a : BTILE ? (rows_b + kQB - 1) / kQB : rows_b;
   const Rsrc scale = rsrc_of(
       (const unsigned char*)(wid < 4 ? g.sa : g.sb) +
-          (long)(wid < 4 ? m0 : BTILE ? n0 / kQB : n0) * scale_row + first / 4 * SB,
-      (long)scale_rows * scale_row - first / 4 * SB);
+          (long)(wid < 4 ? m0 : BTILE ? n0 / kQB : n0) * scale_row,
+      (long)scale_rows * scale_row);
   const unsigned off_s =
       (unsigned)min(BTILE && wid >= 4 ? sr / kQB : sr, scale_rows - 1) * (unsigned)scale_row;
 
@@ -507,10 +523,9 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 
   // Through LDS, so that rows are written in whole lines; 16-byte chunks again
   // spread over the banks by their row.
-  const bool split = g.splits > 1;
   float* bias = (float*)(smem + kRingS);  // the scales' place: 256 floats
   if (thread < 256)
-    bias[thread] = g.bias && !split && n0 + thread < g.n
+    bias[thread] = g.bias && n0 + thread < g.n
                             ? bias_at(g.bias, g.bias_type, n0 + thread) : 0.f;
   __syncthreads();
   auto each_four = [&](int h, auto put) __attribute__((always_inline)) {
@@ -529,7 +544,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
         }
       }
   };
-  if (!EXACT && !split) {
+  if (!EXACT) {
     const bool halves = g.out_type == kTypeF16;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -551,7 +566,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
     }
     return;
   }
-  float* out = (split ? g.split_out + (long)blockIdx.y * g.m * g.n : (float*)g.out) + (long)m0 * g.n + n0;
+  float* out = (float*)g.out + (long)m0 * g.n + n0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (h) __syncthreads();
@@ -567,6 +582,160 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
       if (left >= 4) __builtin_memcpy(to, from, 16);
       else
         for (int r = 0; r < left; ++r) to[r] = from[r];
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
+// 64x64 and 128x128 outputs a workgroup
+// --------------------------------------------------------------------------
+//
+// Between the two others: waves of WM x WN parts of a TM x TN tile share operands
+// through a ring of STAGES steps in LDS. Loads run STAGES - 1 steps ahead and one
+// barrier a step serves both ends of the ring: whoever passes it has its part of
+// this step's loads there and is done with the last step, whose place is then asked
+// for anew. The order of the 16-byte chunks within a block is the same on both
+// sides: a lane has chunks l4 and l4 + 4 of its row.
+template <int KIND, bool EXACT, bool BTILE, int TM, int TN, int WM, int WN, int STAGES>
+__launch_bounds__(WM * WN * 64)
+__global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
+  constexpr bool HW = KIND == kE8M0 && !EXACT;
+  constexpr int WAVES = WM * WN, MT = TM / WM / 16, NT = TN / WN / 16;
+  constexpr int LA = TM / 8 / WAVES, LB = TN / 8 / WAVES, SCALES = (TM + TN) / 64;
+  constexpr int LOADS = LA + LB + 1;  // of a wave in a step
+  constexpr int STAGE = (TM + TN) * (kQB + 4);
+  static_assert(LA * 8 * WAVES == TM && LB * 8 * WAVES == TN && SCALES <= WAVES, "whole loads");
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l15 = lane & 15, l4 = lane >> 4;
+  int tm, tn;
+  tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * TM, n0 = tn * TN;
+  const int first = (int)((long)g.blocks * blockIdx.y / g.splits);
+  const int steps = (int)((long)g.blocks * (blockIdx.y + 1) / g.splits) - first;
+
+  // Rows behind the operand's last are the last one again, and no output of theirs is
+  // stored. The chunk that lands at slot s of row r is s ^ (r & 7).
+  const int rows_a = min(TM, g.m - m0), rows_b = min(TN, g.n - n0);
+  const Rsrc a = rsrc_of(g.a + (long)m0 * g.lda + (long)first * kQB, (long)rows_a * g.lda - (long)first * kQB);
+  const Rsrc b = rsrc_of(g.b + (long)n0 * g.ldb + (long)first * kQB, (long)rows_b * g.ldb - (long)first * kQB);
+  const int r8 = lane >> 3;
+  const unsigned chunk = ((lane & 7) ^ r8) * 16;
+  unsigned off_a[LA], off_b[LB];
+#pragma unroll
+  for (int i = 0; i < LA; ++i)
+    off_a[i] = (unsigned)min((i * WAVES + wid) * 8 + r8, rows_a - 1) * (unsigned)g.lda + chunk;
+#pragma unroll
+  for (int i = 0; i < LB; ++i)
+    off_b[i] = (unsigned)min((i * WAVES + wid) * 8 + r8, rows_b - 1) * (unsigned)g.ldb + chunk;
+  // Each wave brings 64 rows' scales, some of them as another wave does too: all have
+  // the same loads in flight. e8m0: the word that holds the step's byte.
+  const int part = wid % SCALES;
+  const bool of_a = part * 64 < TM;
+  const int row = part * 64 + lane - (of_a ? 0 : TM);
+  const unsigned char* scale =
+      (const unsigned char*)(of_a ? g.sa : g.sb) +
+      (KIND == kE8M0 ? 1l : 4l) *
+          (of_a ? (long)min(m0 + row, g.m - 1) * g.sa_stride
+                : (long)(BTILE ? min(n0 + row, g.n - 1) / kQB : min(n0 + row, g.n - 1)) * g.sb_stride);
+  const int last = steps - 1;
+  auto load = [&](int k) __attribute__((always_inline)) {
+    unsigned char* to = smem + k % STAGES * STAGE;
+    const int at = min(k, last);  // behind the last step it again
+#pragma unroll
+    for (int i = 0; i < LA; ++i) lds_load<16>(a, off_a[i], at * kQB, to + (i * WAVES + wid) * 1024);
+#pragma unroll
+    for (int i = 0; i < LB; ++i) lds_load<16>(b, off_b[i], at * kQB, to + TM * kQB + (i * WAVES + wid) * 1024);
+    const unsigned char* p = scale + (KIND == kE8M0 ? (first + at) & ~3 : (first + at) * 4);
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
+                                     (__attribute__((address_space(3))) void*)(to + (TM + TN) * kQB + part * 256), 4,
+                                     0, 0);
+  };
+
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wm = wid / WN * (TM / WM), wn = wid % WN * (TN / WN);
+  const unsigned char* own = smem + l15 * kQB + ((l4 ^ (l15 & 7)) << 4);
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) load(k);
+  for (int k = 0; k < steps; ++k) {
+    wait_but<LOADS * (STAGES - 2)>();
+    phase_barrier();
+    load(k + STAGES - 1);
+    const int place = k % STAGES * STAGE;
+    auto fragment = [&](int r) __attribute__((always_inline)) {
+      const unsigned char* p = own + place + r * kQB;
+      // chunk l4 + 4 lies where bit 6 is turned over
+      const i32x4 lo = *(const i32x4*)p, hi = *(const i32x4*)(smem + ((unsigned)(p - smem) ^ 64u));
+      return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto scale_of = [&](int r) __attribute__((always_inline)) {
+      const unsigned w = *(const unsigned*)(smem + place + (TM + TN) * kQB + r * 4);
+      return KIND == kE8M0 ? w >> (((first + k) & 3) * 8) & 255u : w;
+    };
+    i32x8 fa[MT], fb[NT];
+    unsigned sa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      fa[i] = fragment(wm + i * 16);
+      sa[i] = scale_of(wm + i * 16 + l15);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fb[j] = fragment(TM + wn + j * 16);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if (KIND == kE8M0) {
+        const unsigned sb = scale_of(TM + wn + j * 16 + l15);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (HW) {
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0, (int)sb, 0,
+                                                                        (int)sa[i]);
+          } else {
+            const float x = __uint_as_float(sa[i] << 23), y = __uint_as_float(sb << 23);
+#pragma unroll
+            for (int q = 0; q < 8; q += 2)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(fb[j][q], fb[j][q + 1], y),
+                                                                  to_bf16(fa[i][q], fa[i][q + 1], x), acc[i][j], 0, 0, 0);
+          }
+        }
+      } else {
+        f32x4 sb;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sb[e] = __uint_as_float(scale_of(TM + wn + j * 16 + (BTILE ? 0 : l4 * 4 + e)));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const f32x4 d = block_product<EXACT>(fb[j], fa[i]);
+          const float x = __uint_as_float(sa[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], x * sb[e], acc[i][j][e]);
+        }
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing lands in LDS after the end
+  const bool split = g.splits > 1;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = m0 + wm + i * 16 + l15;
+    if (m >= g.m) continue;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int n = n0 + wn + j * 16 + l4 * 4;
+      f32x4 v = acc[i][j];
+      if (split) {
+        float* to = g.split_out + ((long)blockIdx.y * g.m + m) * g.n + n;
+        if (n + 4 <= g.n) __builtin_memcpy(to, &v, 16);
+        else
+          for (int e = 0; e < g.n - n; ++e) to[e] = v[e];
+        continue;
+      }
+      if (g.bias)
+        for (int e = 0; e < 4; ++e) v[e] += n + e < g.n ? bias_at(g.bias, g.bias_type, n + e) : 0.f;
+      store_four(g.out, g.out_type, (long)m * g.n + n, v, g.n - n);
     }
   }
 }
@@ -594,61 +763,97 @@ template <typename F> void with_kind(int kind, F f) {
 
 }  // namespace
 
-// Whether the direct kernel's 64x64 tiles are taken: where few workgroups of 256x256
-// outputs would run, fewer than half the chip even with the contraction split; and
-// for 32-bit results with 32-bit scales, which the large tile has no registers for.
-static bool direct_tiles(int kind, int out_type, int m, int n, int blocks) {
-  const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
-  return (kind == kF32 && out_type == kTypeF32) ||
-         tiles * std::max(1, std::min(blocks / 8, 16)) < 128;
+// Which kernel computes a product, by how many workgroups its tiles would make (all
+// figures in us, on 256 compute units, for 16-bit results unless said otherwise):
+//   32x32 direct while each unit has one and a wave has few blocks: 256x1000x2048 7.4
+//     against 8.9 of 64x64, but 64x64x8192 22 against 9.9 of 64x64 in eight parts;
+//   64x64 while each unit has two: 1024x1000x2048 9.7 against 16 of 32x32 and 13 of
+//     128x128; 512x4096x4096 19 against 24;
+//   128x128 in four stages while each has one, in two (which fit twice) while each has
+//     two and tiles are short: 2048x2048x8192 47 against 54 of 256x256, 8192x1000x2048
+//     23 against 25, but 3000x3000x5120 76 against 50;
+//   128x256 for 32-bit results, while each has one: 4096x2048x8192 121 against 139; and
+//     wherever their scales have 32 bits too, for which 256x256 has no registers;
+//   256x256 for the rest: 8192x8192x8192 386 against 575 of 128x128.
+enum Tile { kDirect32, kMid64, kMid128Deep, kMid128, kMid128x256, kBig };
+static Tile tile_for(int kind, int out_type, int m, int n, int blocks) {
+  const bool exact = out_type == kTypeF32;
+  auto groups = [&](int tm, int tn) { return (long)((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
+  if (groups(32, 32) <= 256 && blocks <= 16) return kDirect32;
+  if (groups(64, 64) <= 512) return kMid64;
+  if (groups(128, 128) <= 256) return kMid128Deep;
+  if (exact && (kind == kF32 || groups(128, 256) <= 256)) return kMid128x256;
+  if (!exact && groups(128, 128) <= 512 && blocks <= 16) return kMid128;
+  return kBig;
 }
 
 // How many parts the contraction is split into; the caller gives that many [m][n]
-// matrices of floats where there are more than one.
+// matrices of floats where there are more than one. Only 64x64 tiles are split, to
+// one workgroup a unit and eight steps each: 500x500x8192 26 us in one part, 14 in
+// four; 32x8192x8192 27 and, in two, 19.
 extern "C" int al_fp8_gemm_splits(int kind, int out_type, int m, int n, int blocks) {
-  if (direct_tiles(kind, out_type, m, n, blocks)) return 1;
-  const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256);
-  int s = (int)std::min((long)blocks / 8, 256 / std::max(tiles, 1l));
-  return std::max(1, std::min(s, 16));
+  if (tile_for(kind, out_type, m, n, blocks) != kMid64) return 1;
+  const long tiles = (long)((m + 63) / 64) * ((n + 63) / 64);
+  return (int)std::max(1l, std::min({(long)blocks / 8, 256 / std::max(tiles, 1l), 8l}));
+}
+
+// a launch with more than 64 KB of LDS, which is asked for once on each device
+template <auto KERNEL>
+static void launch_lds(int groups, int splits, int threads, int bytes, hipStream_t stream, Gemm g, int tiles_m,
+                       int tiles_n) {
+  static bool allowed[64];
+  int device = 0;
+  (void)hipGetDevice(&device);
+  if (!allowed[device & 63]) {
+    (void)hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    allowed[device & 63] = true;
+  }
+  hipLaunchKernelGGL(KERNEL, dim3(groups, splits), dim3(threads), bytes, stream, g, tiles_m, tiles_n);
+}
+
+template <int KIND, bool EXACT, bool BTILE, int TM, int TN, int WM, int WN, int STAGES>
+static void launch_mid(const Gemm& g, hipStream_t stream) {
+  const int down = (g.m + TM - 1) / TM, across = (g.n + TN - 1) / TN;
+  launch_lds<gemm_mid_kernel<KIND, EXACT, BTILE, TM, TN, WM, WN, STAGES>>(
+      down * across, g.splits, WM * WN * 64, STAGES * (TM + TN) * (kQB + 4), stream, g, down, across);
+}
+
+template <int KIND, bool EXACT, bool BTILE>
+static void gemm(Tile tile, const Gemm& g, hipStream_t stream) {
+  auto across = [&](int t) { return (g.n + t - 1) / t; };
+  auto down = [&](int t) { return (g.m + t - 1) / t; };
+  if (tile == kDirect32) {
+    hipLaunchKernelGGL((direct_kernel<unsigned char, EXACT, KIND, BTILE, 2, 2, 4>), dim3(across(32) * down(32)),
+                       dim3(256), 0, stream, (const unsigned char*)nullptr, 0l, 0, g, across(32));
+  } else if (tile == kMid64) {
+    launch_mid<KIND, EXACT, BTILE, 64, 64, 2, 2, 4>(g, stream);
+  } else if (tile == kMid128Deep) {
+    launch_mid<KIND, EXACT, BTILE, 128, 128, 2, 4, 4>(g, stream);
+  }
+  if constexpr (EXACT) {
+    if (tile == kMid128x256) launch_mid<KIND, true, BTILE, 128, 256, 2, 4, 3>(g, stream);
+  } else {
+    if (tile == kMid128) launch_mid<KIND, false, BTILE, 128, 128, 2, 4, 2>(g, stream);
+  }
+  if constexpr (!(EXACT && KIND == kF32)) {
+    if (tile == kBig)
+      launch_lds<gemm256_kernel<KIND, EXACT, BTILE>>(
+          down(256) * across(256), 1, 512, kRingS + 2 * 512 * (KIND == kE8M0 ? 4 : 16), stream, g, down(256),
+          across(256));
+  }
 }
 
 extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, int sa_stride,
                             const void* b, const void* sb, long ldb, int sb_stride, int b_tile,
                             int m, int n, int blocks, const void* bias, int bias_type, void* out,
                             int out_type, float* split_out, int splits, hipStream_t stream) {
-  Gemm g = {(const unsigned char*)a, (const unsigned char*)b, sa, sb, lda, ldb, sa_stride,
-            sb_stride, m, n, blocks, b_tile, bias, bias_type, out, out_type, split_out, splits};
+  const Gemm g = {(const unsigned char*)a, (const unsigned char*)b, sa, sb, lda, ldb, sa_stride,
+                  sb_stride, m, n, blocks, b_tile, bias, bias_type, out, out_type, split_out, splits};
+  const Tile tile = tile_for(kind, out_type, m, n, blocks);
   with_kind(kind, [&](auto k) {
     constexpr int KIND = decltype(k)::value;
-    if (direct_tiles(kind, out_type, m, n, blocks)) {
-      auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((n + 63) / 64, (m + 63) / 64), dim3(256), 0, stream,
-                           (const unsigned char*)nullptr, 0l, 0, g);
-      };
-      typedef unsigned char C;
-      if (out_type == kTypeF32) b_tile ? go(direct_kernel<C, true, KIND, true, 4, 4, 4>) : go(direct_kernel<C, true, KIND, false, 4, 4, 4>);
-      else b_tile ? go(direct_kernel<C, false, KIND, true, 4, 4, 4>) : go(direct_kernel<C, false, KIND, false, 4, 4, 4>);
-      return;
-    }
-    const int tiles_m = (m + 255) / 256, tiles_n = (n + 255) / 256;
-    constexpr int bytes = kRingS + 2 * 512 * (KIND == kE8M0 ? 4 : 16);
-    auto go = [&](auto kernel) {
-      static bool allowed[64];  // by device: more than 64 KB of LDS is asked for once
-      int device = 0;
-      (void)hipGetDevice(&device);
-      if (!allowed[device & 63]) {
-        (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        allowed[device & 63] = true;
-      }
-      hipLaunchKernelGGL(kernel, dim3(tiles_m * tiles_n, splits), dim3(512), bytes, stream, g, tiles_m, tiles_n);
-    };
-    if constexpr (KIND == kE8M0) {
-      if (out_type == kTypeF32) {
-        b_tile ? go(gemm256_kernel<KIND, true, true>) : go(gemm256_kernel<KIND, true, false>);
-        return;
-      }
-    }
-    b_tile ? go(gemm256_kernel<KIND, false, true>) : go(gemm256_kernel<KIND, false, false>);
+    if (out_type == kTypeF32) b_tile ? gemm<KIND, true, true>(tile, g, stream) : gemm<KIND, true, false>(tile, g, stream);
+    else b_tile ? gemm<KIND, false, true>(tile, g, stream) : gemm<KIND, false, false>(tile, g, stream);
   });
   if (splits > 1) {
     const int join = (int)std::min(((long)m * n + 255) / 256, 2048l);
@@ -668,8 +873,8 @@ extern "C" void al_fp8_few_rows(int kind, int type, const void* x, long x_stride
       constexpr int KIND = decltype(k)::value;
       constexpr bool EXACT = std::is_same<T, float>::value;
       auto go = [&](auto kernel, int columns) {
-        hipLaunchKernelGGL(kernel, dim3((n + columns - 1) / columns), dim3(512), 0, stream,
-                           (const T*)x, x_stride, dim, g);
+        const int across = (n + columns - 1) / columns;
+        hipLaunchKernelGGL(kernel, dim3(across), dim3(512), 0, stream, (const T*)x, x_stride, dim, g, across);
       };
       // as many columns as still give each compute unit a workgroup: the more of
       // them share the quantisation of x the better

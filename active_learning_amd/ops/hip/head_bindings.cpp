@@ -281,7 +281,8 @@ std::vector<Tensor> fp8_quant_tile(const Tensor& x, long kind, bool tile, bool p
   check_rows(x, "input", x);
   c10::OptionalDeviceGuard guard(x.device());
   const long rows = x.size(0), cols = x.size(1);
-  TORCH_CHECK(rows <= kBlock * 65535, "input has too many rows");
+  TORCH_CHECK_VALUE(rows <= INT_MAX - kBlock && blocks_of(rows) * blocks_of(cols) <= INT_MAX - 1024,
+                    "a matrix of ", rows, " x ", cols, " is too large");
   Tensor none = torch::empty({0}, x.options().dtype(torch::kFloat32));
   Tensor q = none, scale = none, qt = none, scale_t = none, part, sum = none;
   if (plain) {
@@ -341,6 +342,8 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor
   TORCH_CHECK(a.device() == b.device(), "operands must be on one device");
   TORCH_CHECK(kind_of(sa) == kind_of(sb), "operands must have scales of one type");
   check_bias(bias, n, a);
+  // tiles are counted in 32 bits, and a launch has at most 2^32 threads
+  TORCH_CHECK_VALUE((m + 63) / 64 * ((n + 63) / 64) <= (1 << 23), "a product of ", m, " x ", n, " is too large");
   c10::OptionalDeviceGuard guard(a.device());
   Tensor out = torch::empty({m, n}, a.options().dtype(out_type));
   const int ot = type_of(out, "output"), blocks = (int)blocks_of(k);
