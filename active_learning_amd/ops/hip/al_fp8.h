@@ -203,15 +203,29 @@ AL_DEV i32x2 keep_upto(i32x2 codes, int left) {
                                        ((1ul << (left * 8)) - 1));
 }
 
-// maximum over the 16 lanes that hold one block's 128 values, eight each
-AL_DEV unsigned max_over_16(unsigned m) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-  return m;
+// A lane's partner for the reductions over 16 lanes: within pairs, pairs of pairs,
+// halves, and the whole. Once the groups below agree, a mirror reaches the other one.
+template <int STEP> AL_DEV int partner(int v) {
+  constexpr int kCtrl[4] = {0xb1, 0x4e, 0x141, 0x140};  // swap 1, swap 2, mirror 8, mirror 16
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl[STEP], 0xf, 0xf, true);
 }
-
-AL_DEV float wave_allsum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+template <int STEP> AL_DEV float partner(float v) { return __int_as_float(partner<STEP>(__float_as_int(v))); }
+template <int STEP> AL_DEV double partner(double v) {
+  return __hiloint2double(partner<STEP>(__double2hiint(v)), partner<STEP>(__double2loint(v)));
+}
+// over the 16 lanes that hold one block's 128 values, eight each
+AL_DEV unsigned max_over_16(unsigned m) {
+  m = max(m, (unsigned)partner<0>((int)m));
+  m = max(m, (unsigned)partner<1>((int)m));
+  m = max(m, (unsigned)partner<2>((int)m));
+  return max(m, (unsigned)partner<3>((int)m));
+}
+// the sum over a wave, in every lane
+template <typename F> AL_DEV F wave_total(F v) {
+  v += partner<0>(v);
+  v += partner<1>(v);
+  v += partner<2>(v);
+  v += partner<3>(v);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
 }

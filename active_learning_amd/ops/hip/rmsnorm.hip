@@ -7,8 +7,8 @@
 //   dw = sum over rows of dy * u
 //
 // The norm is that of the stored, rounded sum: the backward pass reads the same
-// numbers and differentiates what the forward pass computed. All arithmetic is
-// in 32 bits and rounded once, on the store.
+// numbers and differentiates what the forward pass computed. Arithmetic is in 32
+// bits or more, rounded to the type on the store.
 
 #include "al_fp8.h"
 
@@ -17,14 +17,14 @@ namespace {
 enum { kOutPlain = 0, kOutE8M0 = 1, kOutF32 = 2 };
 
 // sum over the TPR threads of a row; every thread gets it
-template <int TPR> AL_DEV float row_sum(float v, float* lds) {
-  v = wave_allsum(v);
+template <int TPR, typename F> AL_DEV F row_sum(F v, F* lds) {
+  v = wave_total(v);
   if (TPR == 64) return v;
   constexpr int W = TPR / 64;
   __syncthreads();  // the last row's sums have been read
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = 0.f;
+  F s = 0;
 #pragma unroll
   for (int i = 0; i < W; ++i) s += lds[i];
   return s;
@@ -35,8 +35,18 @@ constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 // One row per TPR threads, VPT vectors of eight values each, rows strided over
 // the grid so that the weight stays in registers. VPT == 0: rows of any length,
 // read twice.
+//
+// In front of an e4m3 output the sum is held in 64 bits, and 1 / root and the first
+// product as pairs of floats: y is then the exact value rounded once, and a value next
+// to a border between two codes or scales falls on its own side of it (with 32 bits throughout,
+// 50 codes in 123 million did not). At 130000x2048 in bf16 with a residual that costs
+// 355 us against 336, at 5.3 and 5.5 TB/s; the reductions go through lane permutations
+// of the vector unit (LDS shuffles: 187 us for 160 without a residual).
+//
+// One vector a thread: no more registers than let eight waves share a SIMD, as the
+// grid counts on (with seven the last eighth of the blocks runs alone: 426 us for 355).
 template <typename T, typename W, int TPR, int VPT, bool RES, int OUT>
-__launch_bounds__(block_of(TPR))
+__launch_bounds__(block_of(TPR), VPT == 1 ? 8 : 1)
 __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
                                const T* __restrict__ res, long res_stride,
                                const W* __restrict__ w, T* __restrict__ y,
@@ -44,7 +54,8 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
                                unsigned char* __restrict__ q, void* __restrict__ scale,
                                long rows, int dim, int pitch, int scale_stride,
                                float eps) {
-  __shared__ float lds[16];
+  typedef typename std::conditional<OUT == kOutPlain, float, double>::type Sum;
+  __shared__ Sum lds[16];
   constexpr int RPB = block_of(TPR) / TPR;
   constexpr int N = VPT ? VPT : 1;
   const int t = threadIdx.x % TPR;
@@ -54,12 +65,13 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
 #pragma unroll
     for (int i = 0; i < N; ++i) wv[i] = load8_upto(w + (i * TPR + t) * 8, dim - (i * TPR + t) * 8);
   }
+  const double per_value = 1.0 / (double)dim;
   const long first = (long)blockIdx.x * RPB;
   for (long r0 = first; r0 < rows; r0 += (long)gridDim.x * RPB) {
     const long r = r0 + threadIdx.x / TPR;
     if (RPB > 1 && r >= rows) break;  // whole waves; no barrier when RPB > 1
     f32x8 v[N];
-    float ss = 0.f;
+    Sum ss = 0;
     auto take = [&](int c) {
       f32x8 f = load8_upto(x + r * x_stride + c, dim - c);
       if (RES) {
@@ -74,11 +86,20 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
       for (int k = i; k < sweeps; k += N) {
         v[i] = take((k * TPR + t) * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+        for (int j = 0; j < 8; ++j) ss += (Sum)v[i][j] * (Sum)v[i][j];
       }
     }
     ss = row_sum<TPR>(ss, lds);
-    const float rstd = 1.f / sqrtf(ss / (float)dim + eps);
+    float rstd, rstd_low = 0.f;
+    if (OUT == kOutPlain) {
+      rstd = 1.f / sqrtf((float)ss / (float)dim + eps);
+    } else {  // the hardware's root has 23 bits; a step of Newton's method doubles them
+      const double mean = (double)ss * per_value + (double)eps;
+      double r = __builtin_amdgcn_rsq(mean);
+      r *= 1.5 - 0.5 * mean * r * r;
+      rstd = (float)r;
+      rstd_low = (float)(r - (double)rstd);
+    }
     if (rstd_out && t == 0) rstd_out[r] = rstd;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -92,14 +113,39 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
           f = RES ? load8_upto(total + r * dim + c, dim - c)
                   : load8_upto(x + r * x_stride + c, dim - c);
         }
-        f = f * rstd * ww;
         if (OUT == kOutPlain) {
+          f = f * rstd * ww;
           if (c < dim) store8_upto(y + r * dim + c, f, dim - c);
         } else {
           constexpr int KIND = OUT == kOutE8M0 ? kE8M0 : kF32;
-          const BlockScale b = block_scale<KIND>(max_over_16(amax8(f)));
+          // the exact value's nearest, and what the exact value is over it
+          auto product = [&](int j, float& over) {
+#pragma clang fp contract(off)
+            const float u = f[j] * rstd;
+            const float low = fmaf(f[j], rstd_low, fmaf(f[j], rstd, -u)) * ww[j];
+            const float nearest = fmaf(u, ww[j], low);
+            over = fmaf(u, ww[j], -nearest) + low;
+            return nearest;
+          };
+          f32x8 out;
+          float over;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) out[j] = product(j, over);
+          unsigned top = amax8(out);
+          // the largest value a block's scale can hold, by its nearest: a little more
+          // than that takes the next scale
+          if (KIND == kE8M0 && (top & 0x7fffffu) == 0x600000u) {
+            bool more = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float nearest = product(j, over);
+              more |= abs_bits(nearest) == top && (nearest > 0.f ? over > 0.f : over < 0.f);
+            }
+            top += more;
+          }
+          const BlockScale b = block_scale<KIND>(max_over_16(top));
           if (c < pitch) {
-            *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8<KIND>(f, b), dim - c);
+            *(i32x2*)(q + r * pitch + c) = keep_upto(to_fp8<KIND>(out, b), dim - c);
             if ((t & 15) == 0 && c < dim)
               store_scale<KIND>(scale, r * scale_stride + c / kQB, b.code);
           }
@@ -226,22 +272,29 @@ __global__ void col_sum_kernel(const float* __restrict__ part, W* __restrict__ o
 
 struct Shape { int tpr, vpt; };
 
-// The forward pass: the narrowest group of threads that holds a row in registers,
-// since a wave for each row needs no barrier; where that leaves compute units
-// without a workgroup, four waves. Beyond 32768 values a row is read twice.
-Shape fwd_shape(long rows, int dim) {
-  if (rows < 1024 && dim > 512 && dim <= 2048) return {256, 1};
+// The forward pass. Up to 1024 values a wave holds a row and needs no barrier, longer
+// rows are spread with one vector a thread, up to 32768 with a few: beyond that a row is
+// read twice. Measured on 266 million values in bf16, us with the residual / without:
+//   1024 values, plain:  64 threads x 2 vectors 462 / 189, x 4 (half of them idle, fewer
+//                        waves at once) 396 / 211; to e4m3, x 2, 355 / 183
+//   2048 values:         64 x 4 plain 384 / 206, to e4m3 411; 256 x 1 388 / 192, 355 / 160
+//   4096 values, plain:  256 x 2 460 / 191, 512 x 1 393 / 192
+//   8192 values, e4m3:   256 x 4 403 / 167, 1024 x 1 346 / 171; plain 388 / 209, 391 / 185
+// (their bytes at a copy's rate: plain 396 / 198, e4m3 346 / 148). The rule does not ask
+// for the number of rows, so a row's numbers do not depend on the rows beside it.
+Shape fwd_shape(int dim, bool res, int out) {
+  const bool plain = out == kOutPlain;
   if (dim <= 512) return {64, 1};
-  if (dim <= 1024) return {64, 2};
-  if (dim <= 2048) return {64, 4};
-  if (dim <= 4096) return {256, 2};
-  if (dim <= 8192) return {256, 4};
+  if (dim <= 1024) return {64, res && plain ? 4 : 2};
+  if (dim <= 2048) return {256, 1};
+  if (dim <= 4096) return {512, 1};
+  if (dim <= 8192) return {1024, 1};
   if (dim <= 16384) return {1024, 2};
   if (dim <= 32768) return {1024, 4};
   return {1024, 0};
 }
 // The backward pass holds four times as much for each value: one vector a thread.
-Shape bwd_shape(long, int dim) {
+Shape bwd_shape(int dim) {
   if (dim <= 512) return {64, 1};
   if (dim <= 2048) return {256, 1};
   if (dim <= 4096) return {512, 1};
@@ -251,14 +304,14 @@ Shape bwd_shape(long, int dim) {
 }
 
 template <int N> using Int = std::integral_constant<int, N>;
-template <typename F> void with_fwd_shape(long rows, int dim, F f) {
-  const Shape s = fwd_shape(rows, dim);
+template <typename F> void with_fwd_shape(Shape s, F f) {
   if (s.tpr == 64) s.vpt == 1 ? f(Int<64>{}, Int<1>{}) : s.vpt == 2 ? f(Int<64>{}, Int<2>{}) : f(Int<64>{}, Int<4>{});
-  else if (s.tpr == 256) s.vpt == 1 ? f(Int<256>{}, Int<1>{}) : s.vpt == 2 ? f(Int<256>{}, Int<2>{}) : f(Int<256>{}, Int<4>{});
-  else s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : s.vpt == 4 ? f(Int<1024>{}, Int<4>{}) : f(Int<1024>{}, Int<0>{});
+  else if (s.tpr == 256) f(Int<256>{}, Int<1>{});
+  else if (s.tpr == 512) f(Int<512>{}, Int<1>{});
+  else s.vpt == 1 ? f(Int<1024>{}, Int<1>{}) : s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : s.vpt == 4 ? f(Int<1024>{}, Int<4>{}) : f(Int<1024>{}, Int<0>{});
 }
-template <typename F> void with_bwd_shape(long rows, int dim, F f) {
-  const Shape s = bwd_shape(rows, dim);
+template <typename F> void with_bwd_shape(int dim, F f) {
+  const Shape s = bwd_shape(dim);
   if (s.tpr == 64) f(Int<64>{}, Int<1>{});
   else if (s.tpr == 256) f(Int<256>{}, Int<1>{});
   else if (s.tpr == 512) f(Int<512>{}, Int<1>{});
@@ -274,8 +327,9 @@ template <typename T, typename W>
 void fwd(const void* x, long x_stride, const void* res, long res_stride, const void* w,
          void* y, void* total, float* rstd, void* q, void* scale, int out, long rows,
          int dim, int pitch, int scale_stride, float eps, hipStream_t stream) {
-  const int blocks = blocks_for(fwd_shape(rows, dim), rows, 2048);
-  with_fwd_shape(rows, dim, [&](auto tpr, auto vpt) {
+  const Shape shape = fwd_shape(dim, res != nullptr, out);
+  const int blocks = blocks_for(shape, rows, 2048);
+  with_fwd_shape(shape, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(blocks), dim3(block_of(TPR)), 0, stream, (const T*)x,
@@ -292,7 +346,7 @@ template <typename T, typename W>
 void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const void* w,
          const float* rstd, void* dx, float* part, void* dw, int parts, long rows, int dim,
          hipStream_t stream) {
-  with_bwd_shape(rows, dim, [&](auto tpr, auto vpt) {
+  with_bwd_shape(dim, [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(parts), dim3(block_of(TPR)), TPR < 256 ? dim * 4 : 0,
@@ -332,7 +386,7 @@ extern "C" void al_rms_fwd(int type, int wtype, const void* x, long x_stride,
 
 // how many partial rows of dw the backward pass writes
 extern "C" int al_rms_bwd_parts(long rows, int dim) {
-  return blocks_for(bwd_shape(rows, dim), rows, 1024);
+  return blocks_for(bwd_shape(dim), rows, 1024);
 }
 
 extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,

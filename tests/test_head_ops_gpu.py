@@ -126,6 +126,29 @@ def test_rms_norm_fp8(rows, dim, residual, dtype, kind):
     assert not q._codes[:, dim:].float().any()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,dim,residual", [(3000, 96, False), (700, 777, True), (1500, 1000, True), (1500, 2000, False),
+                                               (700, 4096, True), (300, 8000, False), (150, 12000, True),
+                                               (80, 32768, True), (60, 40000, True)])
+def test_rms_norm_fp8_codes_are_those_of_64_bits(rows, dim, residual, dtype):
+    # y is the 64-bit value rounded once to 32 bits, so a code or a scale may differ from the
+    # 64-bit one's only where a change of U32 moves that over a border (twice it: the borders
+    # themselves are computed through 32 bits here)
+    x, w, r = _norm_inputs(rows, dim, TYPES[dtype], residual, torch.float32)
+    out = rms_norm_fp8(x, w, residual=r, eps=1e-5)
+    out = out[0] if residual else out
+    want = _norm_64(x, w, r, 1e-5)[2]
+    grid = torch.nn.functional.pad(want, (0, -dim % 128)).view(rows, -1, 128)
+    scale = out.scale.double()
+    top = grid.abs().amax(2)
+    assert (scale >= torch.exp2((top * (1 - 2 * U32) / 448).log2().ceil())).all()
+    assert (scale <= torch.exp2((top * (1 + 2 * U32) / 448).log2().ceil())).all()
+    a = (grid / scale[..., None]).view(rows, -1)[:, :dim]
+    ends = [(a * f).float().clamp(-448, 448).to(torch.float8_e4m3fn).float() for f in (1 - 2 * U32, 1 + 2 * U32)]
+    got = out.values.float()
+    assert (got >= torch.minimum(*ends)).all() and (got <= torch.maximum(*ends)).all()
+
+
 def test_rms_norm_strided_rows_and_leading_axes():
     big = randn(40, 300, dtype=torch.bfloat16)
     w = randn(100, seed=9)
