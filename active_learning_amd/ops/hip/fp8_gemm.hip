@@ -772,8 +772,9 @@ template <typename F> void with_kind(int kind, F f) {
 //   128x128 in four stages while each has one, in two (which fit twice) while each has
 //     two and tiles are short: 2048x2048x8192 47 against 54 of 256x256, 8192x1000x2048
 //     23 against 25, but 3000x3000x5120 76 against 50;
-//   128x256 for 32-bit results, while each has one: 4096x2048x8192 121 against 139; and
-//     wherever their scales have 32 bits too, for which 256x256 has no registers;
+//   128x256 while each has one, for 32-bit results, 4096x2048x8192 121 against 139, and
+//     for 32-bit scales, 2500x2500x8192 81 against 96 (with e8m0 256x256 is as fast: 70
+//     and 67); and wherever both have 32 bits, for which 256x256 has no registers;
 //   256x256 for the rest: 8192x8192x8192 386 against 575 of 128x128.
 enum Tile { kDirect32, kMid64, kMid128Deep, kMid128, kMid128x256, kBig };
 static Tile tile_for(int kind, int out_type, int m, int n, int blocks) {
@@ -782,8 +783,9 @@ static Tile tile_for(int kind, int out_type, int m, int n, int blocks) {
   if (groups(32, 32) <= 256 && blocks <= 16) return kDirect32;
   if (groups(64, 64) <= 512) return kMid64;
   if (groups(128, 128) <= 256) return kMid128Deep;
-  if (exact && (kind == kF32 || groups(128, 256) <= 256)) return kMid128x256;
+  if (exact && kind == kF32) return kMid128x256;
   if (!exact && groups(128, 128) <= 512 && blocks <= 16) return kMid128;
+  if ((exact || kind == kF32) && groups(128, 256) <= 256) return kMid128x256;
   return kBig;
 }
 
@@ -830,9 +832,10 @@ static void gemm(Tile tile, const Gemm& g, hipStream_t stream) {
   } else if (tile == kMid128Deep) {
     launch_mid<KIND, EXACT, BTILE, 128, 128, 2, 4, 4>(g, stream);
   }
-  if constexpr (EXACT) {
-    if (tile == kMid128x256) launch_mid<KIND, true, BTILE, 128, 256, 2, 4, 3>(g, stream);
-  } else {
+  if constexpr (EXACT || KIND == kF32) {
+    if (tile == kMid128x256) launch_mid<KIND, EXACT, BTILE, 128, 256, 2, 4, 3>(g, stream);
+  }
+  if constexpr (!EXACT) {
     if (tile == kMid128) launch_mid<KIND, false, BTILE, 128, 128, 2, 4, 2>(g, stream);
   }
   if constexpr (!(EXACT && KIND == kF32)) {
