@@ -151,6 +151,8 @@ def _quantize_cpu(x, kind, tile):
     inverse = torch.where(bad, torch.tensor(float("nan")), inverse)
     scaled = (grid * inverse[:, None, :, None]).reshape(up, across)[:rows, :cols]
     values = scaled.clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
+    if cols == 0:  # the transpose of no rows
+        return Fp8Blocks._of(values, scale, x.shape, tile)
     return Fp8Blocks(values, scale, tile)
 
 

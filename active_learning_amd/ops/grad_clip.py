@@ -35,16 +35,17 @@ def _distinct(tensors):
 def _norm_factor(grads, max_norm):
     """Norm and factor of gradients on the CPU."""
     norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
-    factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+    factor = (torch.ones_like(norm) if max_norm == float("inf")
+              else (max_norm / (norm + 1e-6)).clamp(max=1.0))
     return torch.stack([norm, factor]).float()
 
 
-def _params_norm_factor(params, max_norm, max_dev=None):
-    """Two floats on the device of the parameters' gradients, or None where there
-    are no gradients."""
+def _params_norm_factor(params, max_norm, max_dev=None, to=None):
+    """Two floats on the device of the parameters' gradients (GPU: in ``to`` where it
+    is given), or None where there are no gradients."""
     on_gpu = next((p.is_cuda for p in params if p.grad is not None), None)
     if on_gpu:
-        return require_extension().params_norm_factor(params, max_norm, max_dev)
+        return require_extension().params_norm_factor(params, max_norm, max_dev, to)
     if on_gpu is None:
         return None
     return _norm_factor(_distinct(p.grad for p in params), max_norm)
@@ -68,8 +69,8 @@ def clip_grad_norm_(parameters, max_norm):
     ``max_norm``, and returns the norm they had.
 
     A NaN makes all gradients NaN; an infinity makes the factor zero, so that it
-    becomes NaN itself and everything else zero. Gradients that share memory are
-    refused.
+    becomes NaN itself and everything else zero; an infinite ``max_norm`` leaves
+    everything as it is. Gradients that share memory are refused.
     """
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = float(max_norm)
@@ -82,6 +83,11 @@ def clip_grad_norm_(parameters, max_norm):
         if both.is_cuda:
             require_extension().scale_grads(parameters, both)
         else:
-            for g in _distinct(p.grad for p in parameters):
+            grads = _distinct(p.grad for p in parameters)
+            spans = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size())
+                           for g in grads if g.is_contiguous() and g.numel())
+            if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+                raise RuntimeError("gradients that share memory cannot be scaled in place")
+            for g in grads:
                 g.mul_(both[1])
     return both[0]

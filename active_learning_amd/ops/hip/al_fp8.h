@@ -102,11 +102,6 @@ template <int KIND> AL_DEV void store_scale(void* p, long at, unsigned code) {
   if (KIND == kE8M0) ((unsigned char*)p)[at] = (unsigned char)code;
   else ((unsigned*)p)[at] = code;
 }
-template <int KIND> AL_DEV float load_scale(const void* p, long at) {
-  if (KIND == kF32) return ((const float*)p)[at];
-  const unsigned c = ((const unsigned char*)p)[at];
-  return __uint_as_float(c == 255u ? 0x7fc00000u : c << 23);
-}
 
 // Eight values as they are in memory, and the work on them that needs no unpacking:
 // 16-bit magnitudes are compared as whole numbers, two at a time, and the conversion

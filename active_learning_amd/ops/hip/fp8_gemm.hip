@@ -22,7 +22,6 @@ struct Gemm {
   long lda, ldb;              // bytes from row to row, 128 for each block
   int sa_stride, sb_stride;   // scales from row to row
   int m, n, blocks;           // blocks: of 128 along the contraction
-  int b_tile;                 // b's scales are those of 128x128 tiles
   const void* bias;
   int bias_type;
   void* out;
@@ -851,7 +850,7 @@ extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, i
                             int m, int n, int blocks, const void* bias, int bias_type, void* out,
                             int out_type, float* split_out, int splits, hipStream_t stream) {
   const Gemm g = {(const unsigned char*)a, (const unsigned char*)b, sa, sb, lda, ldb, sa_stride,
-                  sb_stride, m, n, blocks, b_tile, bias, bias_type, out, out_type, split_out, splits};
+                  sb_stride, m, n, blocks, bias, bias_type, out, out_type, split_out, splits};
   const Tile tile = tile_for(kind, out_type, m, n, blocks);
   with_kind(kind, [&](auto k) {
     constexpr int KIND = decltype(k)::value;
@@ -869,7 +868,7 @@ extern "C" void al_fp8_few_rows(int kind, int type, const void* x, long x_stride
                                 int m, int n, int blocks, const void* bias, int bias_type,
                                 void* out, hipStream_t stream) {
   Gemm g = {nullptr, (const unsigned char*)b, nullptr, sb, 0, ldb, 0, sb_stride, m, n, blocks,
-            b_tile, bias, bias_type, out, type, nullptr, 1};
+            bias, bias_type, out, type, nullptr, 1};
   with_type(type, [&](auto* t) {
     with_kind(kind, [&](auto k) {
       typedef std::remove_pointer_t<decltype(t)> T;

@@ -120,11 +120,16 @@ void check_norm(const Tensor& x, const Tensor& w, const OptTensor& res, double e
     TORCH_CHECK_VALUE(value(res).device() == x.device(), "residual is on ", value(res).device(),
                       ", the input on ", x.device());
   }
-  TORCH_CHECK_VALUE(eps > 0, "eps must be positive, got ", eps);
+  TORCH_CHECK_VALUE((float)eps > 0, "eps must be positive, got ", eps);
 }
 
 // (rows, last axis) with a dense last axis; a view wherever there is one
 Tensor as_rows(const Tensor& t) {
+  if (!t.numel()) {  // what is empty counts as dense, whatever its strides
+    long rows = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+    return torch::empty({rows, t.size(-1)}, t.options());
+  }
   if (t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1)) return t;
   const Tensor r = t.reshape({-1, t.size(-1)});
   return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
@@ -150,12 +155,13 @@ struct NormOut {
   Tensor y, total, rstd;
 };
 
-// rows of a checked input; rstd only where it is asked for
-NormOut norm_rows(const Tensor& x, const Tensor& w, const OptTensor& res, double eps, bool need_rstd) {
+// rows of a checked input, as outputs of the given shape; rstd only where it is asked for
+NormOut norm_rows(const Tensor& x, const Tensor& w, const OptTensor& res, double eps, bool need_rstd,
+                  torch::IntArrayRef shape) {
   const long rows = x.size(0), dim = x.size(1);
   NormOut o;
-  o.y = torch::empty({rows, dim}, x.options());
-  o.total = res ? torch::empty({rows, dim}, x.options()) : x;
+  o.y = torch::empty(shape, x.options());
+  if (res) o.total = torch::empty(shape, x.options());
   if (need_rstd) o.rstd = torch::empty({rows}, x.options().dtype(torch::kFloat32));
   if (rows) {
     al_rms_fwd(type_of(x, "input"), type_of(w, "weight"), x.data_ptr(), row_stride(x),
@@ -190,17 +196,19 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
                                                 const Tensor& w, const OptTensor& res, double eps) {
     ctx->set_materialize_grads(false);
     c10::OptionalDeviceGuard guard(x.device());
-    const NormOut o = norm_rows(as_rows(x), w, res ? OptTensor(as_rows(*res)) : res, eps, true);
-    ctx->save_for_backward({o.total, w, o.rstd});
+    const Tensor rows = as_rows(x);
+    const NormOut o = norm_rows(rows, w, res ? OptTensor(as_rows(*res)) : res, eps, true, x.sizes());
+    // the sum as it goes out, not a view of it: a change in place is noticed
+    ctx->save_for_backward({res ? o.total : rows, w, o.rstd});
     ctx->saved_data["residual"] = res.has_value();
-    if (!res) return {o.y.view(x.sizes())};
-    return {o.y.view(x.sizes()), o.total.view(x.sizes())};
+    if (!res) return {o.y};
+    return {o.y, o.total};
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &total = saved[0], &w = saved[1], &rstd = saved[2];
+    const Tensor total = as_rows(saved[0]), &w = saved[1], &rstd = saved[2];
     const bool res = ctx->saved_data["residual"].toBool();
     const bool need_w = ctx->needs_input_grad(1);
     Tensor dy = grads[0], dsum = res ? grads[1] : Tensor();
@@ -228,9 +236,9 @@ std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& w_in, const OptTenso
   if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || (res && wants_grad(*res))))
     return RmsNorm::apply(x, w, res, eps);
   c10::OptionalDeviceGuard guard(x.device());
-  const NormOut o = norm_rows(as_rows(x), w, res ? OptTensor(as_rows(*res)) : res, eps, false);
-  if (!res) return {o.y.view(x.sizes())};
-  return {o.y.view(x.sizes()), o.total.view(x.sizes())};
+  const NormOut o = norm_rows(as_rows(x), w, res ? OptTensor(as_rows(*res)) : res, eps, false, x.sizes());
+  if (!res) return {o.y};
+  return {o.y, o.total};
 }
 
 // (codes, scales, stored sum)
@@ -335,8 +343,11 @@ void check_bias(const OptTensor& bias, long n, const Tensor& like) {
               "bias must be a dense vector of one value for each output column, on the operands' device");
 }
 
-Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool b_tile,
-                long m, long n, long k, const OptTensor& bias, torch::ScalarType out_type) {
+// [m, n], or that in the given shape: outputs of a differentiable function are no
+// views, so that they may be changed in place
+Tensor fp8_gemm_as(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool b_tile,
+                   long m, long n, long k, const OptTensor& bias, torch::ScalarType out_type,
+                   torch::IntArrayRef shape) {
   check_codes(a, sa, m, k, false, "left operand's");
   check_codes(b, sb, n, k, b_tile, "right operand's");
   TORCH_CHECK(a.device() == b.device(), "operands must be on one device");
@@ -345,9 +356,14 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor
   // tiles are counted in 32 bits, and a launch has at most 2^32 threads
   TORCH_CHECK_VALUE((m + 63) / 64 * ((n + 63) / 64) <= (1 << 23), "a product of ", m, " x ", n, " is too large");
   c10::OptionalDeviceGuard guard(a.device());
-  Tensor out = torch::empty({m, n}, a.options().dtype(out_type));
+  Tensor out = torch::empty(shape, a.options().dtype(out_type));
   const int ot = type_of(out, "output"), blocks = (int)blocks_of(k);
   if (!m || !n) return out;
+  if (!k) {  // sums of nothing
+    out.zero_();
+    if (bias) out.view({m, n}).add_(value(bias));
+    return out;
+  }
   const int splits = al_fp8_gemm_splits(kind_of(sa), ot, (int)m, (int)n, blocks);
   Tensor split;
   if (splits > 1) split = torch::empty({splits, m, n}, a.options().dtype(torch::kFloat32));
@@ -357,6 +373,10 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor
               out.data_ptr(), ot, splits > 1 ? split.data_ptr<float>() : nullptr, splits, cur_stream());
   check_launch("fp8_matmul");
   return out;
+}
+Tensor fp8_gemm(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, bool b_tile,
+                long m, long n, long k, const OptTensor& bias, torch::ScalarType out_type) {
+  return fp8_gemm_as(a, sa, b, sb, b_tile, m, n, k, bias, out_type, {m, n});
 }
 
 // x [m <= 16, k] in its own type times the blocks of b
@@ -370,6 +390,7 @@ Tensor fp8_few_rows(const Tensor& x, const Tensor& b, const Tensor& sb, bool b_t
   check_bias(bias, n, x);
   c10::OptionalDeviceGuard guard(x.device());
   Tensor out = torch::empty({m, n}, x.options());
+  TORCH_CHECK_VALUE(k > 0, "x needs a last axis of at least one value");
   if (!m || !n) return out;
   al_fp8_few_rows(kind_of(sb), type, x.data_ptr(), row_stride(x), (int)k, b.data_ptr(), sb.data_ptr(),
                   b.size(1), (int)sb.size(1), b_tile, (int)m, (int)n, (int)blocks_of(k),
@@ -398,7 +419,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     ctx->saved_data["bias"] = bias ? (int64_t)value(bias).scalar_type() : -1;
     auto shape = x.sizes().vec();
     shape.back() = n;
-    return fp8_gemm(xq[0], xq[1], wq[0], wq[1], true, m, n, k, bias, x.scalar_type()).view(shape);
+    return fp8_gemm_as(xq[0], xq[1], wq[0], wq[1], true, m, n, k, bias, x.scalar_type(), shape);
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
@@ -509,8 +530,10 @@ std::vector<Tensor> grads_of(const std::vector<Tensor>& params) {
   return distinct(grads);
 }
 
-// [norm, factor] of distinct tensors; max_dev, where given, holds the bound on the device
-Tensor norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptTensor& max_dev) {
+// [norm, factor] of distinct tensors, in `to` where it is given; max_dev, where given,
+// holds the bound on the device
+Tensor norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptTensor& max_dev,
+                   const OptTensor& to) {
   const Tensor& first = grads[0];
   c10::OptionalDeviceGuard guard(first.device());
   Batches all;
@@ -526,7 +549,10 @@ Tensor norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptT
   int parts = 0;
   for (auto& b : all.batch) parts += al_norm_blocks(b.data());
   Tensor part = torch::empty({std::max(parts, 1)}, first.options().dtype(torch::kFloat64));
-  Tensor out = torch::empty({2}, first.options().dtype(torch::kFloat32));
+  if (to)
+    TORCH_CHECK(value(to).device() == first.device() && value(to).numel() == 2 && value(to).is_contiguous() &&
+                    value(to).scalar_type() == torch::kFloat32, "norm and factor");
+  Tensor out = to ? value(to) : torch::empty({2}, first.options().dtype(torch::kFloat32));
   int at = 0;
   for (size_t i = 0; i < all.batch.size(); ++i) {
     al_sq_sum(all.type[i], all.batch[i].data(), part.data_ptr<double>() + at, cur_stream());
@@ -539,11 +565,12 @@ Tensor norm_factor(const std::vector<Tensor>& grads, double max_norm, const OptT
 }
 
 Tensor grad_norm_factor(const std::vector<Tensor>& tensors, double max_norm, const OptTensor& max_dev) {
-  return norm_factor(distinct(tensors), max_norm, max_dev);
+  return norm_factor(distinct(tensors), max_norm, max_dev, std::nullopt);
 }
 
-Tensor params_norm_factor(const std::vector<Tensor>& params, double max_norm, const OptTensor& max_dev) {
-  return norm_factor(grads_of(params), max_norm, max_dev);
+Tensor params_norm_factor(const std::vector<Tensor>& params, double max_norm, const OptTensor& max_dev,
+                          const OptTensor& to) {
+  return norm_factor(grads_of(params), max_norm, max_dev, to);
 }
 
 // the parameters' gradients times the factor, in place

@@ -284,7 +284,8 @@ __global__ void norm_factor_kernel(const double* __restrict__ part, int parts, f
   __syncthreads();
   if (threadIdx.x == 0) {
     const double norm = sqrt(lds[0] + lds[1] + lds[2] + lds[3]);
-    const double f = (double)(max_dev ? *max_dev : max_norm) / (norm + 1e-6);
+    const float bound = max_dev ? *max_dev : max_norm;
+    const double f = isinf(bound) ? 1.0 : (double)bound / (norm + 1e-6);  // none: no look at the norm
     out[0] = (float)norm;
     out[1] = f < 1.0 ? (float)f : f >= 1.0 ? 1.f : __builtin_nanf("");
   }

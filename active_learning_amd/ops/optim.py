@@ -67,6 +67,8 @@ class FusedSGD(torch.optim.Optimizer):
         self.max_grad_norm = _check_max_norm(max_grad_norm)
         self.last_grad_norm = None
         self._clip_dev = None    # device max_grad_norm; graph-capture mode
+        self._clip_to = None
+        self._captured_plain = False  # a step without max_grad_norm was captured
 
     def enable_persistent_grads(self):
         """Persistent-grad mode for hipGraph capture: the caller must NOT call
@@ -91,22 +93,29 @@ class FusedSGD(torch.optim.Optimizer):
         if tuple(self._hyper_host.tolist()) != vals:
             self._hyper_host.copy_(torch.tensor(vals))
             self._hyper_dev.copy_(self._hyper_host, non_blocking=True)
-        if self.max_grad_norm is not None:
-            if self._clip_dev is None:
-                self._clip_dev = torch.full((1,), float(self.max_grad_norm),
-                                            device=self._hyper_dev.device)
-                self._clip_host = self.max_grad_norm
-            elif self._clip_host != self.max_grad_norm:
-                self._clip_dev.fill_(float(self.max_grad_norm))
-                self._clip_host = self.max_grad_norm
+        bound = self.max_grad_norm
+        if bound is not None and self._captured_plain:
+            raise ValueError("the step was captured without max_grad_norm: set it before the "
+                             "capture")
+        if bound is not None and self._clip_dev is None:
+            self._clip_dev = torch.full((1,), float(bound), device=self._hyper_dev.device)
+            # where captured and eager steps alike leave the norm and the factor
+            self._clip_to = torch.zeros(2, device=self._hyper_dev.device)
+            self._clip_host = bound
+        elif self._clip_dev is not None and self._clip_host != bound:
+            # a captured step goes on to look at the bound: none is an infinite one
+            self._clip_dev.fill_(float("inf") if bound is None else float(bound))
+            self._clip_host = bound
 
     def _clip(self):
         """(norm, factor) of this step's gradients on their device; None without
         max_grad_norm or gradients."""
         if self.max_grad_norm is None:
+            if self._hyper_dev is not None and torch.cuda.is_current_stream_capturing():
+                self._captured_plain = True
             return None
         both = _params_norm_factor(_all_params(self), float(self.max_grad_norm),
-                                   self._clip_dev)
+                                   self._clip_dev, self._clip_to)
         if both is not None:
             self.last_grad_norm = both[0]
         return both

@@ -41,38 +41,25 @@ def _check(x, weight, residual, eps):
                              f"{tuple(x.shape)} {x.dtype}")
         if residual.device != x.device:
             raise ValueError(f"residual is on {residual.device}, the input on {x.device}")
-    if not eps > 0:
+    if not torch.tensor(eps, dtype=torch.float32) > 0:
         raise ValueError(f"eps must be positive, got {eps}")
-
-
-def _rows(t):
-    """(rows, last axis) with a dense last axis; a view wherever there is one."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _forward_cpu(x, weight, residual, eps):
     total = x if residual is None else (x.float() + residual.float()).to(x.dtype)
     s = total.float()
     rstd = 1.0 / torch.sqrt(s.square().mean(-1, keepdim=True) + eps)
-    return s * rstd * weight.float(), total, rstd[..., 0]
+    return s * rstd * weight.float(), total, rstd
 
 
 class _RMSNormCPU(Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.set_materialize_grads(False)
-        shape = x.shape
-        x = _rows(x)
-        if residual is not None:
-            residual = _rows(residual)
-        weight = weight.contiguous()
         y, total, rstd = _forward_cpu(x, weight, residual, eps)
-        y = y.to(x.dtype)
         ctx.save_for_backward(total, weight, rstd)
-        if residual is None:
-            return y.view(shape)
-        return y.view(shape), total.view(shape)
+        y = y.to(x.dtype)
+        return y if residual is None else (y, total)
 
     @staticmethod
     @once_differentiable
@@ -82,17 +69,13 @@ class _RMSNormCPU(Function):
         if dy is None:  # only the sum was used
             dw = torch.zeros_like(weight) if need_w else None
             return dsum if need_x else None, dw, dsum if need_r else None, None
-        shape = dy.shape
-        dy = dy.reshape(total.shape)
-        if dsum is not None:
-            dsum = dsum.reshape(total.shape)
-        u = total.float() * rstd[:, None]
+        u = total.float() * rstd
         g = dy.float() * weight.float()
-        dx = (g - u * (g * u).mean(-1, keepdim=True)) * rstd[:, None]
+        dx = (g - u * (g * u).mean(-1, keepdim=True)) * rstd
         if dsum is not None:
             dx = dx + dsum.float()
-        dx = dx.to(total.dtype).view(shape)
-        dw = (dy.float() * u).sum(0).to(weight.dtype)
+        dx = dx.to(total.dtype)
+        dw = (dy.float() * u).reshape(-1, u.shape[-1]).sum(0).to(weight.dtype)
         return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
 
 
@@ -128,13 +111,9 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
             t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to "
                            "train, or torch.no_grad()")
-    shape = x.shape
-    x = _rows(x)
-    if residual is not None:
-        residual = _rows(residual)
     y, total, _ = _forward_cpu(x, weight, residual, eps)
-    blocks = quantize_fp8(y, scale=scale)
-    return blocks if residual is None else (blocks, total.view(shape))
+    blocks = quantize_fp8(y.reshape(-1, y.shape[-1]), scale=scale)
+    return blocks if residual is None else (blocks, total)
 
 
 class RMSNorm(nn.Module):

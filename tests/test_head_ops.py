@@ -333,3 +333,48 @@ def test_head_step_from_norm_to_clipped_update():
     (a, na), (b, nb) = train(), train()
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(na, nb)
     assert all(torch.isfinite(p).all() for p in a) and na > 0
+
+
+def test_outputs_may_be_changed_in_place():
+    x = torch.randn(2, 3, 64, requires_grad=True)
+    w = torch.nn.Parameter(torch.randn(64))
+    y = rms_norm(x, w)
+    y.mul_(2)
+    y.sum().backward()
+    want = torch.autograd.grad((rms_norm(x, w) * 2).sum(), (x, w))
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+    y, total = rms_norm(x, w, residual=x.detach())
+    total.add_(1)  # the backward pass needs it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("eps", [0.0, -1.0, 1e-46, float("nan")])
+def test_eps_that_32_bits_do_not_hold(eps):
+    with pytest.raises(ValueError, match="eps must be positive"):
+        rms_norm(torch.zeros(1, 8), torch.ones(8), eps=eps)
+
+
+def test_clip_refuses_shared_memory_and_leaves_all_without_a_bound():
+    both = torch.randn(6)
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(4))
+    p.grad, q.grad = both[:4], both[2:]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_([p, q], 0.1)
+    p.grad, q.grad = torch.full((4,), float("inf")), torch.ones(4)
+    assert clip_grad_norm_([p, q], float("inf")) == float("inf")
+    assert torch.equal(q.grad, torch.ones(4))
+
+
+def test_no_rows_and_no_outputs():
+    x, w = torch.zeros(3, 0, 256, requires_grad=True), torch.ones(256, requires_grad=True)
+    weight = torch.randn(40, 256, requires_grad=True)
+    y, total = rms_norm(x, w, residual=x.detach())
+    z = fp8_linear(y, weight)
+    assert z.shape == (3, 0, 40) and total.shape == x.shape
+    grads = torch.autograd.grad(z.sum(), (x, w, weight))
+    assert all((g == 0).all() for g in grads)
+    x = torch.randn(5, 256, requires_grad=True)
+    z = fp8_linear(x, weight[:0])
+    (dx,) = torch.autograd.grad(z.sum(), x)
+    assert z.shape == (5, 0) and (dx == 0).all()

@@ -600,6 +600,114 @@ def test_captured_training_step_matches_eager():
     assert all(torch.equal(a, b) for a, b in zip(eager[0], graphed[0]))
 
 
+def test_captured_step_among_eager_ones():
+    """Steps of another batch size run eagerly between replays: the norm is always the
+    last step's, no bound is an infinite one, and a bound comes too late for a step that
+    was captured without."""
+    from active_learning_amd.ops.graph import GraphedTrainStep
+    from active_learning_amd.ops.loss import CrossEntropyLoss
+    dev = torch.device("cuda", torch.cuda.current_device())
+    sizes = [64, 64, 64, 40, 64, 40, 64, 64]
+    xs = [randn(n, 512, seed=s) for s, n in enumerate(sizes)]
+
+    def run(warmup, bound):
+        net = _head(1)
+        opt = FusedSGD(net.parameters(), lr=0.1, momentum=0.9, max_grad_norm=bound)
+        step = GraphedTrainStep(net, opt, CrossEntropyLoss().to(dev), dev, warmup=warmup)
+        norms = []
+        for i, x in enumerate(xs):
+            if i == 6 and bound is not None:
+                opt.max_grad_norm = None
+            step.step(x, torch.arange(len(x), device="cuda") % 10)
+            if bound is not None:
+                if i < 6:
+                    norms.append(opt.last_grad_norm.item())
+        torch.cuda.synchronize()
+        return [p.detach().clone() for p in net.parameters()], norms, step, opt
+
+    eager, graphed = run(100, 0.2), run(2, 0.2)
+    assert eager[2]._graph is None and graphed[2]._graph is not None
+    assert eager[1] == graphed[1] and len(set(eager[1])) == 6
+    assert all(torch.equal(a, b) for a, b in zip(eager[0], graphed[0]))
+    _, _, step, opt = run(2, None)
+    opt.max_grad_norm = 0.1
+    with pytest.raises(ValueError, match="captured without max_grad_norm"):
+        step.step(xs[0], torch.arange(64, device="cuda") % 10)
+
+
+def test_outputs_may_be_changed_in_place():
+    x, w = randn(2, 3, 200, seed=1).requires_grad_(), randn(200, seed=2).requires_grad_()
+    weight = randn(24, 200, seed=3).requires_grad_()
+    for f in (lambda: rms_norm(x, w), lambda: fp8_linear(x, weight)):
+        leaves = [t for t in (x, w, weight) if t is not (weight if f() .shape[-1] == 200 else w)]
+        want = torch.autograd.grad(torch.relu(f()).sum(), leaves)
+        y = f()
+        got = torch.autograd.grad(torch.nn.functional.relu(y, inplace=True).sum(), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, total = rms_norm(x, w, residual=x.detach())
+    total.add_(1)  # the backward pass needs it
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    x2 = x.detach().requires_grad_()
+    y = fp8_linear(x2 * 1, weight)
+    y.sum().backward(retain_graph=True)
+    first = x2.grad.clone()
+    y.sum().backward()
+    assert torch.equal(x2.grad, 2 * first)
+
+
+def test_no_outputs():
+    x, weight = randn(70, 300, seed=1).requires_grad_(), torch.zeros(0, 300, device="cuda", requires_grad=True)
+    y = fp8_linear(x, weight)
+    dx, dw = torch.autograd.grad(y.sum(), (x, weight))
+    assert y.shape == (70, 0) and dw.shape == weight.shape and dx.shape == x.shape and (dx == 0).all()
+
+
+@pytest.mark.parametrize("shape", [(0, 256), (3, 0, 256), (256,)])
+def test_no_rows_and_single_vectors(shape):
+    x = randn(*shape, dtype=torch.bfloat16).requires_grad_()
+    w = randn(256, seed=1).requires_grad_()
+    weight, bias = randn(40, 256, seed=2).requires_grad_(), randn(40, seed=3).requires_grad_()
+    y, total = rms_norm(x, w, residual=x.detach())
+    z = fp8_linear(y, weight, bias)
+    assert y.shape == total.shape == shape and z.shape == (*shape[:-1], 40)
+    grads = torch.autograd.grad(z.float().sum(), (x, w, weight, bias))
+    assert [g.shape for g in grads] == [x.shape, w.shape, weight.shape, bias.shape]
+    if x.numel() == 0:
+        assert all((g == 0).all() for g in grads)
+    with torch.no_grad():
+        blocks = quantize_fp8(weight, tile=True)
+        assert fp8_linear(x, blocks, bias).shape == z.shape
+        q = rms_norm_fp8(x, w)
+        assert q.shape == (x.numel() // 256, 256)
+        assert fp8_matmul(q, blocks).shape == (x.numel() // 256, 40)
+        assert quantize_fp8(weight[:0], tile=True).shape == (0, 256)
+
+
+def test_same_tensor_twice_and_broadcast_operands():
+    x, w = randn(70, 300, seed=1).requires_grad_(), randn(300, seed=2)
+    y, total = rms_norm(x, w, residual=x)
+    (got,) = torch.autograd.grad((y, total), x, (y.detach(), total.detach()))
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    y, total = rms_norm(a, w, residual=b)
+    ga, gb = torch.autograd.grad((y, total), (a, b), (y.detach(), total.detach()))
+    assert torch.equal(got, ga + gb)
+    row = randn(1, 300, seed=3).requires_grad_()
+    weight = randn(1, 300, seed=4).requires_grad_()
+    bias = randn(1, seed=5).requires_grad_()
+    args = (row.expand(64, 300), weight.expand(32, 300), bias.expand(32))
+    z = fp8_linear(*args)
+    assert (z == z[0, 0]).all()
+    dz = randn(64, 32, seed=6)
+    got = torch.autograd.grad(z, (row, weight, bias), dz)
+    full = [t.detach().clone().requires_grad_() for t in args]
+    each = torch.autograd.grad(fp8_linear(*full), full, dz)
+    # 32-bit sums of at most 64 terms in another order
+    for g, e in zip(got, each):
+        within(g, e.double().sum(0, keepdim=g.dim() > 1).reshape(g.shape),
+               64 * U32 * e.double().abs().sum(0).reshape(g.shape))
+
+
 def test_side_stream():
     x, w = randn(300, 2048, dtype=torch.bfloat16), quantize_fp8(randn(500, 2048, seed=1), tile=True)
     want = fp8_linear(x, w)
