@@ -206,7 +206,8 @@ extern "C" void al_adam_step(float* p, const float* g, float* m, float* v, float
 // a captured launch keeps its own. Squares are summed in 64 bits, so that neither
 // large nor tiny values leave the range, first by thread, then by block, then
 // over the blocks' partial sums, each in a fixed order. Bound by one read of the
-// gradients.
+// gradients: 301 tensors of 400 million floats together in 286 us, 5.6 TB/s, and as
+// bf16 in 148. Four vectors in flight a thread instead of one: 284 and 151.
 
 constexpr int kNormTensors = 160;  // 24 bytes each: the arguments stay under 4 KB
 constexpr int kNormChunk = 16384;  // values a block takes at a time
@@ -244,16 +245,6 @@ __global__ void sq_sum_kernel(NormBatch b, double* __restrict__ part) {
     int n;
     const T* p = norm_chunk<T>(b, c, n);
     int i = threadIdx.x * 8;
-    // four vectors in flight: at one the loads' latency is the bound (4.3 TB/s)
-    for (; i + 3 * 256 * 8 + 8 <= n; i += 4 * 256 * 8) {
-      f32x8 f[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) f[u] = load8(p + i + u * 256 * 8);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s += (double)f[u][j] * (double)f[u][j];
-    }
     for (; i + 8 <= n; i += 256 * 8) {
       const f32x8 f = load8(p + i);
 #pragma unroll
@@ -308,7 +299,9 @@ __global__ void scale_kernel(NormBatch b, const float* __restrict__ norm_factor)
 
 // The multi-tensor SGD step with clipped gradients: the factor is applied as the
 // gradient is read, which costs no pass of its own, and p.grad keeps its values.
-// Four blocks share a table row, so that a small network fills the chip.
+// Bound by memory: 20 bytes a value with momentum. Norm and step over 301 tensors of
+// 400 million floats take 1.87 ms, 24 bytes a value at 5.1 TB/s. Four blocks share a
+// table row, so that a small network fills the chip.
 constexpr int kSgdSub = 4;
 template <bool ZG>
 __launch_bounds__(256)

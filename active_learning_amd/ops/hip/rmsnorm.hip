@@ -96,7 +96,7 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
     } else {  // the hardware's root has 23 bits; a step of Newton's method doubles them
       const double mean = (double)ss * per_value + (double)eps;
       double r = __builtin_amdgcn_rsq(mean);
-      r *= 1.5 - 0.5 * mean * r * r;
+      if (!isinf(mean)) r *= 1.5 - 0.5 * mean * r * r;
       rstd = (float)r;
       rstd_low = (float)(r - (double)rstd);
     }

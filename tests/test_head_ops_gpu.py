@@ -149,6 +149,19 @@ def test_rms_norm_fp8_codes_are_those_of_64_bits(rows, dim, residual, dtype):
     assert (got >= torch.minimum(*ends)).all() and (got <= torch.maximum(*ends)).all()
 
 
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rms_norm_fp8_not_finite_as_on_the_cpu(residual, kind):
+    # an infinity leaves zeros beside its block and NaN in it, a NaN its whole row NaN
+    x = torch.ones(4, 300)
+    x[0, 5], x[1, 299], x[2, 130] = float("inf"), float("-inf"), float("nan")
+    w, r = torch.ones(300), torch.ones(4, 300) if residual else None
+    want = rms_norm_fp8(x, w, residual=r, scale=kind)
+    got = rms_norm_fp8(x.cuda(), w.cuda(), residual=None if r is None else r.cuda(), scale=kind)
+    want, got = (want[0], got[0]) if residual else (want, got)
+    same_blocks(got, want)
+
+
 def test_rms_norm_strided_rows_and_leading_axes():
     big = randn(40, 300, dtype=torch.bfloat16)
     w = randn(100, seed=9)
