@@ -705,12 +705,14 @@ __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
         f32x4 sb;
 #pragma unroll
         for (int e = 0; e < 4; ++e) sb[e] = __uint_as_float(scale_of(TM + wn + j * 16 + (BTILE ? 0 : l4 * 4 + e)));
+        f32x4 d[MT];  // all before the first is used: 2500x2500x8192 77 us, one by one 81
+#pragma unroll
+        for (int i = 0; i < MT; ++i) d[i] = block_product<EXACT>(fb[j], fa[i]);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const f32x4 d = block_product<EXACT>(fb[j], fa[i]);
           const float x = __uint_as_float(sa[i]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], x * sb[e], acc[i][j][e]);
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[i][e], x * sb[e], acc[i][j][e]);
         }
       }
     }
@@ -772,7 +774,7 @@ template <typename F> void with_kind(int kind, F f) {
 //     two and tiles are short: 2048x2048x8192 47 against 54 of 256x256, 8192x1000x2048
 //     23 against 25, but 3000x3000x5120 76 against 50;
 //   128x256 while each has one, for 32-bit results, 4096x2048x8192 121 against 139, and
-//     for 32-bit scales, 2500x2500x8192 81 against 96 (with e8m0 256x256 is as fast: 70
+//     for 32-bit scales, 2500x2500x8192 77 against 96 (with e8m0 256x256 is as fast: 70
 //     and 67); and wherever both have 32 bits, for which 256x256 has no registers;
 //   256x256 for the rest: 8192x8192x8192 386 against 575 of 128x128.
 enum Tile { kDirect32, kMid64, kMid128Deep, kMid128, kMid128x256, kBig };
