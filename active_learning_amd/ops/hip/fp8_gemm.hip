@@ -26,6 +26,7 @@ struct Gemm {
   int bias_type;
   void* out;
   int out_type;
+  int ldo;                    // values from row to row of the result
   float* split_out;           // partial sums [split][m][n] where the contraction is split
   int splits;
 };
@@ -233,7 +234,7 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
     for (int e = 0; e < 4; ++e) {
       const int n = n0 + j * 16 + l4 * 4 + e;
       if (n < g.n)
-        store_out(g.out, g.out_type, (long)m * g.n + n,
+        store_out(g.out, g.out_type, (long)m * g.ldo + n,
                   v[e] + (g.bias ? bias_at(g.bias, g.bias_type, n) : 0.f));
     }
   }
@@ -439,21 +440,25 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
         }
     } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        f32x16 d[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f32x16 d;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) d[r] = 0.f;
+          for (int r = 0; r < 16; ++r) d[i][r] = 0.f;
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][half], fa[i][half], d, 0, 0, 0, 0, 0, 0);
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            d[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][half], fa[i][half], d[i], 0, 0, 0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int by = BTILE ? sb[j] : scale_of(256 + wc * 64 + j * 32 + (r >> 2) * 8 + l5 * 4 + (r & 3), k, s);
-            c[i][j][r] = fmaf(d[r], __int_as_float(sa[i]) * __int_as_float(by), c[i][j][r]);
+            c[i][j][r] = fmaf(d[i][r], __int_as_float(sa[i]) * __int_as_float(by), c[i][j][r]);
           }
-        }
+      }
     }
     __builtin_amdgcn_s_setprio(0);
   };
@@ -555,17 +560,17 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
     __syncthreads();
     const int c = thread & 31, left = g.n - n0 - c * 8;
     const int high = left > 0 ? min(256, g.m - m0) : 0;
-    short* out = (short*)g.out + (long)m0 * g.n + n0 + c * 8;
+    short* out = (short*)g.out + (long)m0 * g.ldo + n0 + c * 8;
     for (int m = thread >> 5; m < high; m += 16) {
       const s16x8 v = *(const s16x8*)(smem + m * 512 + ((c ^ (m & 31)) << 4));
-      short* to = out + (long)m * g.n;
+      short* to = out + (long)m * g.ldo;
       if (left >= 8) __builtin_memcpy(to, &v, 16);
       else
         for (int r = 0; r < left; ++r) to[r] = *(const short*)(smem + m * 512 + ((c ^ (m & 31)) << 4) + r * 2);
     }
     return;
   }
-  float* out = (float*)g.out + (long)m0 * g.n + n0;
+  float* out = (float*)g.out + (long)m0 * g.ldo + n0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (h) __syncthreads();
@@ -577,7 +582,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
     const int high = left > 0 ? min(128, g.m - m0 - h * 128) : 0;
     for (int m = thread >> 6; m < high; m += 8) {
       const float* from = (const float*)(smem + m * 1024 + ((c ^ (m & 31)) << 4));
-      float* to = out + (long)(h * 128 + m) * g.n + c * 4;
+      float* to = out + (long)(h * 128 + m) * g.ldo + c * 4;
       if (left >= 4) __builtin_memcpy(to, from, 16);
       else
         for (int r = 0; r < left; ++r) to[r] = from[r];
@@ -736,7 +741,7 @@ __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
       }
       if (g.bias)
         for (int e = 0; e < 4; ++e) v[e] += n + e < g.n ? bias_at(g.bias, g.bias_type, n + e) : 0.f;
-      store_four(g.out, g.out_type, (long)m * g.n + n, v, g.n - n);
+      store_four(g.out, g.out_type, (long)m * g.ldo + n, v, g.n - n);
     }
   }
 }
@@ -788,6 +793,19 @@ static Tile tile_for(int kind, int out_type, int m, int n, int blocks) {
   if (!exact && groups(128, 128) <= 512 && blocks <= 16) return kMid128;
   if ((exact || kind == kF32) && groups(128, 256) <= 256) return kMid128x256;
   return kBig;
+}
+
+// How many columns 256x256 tiles take where their last round on the 256 units would be
+// the shorter part of one: whole rounds, if smaller tiles compute the rest in less than
+// the round that it saves (a half with 128x128, three quarters with 128x256), and a
+// round is long enough for another launch. 4096x4452x4096 87 us in one launch, 71 in
+// two; 8192x4608x8192 252 and 235; with 32-bit scales 114 and 84, 330 and 289.
+static int columns_of_rounds(int kind, int out_type, int m, int n, int blocks) {
+  const int down = (m + 255) / 256, rounds = (int)((long)down * ((n + 255) / 256) / 256);
+  const int columns = rounds * 256 / down * 256;
+  if (blocks < 16 || columns == 0 || columns >= n) return n;
+  const Tile rest = tile_for(kind, out_type, m, n - columns, blocks);
+  return rest == kBig || rest == kMid128 ? n : columns;
 }
 
 // How many parts the contraction is split into; the caller gives that many [m][n]
@@ -852,13 +870,28 @@ extern "C" void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, i
                             int m, int n, int blocks, const void* bias, int bias_type, void* out,
                             int out_type, float* split_out, int splits, hipStream_t stream) {
   const Gemm g = {(const unsigned char*)a, (const unsigned char*)b, sa, sb, lda, ldb, sa_stride,
-                  sb_stride, m, n, blocks, bias, bias_type, out, out_type, split_out, splits};
-  const Tile tile = tile_for(kind, out_type, m, n, blocks);
-  with_kind(kind, [&](auto k) {
-    constexpr int KIND = decltype(k)::value;
-    if (out_type == kTypeF32) b_tile ? gemm<KIND, true, true>(tile, g, stream) : gemm<KIND, true, false>(tile, g, stream);
-    else b_tile ? gemm<KIND, false, true>(tile, g, stream) : gemm<KIND, false, false>(tile, g, stream);
-  });
+                  sb_stride, m, n, blocks, bias, bias_type, out, out_type, n, split_out, splits};
+  auto run = [&](const Gemm& g) {
+    const Tile tile = tile_for(kind, out_type, g.m, g.n, blocks);
+    with_kind(kind, [&](auto k) {
+      constexpr int KIND = decltype(k)::value;
+      if (out_type == kTypeF32) b_tile ? gemm<KIND, true, true>(tile, g, stream) : gemm<KIND, true, false>(tile, g, stream);
+      else b_tile ? gemm<KIND, false, true>(tile, g, stream) : gemm<KIND, false, false>(tile, g, stream);
+    });
+  };
+  const int columns = tile_for(kind, out_type, m, n, blocks) == kBig ? columns_of_rounds(kind, out_type, m, n, blocks) : n;
+  Gemm part = g;
+  part.n = columns;
+  run(part);
+  if (columns < n) {  // a multiple of 256
+    const int bytes = out_type == kTypeF32 ? 4 : 2;
+    part.n = n - columns;
+    part.b = g.b + (long)columns * ldb;
+    part.sb = (const unsigned char*)sb + (long)(b_tile ? columns / kQB : columns) * sb_stride * (kind == kE8M0 ? 1 : 4);
+    part.out = (unsigned char*)out + (long)columns * bytes;
+    if (bias) part.bias = (const unsigned char*)bias + (long)columns * (bias_type == kTypeF32 ? 4 : 2);
+    run(part);
+  }
   if (splits > 1) {
     const int join = (int)std::min(((long)m * n + 255) / 256, 2048l);
     hipLaunchKernelGGL(gemm_join_kernel, dim3(join), dim3(256), 0, stream, g);
@@ -870,7 +903,7 @@ extern "C" void al_fp8_few_rows(int kind, int type, const void* x, long x_stride
                                 int m, int n, int blocks, const void* bias, int bias_type,
                                 void* out, hipStream_t stream) {
   Gemm g = {nullptr, (const unsigned char*)b, nullptr, sb, 0, ldb, 0, sb_stride, m, n, blocks,
-            bias, bias_type, out, type, nullptr, 1};
+            bias, bias_type, out, type, n, nullptr, 1};
   with_type(type, [&](auto* t) {
     with_kind(kind, [&](auto k) {
       typedef std::remove_pointer_t<decltype(t)> T;

@@ -800,7 +800,8 @@ def test_no_second_gradient(what):
 @pytest.mark.parametrize("m,n,k", [(4096, 4608, 100), (4097, 4500, 256), (4200, 4352, 384), (8000, 2300, 512),
                                    (2100, 9000, 640), (5000, 4100, 1100), (300, 33000, 900), (2048, 2048, 2176),
                                    (700, 900, 300), (2100, 1500, 700), (4000, 2000, 500), (2500, 3000, 900),
-                                   (70, 500, 4200), (2100, 1500, 3), (1000, 2000, 3900), (2500, 2501, 2100)])
+                                   (70, 500, 4200), (2100, 1500, 3), (1000, 2000, 3900), (2500, 2501, 2100),
+                                   (4096, 4452, 2100), (4000, 4797, 2050), (4099, 5003, 2100)])
 def test_matmul_many_tiles(m, n, k, kind):
     x, w = randn(m, k, seed=1), randn(n, k, seed=2)
     bias = randn(n, seed=3)
