@@ -23,7 +23,7 @@ void al_rms_fwd(int type, int wtype, const void* x, long x_stride, const void* r
                 long res_stride, const void* w, void* y, void* total, float* rstd, void* q,
                 void* scale, int out, long rows, int dim, int pitch, int scale_stride, float eps,
                 void* stream);
-int al_rms_bwd_parts(long rows, int dim);
+int al_rms_bwd_parts(int type, long rows, int dim);
 void al_rms_bwd(int type, int wtype, const void* s, long s_stride, const void* dy,
                 const void* dsum, const void* w, const float* rstd, void* dx, float* part,
                 void* dw, int parts, long rows, int dim, void* stream);
@@ -181,7 +181,7 @@ std::pair<Tensor, Tensor> norm_rows_bwd(const Tensor& s, const Tensor& w, const 
   Tensor dx = torch::empty({rows, dim}, s.options()), dw, part;
   if (need_dw) dw = rows ? torch::empty({dim}, w.options()) : torch::zeros({dim}, w.options());
   if (!rows) return {dx, dw};
-  const int parts = al_rms_bwd_parts(rows, (int)dim);
+  const int parts = al_rms_bwd_parts(type_of(s, "input"), rows, (int)dim);
   if (need_dw) part = torch::empty({parts, dim}, s.options().dtype(torch::kFloat32));
   al_rms_bwd(type_of(s, "input"), type_of(w, "weight"), s.data_ptr(), row_stride(s), dy.data_ptr(),
              dsum.defined() ? dsum.data_ptr() : nullptr, w.data_ptr(), rstd.data_ptr<float>(),

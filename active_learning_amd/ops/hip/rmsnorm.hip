@@ -293,9 +293,16 @@ Shape fwd_shape(int dim, bool res, int out) {
   if (dim <= 32768) return {1024, 4};
   return {1024, 0};
 }
-// The backward pass holds four times as much for each value: one vector a thread.
-Shape bwd_shape(int dim) {
+// The backward pass holds four times as much for each value: one vector a thread, or
+// two where a wave holds a row. As many blocks as are resident at once (of 512 threads
+// three a unit). Measured on 67 million values, us with the sum's gradient / without:
+//   1000 values, bf16:  64 threads x 2 108 / 83, 256 x 1 170 / 129; fp32: 212 / 161, 206 / 148
+//   4096 values, bf16:  768 blocks 103 / 79, 1024 blocks 120 / 92
+// (their bytes at a copy's rate: bf16 100 / 75, fp32 200 / 150). Eight waves a SIMD by
+// spilling registers: 4096 values 134.
+Shape bwd_shape(bool wide, int dim) {
   if (dim <= 512) return {64, 1};
+  if (dim <= 1024 && !wide) return {64, 2};
   if (dim <= 2048) return {256, 1};
   if (dim <= 4096) return {512, 1};
   if (dim <= 8192) return {1024, 1};
@@ -310,9 +317,8 @@ template <typename F> void with_fwd_shape(Shape s, F f) {
   else if (s.tpr == 512) f(Int<512>{}, Int<1>{});
   else s.vpt == 1 ? f(Int<1024>{}, Int<1>{}) : s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : s.vpt == 4 ? f(Int<1024>{}, Int<4>{}) : f(Int<1024>{}, Int<0>{});
 }
-template <typename F> void with_bwd_shape(int dim, F f) {
-  const Shape s = bwd_shape(dim);
-  if (s.tpr == 64) f(Int<64>{}, Int<1>{});
+template <typename F> void with_bwd_shape(Shape s, F f) {
+  if (s.tpr == 64) s.vpt == 1 ? f(Int<64>{}, Int<1>{}) : f(Int<64>{}, Int<2>{});
   else if (s.tpr == 256) f(Int<256>{}, Int<1>{});
   else if (s.tpr == 512) f(Int<512>{}, Int<1>{});
   else s.vpt == 1 ? f(Int<1024>{}, Int<1>{}) : s.vpt == 2 ? f(Int<1024>{}, Int<2>{}) : f(Int<1024>{}, Int<0>{});
@@ -346,7 +352,7 @@ template <typename T, typename W>
 void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const void* w,
          const float* rstd, void* dx, float* part, void* dw, int parts, long rows, int dim,
          hipStream_t stream) {
-  with_bwd_shape(dim, [&](auto tpr, auto vpt) {
+  with_bwd_shape(bwd_shape(std::is_same<T, float>::value, dim), [&](auto tpr, auto vpt) {
     constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(parts), dim3(block_of(TPR)), TPR < 256 ? dim * 4 : 0,
@@ -385,8 +391,9 @@ extern "C" void al_rms_fwd(int type, int wtype, const void* x, long x_stride,
 }
 
 // how many partial rows of dw the backward pass writes
-extern "C" int al_rms_bwd_parts(long rows, int dim) {
-  return blocks_for(bwd_shape(dim), rows, 1024);
+extern "C" int al_rms_bwd_parts(int type, long rows, int dim) {
+  const Shape shape = bwd_shape(type == kTypeF32, dim);
+  return blocks_for(shape, rows, shape.tpr == 512 ? 768 : 1024);
 }
 
 extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,
