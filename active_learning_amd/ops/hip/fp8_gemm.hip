@@ -94,6 +94,10 @@ template <int KIND> AL_DEV unsigned scale_code(const void* p, long at) {
 // values, at most 16 of them, and each wave quantises the blocks that it reads:
 // a launch less, and b's bytes are what it costs. With T unsigned char they come
 // as codes.
+//
+// 1x1000x2048 with values takes 4.6 us, a launch; 16x8192x8192 21 us for 67 MB of b, which a
+// copy moves in 12.5, and 16x16384x8192 31.5 us (24.9): each step of a wave waits once for
+// memory. Three blocks in flight a wave, without a branch in the loop, took 24 and 36.
 template <typename T, bool EXACT, int KIND, bool BTILE, int MT, int NT, int WAVES>
 __launch_bounds__(WAVES * 64)
 __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g, int across) {
@@ -257,6 +261,11 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 // With e8m0 scales the matrix instruction applies them, or, in the EXACT form (bf16
 // instructions), the conversion to bf16. 32-bit scales multiply each block's sum as
 // it is added to the total.
+//
+// 8192x8192x8192: e8m0 376 to 395 us, 2.8 to 2.9 PFLOP/s, the matrix cores busy in 79% of
+// the cycles and the clock at 1.66 GHz, which power leaves; 32-bit scales 473 us, where the
+// scaling takes as many vector cycles as the products take matrix cycles; EXACT 737 us,
+// 1.49 PFLOP/s. LDS conflicts: 1 cycle in 150.
 
 constexpr int kHalf = 128 * 128;       // bytes of half a tile: 128 rows of a block
 constexpr int kRingB = 5 * kHalf;      // where b's ring begins
@@ -600,6 +609,12 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 // this step's loads there and is done with the last step, whose place is then asked
 // for anew. The order of the 16-byte chunks within a block is the same on both
 // sides: a lane has chunks l4 and l4 + 4 of its row.
+//
+// 2048x2048x8192 takes 44 us, and for 32-bit results 73; 4096x2048x8192 for 32-bit results
+// 118 (a bf16 product at the library's rate: 97). There the matrix cores are busy in 44% of
+// the cycles and the vector units, which convert, in 35%: waves that meet at a barrier each
+// step do both at the same times. Fragments read a step ahead, 16 waves of 32x64 and four
+// of 64x128 took 119, 128 and 141 us.
 template <int KIND, bool EXACT, bool BTILE, int TM, int TN, int WM, int WN, int STAGES>
 __launch_bounds__(WM * WN * 64)
 __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
