@@ -98,11 +98,13 @@ class Fp8Blocks:
 
     @property
     def values(self):
-        return self._codes[:, :self.shape[1]]
+        cols = self.shape[1]
+        return self._codes if self._codes.shape[1] == cols else self._codes[:, :cols]
 
     @property
     def scale(self):
-        return self._scales[:, :_blocks(self.shape[1])]
+        blocks = _blocks(self.shape[1])
+        return self._scales if self._scales.shape[1] == blocks else self._scales[:, :blocks]
 
     @property
     def device(self):
