@@ -96,8 +96,9 @@ template <int KIND> AL_DEV unsigned scale_code(const void* p, long at) {
 // as codes.
 //
 // 1x1000x2048 with values takes 4.6 us, a launch; 16x8192x8192 21 us for 67 MB of b, which a
-// copy moves in 12.5, and 16x16384x8192 31.5 us (24.9): each step of a wave waits once for
-// memory. Three blocks in flight a wave, without a branch in the loop, took 24 and 36.
+// copy moves in 12.5, and 16x16384x8192 31.5 us (24.9): each unit takes 25 KB a microsecond of
+// x and b together, with 16 waves (21), three blocks in flight a wave (24) and blocks in an
+// order of each workgroup's own (22) too.
 template <typename T, bool EXACT, int KIND, bool BTILE, int MT, int NT, int WAVES>
 __launch_bounds__(WAVES * 64)
 __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, Gemm g, int across) {

@@ -4,8 +4,8 @@
     y = s * rstd * weight
 
 The norm is that of the rounded sum, which is also what comes back for the next
-residual and what the backward pass reads. All arithmetic is in 32 bits, rounded
-once. GPU tensors run rmsnorm.hip; CPU tensors run the torch math below, which
+residual and what the backward pass reads. Arithmetic is in 32 bits or more (64 in
+front of an e4m3 output) and rounded to the type once. GPU tensors run rmsnorm.hip; CPU tensors run the torch math below, which
 defines the semantics that the kernels are tested against.
 
 Stands beside batch_norm_act (ops/functional.py): a norm for embeddings and
@@ -45,11 +45,11 @@ def _check(x, weight, residual, eps):
         raise ValueError(f"eps must be positive, got {eps}")
 
 
-def _forward_cpu(x, weight, residual, eps):
+def _forward_cpu(x, weight, residual, eps, wide=torch.float32):
     total = x if residual is None else (x.float() + residual.float()).to(x.dtype)
-    s = total.float()
+    s = total.to(wide)
     rstd = 1.0 / torch.sqrt(s.square().mean(-1, keepdim=True) + eps)
-    return s * rstd * weight.float(), total, rstd
+    return s * rstd * weight.to(wide), total, rstd
 
 
 class _RMSNormCPU(Function):
@@ -97,8 +97,8 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
     """``rms_norm`` straight into e4m3 with a scale for each 128 values of a row.
 
     Returns Fp8Blocks of (rows, dim), the leading axes flattened, or (blocks,
-    sum) where a residual is given. The norm is quantised from 32 bits, without a
-    rounding to x's type between. For inference: it has no gradient, and inputs
+    sum) where a residual is given. Codes and scales are those of the norm in 64 bits,
+    without a rounding to x's type between. For inference: it has no gradient, and inputs
     that ask for one are refused.
     """
     kind = check_scale_kind(scale)
@@ -111,8 +111,8 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
             t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to "
                            "train, or torch.no_grad()")
-    y, total, _ = _forward_cpu(x, weight, residual, eps)
-    blocks = quantize_fp8(y.reshape(-1, y.shape[-1]), scale=scale)
+    y, total, _ = _forward_cpu(x, weight, residual, eps, torch.float64)
+    blocks = quantize_fp8(y.float().reshape(-1, y.shape[-1]), scale=scale)
     return blocks if residual is None else (blocks, total)
 
 
