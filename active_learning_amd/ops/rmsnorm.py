@@ -5,8 +5,9 @@
 
 The norm is that of the rounded sum, which is also what comes back for the next
 residual and what the backward pass reads. Arithmetic is in 32 bits or more (64 in
-front of an e4m3 output) and rounded to the type once. GPU tensors run rmsnorm.hip; CPU tensors run the torch math below, which
-defines the semantics that the kernels are tested against.
+front of an e4m3 output) and rounded to the type once. GPU tensors run rmsnorm.hip;
+CPU tensors run the torch math below, which defines the semantics that the kernels
+are tested against.
 
 Stands beside batch_norm_act (ops/functional.py): a norm for embeddings and
 heads, whose rows are independent of the batch.
