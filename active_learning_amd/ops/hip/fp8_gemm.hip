@@ -264,7 +264,7 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 // it is added to the total.
 //
 // 8192x8192x8192: e8m0 376 to 395 us, 2.8 to 2.9 PFLOP/s, the matrix cores busy in 79% of
-// the cycles and the clock at 1.66 GHz, which power leaves; 32-bit scales 473 us, where the
+// the cycles and the clock at 1.66 GHz, which power leaves; 32-bit scales 460 us, where the
 // scaling takes as many vector cycles as the products take matrix cycles; EXACT 737 us,
 // 1.49 PFLOP/s. LDS conflicts: 1 cycle in 150.
 
@@ -449,26 +449,34 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
           c[1][1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y1, x1, c[1][1], 0, 0, 0);
         }
     } else {
+      // three tiles' products ahead of their scaling, as many as registers hold: one ahead
+      // 472 us where this takes 460
+      f32x16 d[3];
+      auto start = [&](f32x16& d, int t) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        f32x16 d[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) d[i][r] = 0.f;
+        for (int r = 0; r < 16; ++r) d[r] = 0.f;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
+          d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[t >> 1][half], fa[t & 1][half], d, 0, 0, 0, 0, 0, 0);
+      };
+      auto add = [&](f32x16& d, int t) __attribute__((always_inline)) {
+        const int i = t & 1, j = t >> 1;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            d[i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j][half], fa[i][half], d[i], 0, 0, 0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int by = BTILE ? sb[j] : scale_of(256 + wc * 64 + j * 32 + (r >> 2) * 8 + l5 * 4 + (r & 3), k, s);
-            c[i][j][r] = fmaf(d[i][r], __int_as_float(sa[i]) * __int_as_float(by), c[i][j][r]);
-          }
-      }
+        for (int r = 0; r < 16; ++r) {
+          const int by = BTILE ? sb[j] : scale_of(256 + wc * 64 + j * 32 + (r >> 2) * 8 + l5 * 4 + (r & 3), k, s);
+          c[i][j][r] = fmaf(d[r], __int_as_float(sa[i]) * __int_as_float(by), c[i][j][r]);
+        }
+      };
+      start(d[0], 0);
+      start(d[1], 1);
+      start(d[2], 2);
+      __builtin_amdgcn_sched_barrier(0);
+      add(d[0], 0);
+      start(d[0], 3);
+      __builtin_amdgcn_sched_barrier(0);
+      add(d[1], 1);
+      add(d[2], 2);
+      add(d[0], 3);
     }
     __builtin_amdgcn_s_setprio(0);
   };
