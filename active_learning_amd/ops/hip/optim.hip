@@ -93,7 +93,9 @@ extern "C" void al_sgd_step_multi(const void* table, int nchunks, float lr,
 
 // Variant reading (lr, momentum, wd) from device memory: lets a hipGraph-
 // captured training step track the LR schedule — the host updates the
-// 3-float hyper buffer between replays instead of re-capturing.
+// 3-float hyper buffer between replays instead of re-capturing. A step that was
+// captured without momentum has no buffers, whatever the hyper buffer says later:
+// the kernels that read it look for both.
 template <bool ZG>
 __global__ void sgd_mt_kernel_dev(const SgdChunk* __restrict__ table,
                                   const float* __restrict__ hyper) {
@@ -107,7 +109,7 @@ __global__ void sgd_mt_kernel_dev(const SgdChunk* __restrict__ table,
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     float grad = g[i] + wd * p[i];
     if (ZG) g[i] = 0.f;
-    if (momentum != 0.f) {
+    if (buf && momentum != 0.f) {
       const float b = buf[i] * momentum + grad;
       buf[i] = b;
       grad = b;
@@ -325,7 +327,7 @@ __global__ void sgd_mt_clip_kernel(const SgdChunk* __restrict__ table, float lr,
     f32x8 w = load8_upto(p + i, left);
     f32x8 grad = load8_upto(g + i, left) * factor + wd * w;
     if (ZG) store8_upto(g + i, f32x8{0, 0, 0, 0, 0, 0, 0, 0}, left);
-    if (momentum != 0.f) {
+    if (buf && momentum != 0.f) {
       grad = load8_upto(buf + i, left) * momentum + grad;
       store8_upto(buf + i, grad, left);
     }
@@ -344,7 +346,7 @@ __global__ void sgd_clip_kernel(float* __restrict__ p, const float* __restrict__
   const float factor = norm_factor[1];
   for (long i = grid_stride_begin(); i < n; i += grid_stride_step()) {
     float grad = g[i] * factor + wd * p[i];
-    if (momentum != 0.f) {
+    if (buf && momentum != 0.f) {
       grad = buf[i] * momentum + grad;
       buf[i] = grad;
     }

@@ -69,6 +69,7 @@ class FusedSGD(torch.optim.Optimizer):
         self._clip_dev = None    # device max_grad_norm; graph-capture mode
         self._clip_to = None
         self._captured_plain = False  # a step without max_grad_norm was captured
+        self._captured_still = False  # a step with a parameter without momentum was captured
 
     def enable_persistent_grads(self):
         """Persistent-grad mode for hipGraph capture: the caller must NOT call
@@ -81,15 +82,21 @@ class FusedSGD(torch.optim.Optimizer):
         """Switch the fused update to read (lr, momentum, wd) from device
         memory so a hipGraph-captured step tracks LR-schedule changes without
         re-capture; call sync_hyper() OUTSIDE capture whenever the schedule
-        steps."""
+        steps. What a captured step has no memory for (momentum, where it was 0;
+        a clipping bound, where there was none) cannot come later: sync_hyper
+        refuses it."""
         assert len(self.param_groups) == 1, "device-hyper mode: single group"
-        self._hyper_host = torch.zeros(3, dtype=torch.float32).pin_memory()
+        self._hyper_host = torch.zeros(3, dtype=torch.float32)
+        if torch.device(device).type == "cuda":
+            self._hyper_host = self._hyper_host.pin_memory()
         self._hyper_dev = torch.zeros(3, dtype=torch.float32, device=device)
         self.sync_hyper()
 
     def sync_hyper(self):
         g = self.param_groups[0]
         vals = (float(g["lr"]), float(g["momentum"]), float(g["weight_decay"]))
+        if self._captured_still and vals[1] != 0:
+            raise ValueError("the step was captured without momentum: set it before the capture")
         if tuple(self._hyper_host.tolist()) != vals:
             self._hyper_host.copy_(torch.tensor(vals))
             self._hyper_dev.copy_(self._hyper_host, non_blocking=True)
@@ -125,12 +132,16 @@ class FusedSGD(torch.optim.Optimizer):
         loss = closure() if closure is not None else None
         ext = load_extension() if extension_available() else None
         clip = self._clip()
+        capturing = self._hyper_dev is not None and torch.cuda.is_current_stream_capturing()
         for gi, group in enumerate(self.param_groups):
             lr = group["lr"]
             momentum = group["momentum"]
             wd = group["weight_decay"]
             fused = []
             params = [p for p in group["params"] if p.grad is not None]
+            if capturing and momentum == 0 and any(
+                    "momentum_buffer" not in self.state.get(p, ()) for p in params):
+                self._captured_still = True
             if ext is not None and params and ext.sgd_fusable(params):
                 fused, params = params, []  # all of them: no look at each in Python
             for p in params:
