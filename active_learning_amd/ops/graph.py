@@ -20,6 +20,7 @@ by autograd hooks on the host, which a replay skips — world_size > 1 keeps
 the eager loop (its collectives already overlap backward).
 """
 
+import contextlib
 import logging
 
 import torch
@@ -153,7 +154,8 @@ class GraphedTrainStep:
         import gc
         gc.collect()  # drop any lingering warmup autograd graphs for certain
         g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
+        owned = (self.opt.capture_of(self) if self._persistent else contextlib.nullcontext())
+        with owned, torch.cuda.graph(g):
             out = self.net(self.x_static)
             loss = self.crit(out, self.y_static)
             loss.backward()
@@ -186,6 +188,8 @@ class GraphedTrainStep:
             if self._calls < self.warmup:
                 self._calls += 1
                 return self._eager(self.x_static, self.y_static)
+            if self._persistent:
+                self.opt.sync_hyper()  # the first replay reads what is set now
             try:
                 torch.cuda.synchronize()
                 self._capture()

@@ -11,8 +11,9 @@ Constructor signatures match torch.optim so arg-pool optimizer_args apply
 unchanged; the trainer maps names through OPTIMIZERS.
 """
 
-import math
+import contextlib
 import struct
+import weakref
 
 import torch
 
@@ -67,9 +68,12 @@ class FusedSGD(torch.optim.Optimizer):
         self.max_grad_norm = _check_max_norm(max_grad_norm)
         self.last_grad_norm = None
         self._clip_dev = None    # device max_grad_norm; graph-capture mode
-        self._clip_to = None
-        self._captured_plain = False  # a step without max_grad_norm was captured
-        self._captured_still = False  # a step with a parameter without momentum was captured
+        self._clip_to = None     # where captured and eager steps alike leave norm and factor
+        self._clip_host = None
+        # who holds a captured step -> what that step cannot follow: "max_grad_norm"
+        # where it was captured without, "momentum" where a buffer was missing
+        self._left_out = weakref.WeakKeyDictionary()
+        self._capture_owner = None
 
     def enable_persistent_grads(self):
         """Persistent-grad mode for hipGraph capture: the caller must NOT call
@@ -79,37 +83,62 @@ class FusedSGD(torch.optim.Optimizer):
         self._persistent = True
 
     def enable_device_hyper(self, device):
-        """Switch the fused update to read (lr, momentum, wd) from device
-        memory so a hipGraph-captured step tracks LR-schedule changes without
-        re-capture; call sync_hyper() OUTSIDE capture whenever the schedule
-        steps. What a captured step has no memory for (momentum, where it was 0;
-        a clipping bound, where there was none) cannot come later: sync_hyper
-        refuses it."""
+        """Switch the fused update to read (lr, momentum, wd) and the clipping bound
+        from device memory so a hipGraph-captured step tracks their changes without
+        re-capture; call sync_hyper() OUTSIDE capture right before it and whenever
+        one of them changed. What a captured step has no part for (momentum, where
+        a buffer was missing; a clipping bound, where there was none) cannot come
+        later: sync_hyper refuses it as long as the step is there."""
         assert len(self.param_groups) == 1, "device-hyper mode: single group"
-        self._hyper_host = torch.zeros(3, dtype=torch.float32)
-        if torch.device(device).type == "cuda":
-            self._hyper_host = self._hyper_host.pin_memory()
-        self._hyper_dev = torch.zeros(3, dtype=torch.float32, device=device)
+        device = torch.empty(0, device=device).device
+        if self._hyper_dev is None or self._hyper_dev.device != device:
+            # otherwise a step that was captured before goes on to follow
+            self._hyper_host = torch.zeros(3, dtype=torch.float32)
+            if device.type == "cuda":
+                self._hyper_host = self._hyper_host.pin_memory()
+            self._hyper_dev = torch.zeros(3, dtype=torch.float32, device=device)
+            self._clip_dev = torch.full((1,), float("inf"), device=device)
+            self._clip_to = torch.zeros(2, device=device)
+            self._clip_host = None
         self.sync_hyper()
+
+    @contextlib.contextmanager
+    def capture_of(self, owner):
+        """Around a capture of step(): ``owner`` is what holds the captured step. A
+        capture outside of this counts as the optimizer's own, for good."""
+        self._capture_owner = owner
+        try:
+            yield
+        except BaseException:
+            self._left_out.pop(owner, None)
+            raise
+        finally:
+            self._capture_owner = None
+
+    def _leave_out(self, what):
+        owner = self if self._capture_owner is None else self._capture_owner
+        self._left_out.setdefault(owner, set()).add(what)
+
+    def _capturing(self):
+        return self._hyper_dev is not None and torch.cuda.is_current_stream_capturing()
 
     def sync_hyper(self):
         g = self.param_groups[0]
         vals = (float(g["lr"]), float(g["momentum"]), float(g["weight_decay"]))
-        if self._captured_still and vals[1] != 0:
+        left_out = set().union(*self._left_out.values())
+        if "momentum" in left_out and vals[1] != 0:
             raise ValueError("the step was captured without momentum: set it before the capture")
+        if "max_grad_norm" in left_out and self.max_grad_norm is not None:
+            raise ValueError("the step was captured without max_grad_norm: set it before the "
+                             "capture")
         if tuple(self._hyper_host.tolist()) != vals:
             self._hyper_host.copy_(torch.tensor(vals))
             self._hyper_dev.copy_(self._hyper_host, non_blocking=True)
+        self._sync_bound()
+
+    def _sync_bound(self):
         bound = self.max_grad_norm
-        if bound is not None and self._captured_plain:
-            raise ValueError("the step was captured without max_grad_norm: set it before the "
-                             "capture")
-        if bound is not None and self._clip_dev is None:
-            self._clip_dev = torch.full((1,), float(bound), device=self._hyper_dev.device)
-            # where captured and eager steps alike leave the norm and the factor
-            self._clip_to = torch.zeros(2, device=self._hyper_dev.device)
-            self._clip_host = bound
-        elif self._clip_dev is not None and self._clip_host != bound:
+        if self._clip_host != bound:
             # a captured step goes on to look at the bound: none is an infinite one
             self._clip_dev.fill_(float("inf") if bound is None else float(bound))
             self._clip_host = bound
@@ -117,10 +146,16 @@ class FusedSGD(torch.optim.Optimizer):
     def _clip(self):
         """(norm, factor) of this step's gradients on their device; None without
         max_grad_norm or gradients."""
+        capturing = self._capturing()
         if self.max_grad_norm is None:
-            if self._hyper_dev is not None and torch.cuda.is_current_stream_capturing():
-                self._captured_plain = True
+            if capturing:
+                self._leave_out("max_grad_norm")
             return None
+        if self._clip_dev is not None:
+            if not capturing:
+                self._sync_bound()
+            elif self._clip_host != self.max_grad_norm:
+                raise RuntimeError("max_grad_norm changed: call sync_hyper() before the capture")
         both = _params_norm_factor(_all_params(self), float(self.max_grad_norm),
                                    self._clip_dev, self._clip_to)
         if both is not None:
@@ -132,7 +167,7 @@ class FusedSGD(torch.optim.Optimizer):
         loss = closure() if closure is not None else None
         ext = load_extension() if extension_available() else None
         clip = self._clip()
-        capturing = self._hyper_dev is not None and torch.cuda.is_current_stream_capturing()
+        capturing = self._capturing()
         for gi, group in enumerate(self.param_groups):
             lr = group["lr"]
             momentum = group["momentum"]
@@ -141,7 +176,7 @@ class FusedSGD(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             if capturing and momentum == 0 and any(
                     "momentum_buffer" not in self.state.get(p, ()) for p in params):
-                self._captured_still = True
+                self._leave_out("momentum")
             if ext is not None and params and ext.sgd_fusable(params):
                 fused, params = params, []  # all of them: no look at each in Python
             for p in params:

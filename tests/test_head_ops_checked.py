@@ -49,3 +49,82 @@ def test_momentum_cannot_come_after_the_capture(capturing, bound):
     opt.param_groups[0]["momentum"] = 0.9
     opt.sync_hyper()
     assert abs(opt._hyper_dev[1] - 0.9) < 1e-6
+
+
+@pytest.fixture
+def norm_calls(monkeypatch):
+    """What each step hands to the norm: the bound on the host, on the device, and where to."""
+    from active_learning_amd.ops import optim
+    calls, real = [], optim._params_norm_factor
+
+    def spy(params, max_norm, max_dev=None, to=None):
+        calls.append((max_norm, max_dev, to))
+        return real(params, max_norm)
+
+    monkeypatch.setattr(optim, "_params_norm_factor", spy)
+    return calls
+
+
+def test_bound_set_at_the_capture_is_followed(capturing, norm_calls):
+    """A bound that is set or changed on exactly the step that is captured is read from
+    the device, so that later changes reach the captured step."""
+    opt = FusedSGD(_params([(3, 4)]), lr=0.1)
+    opt.enable_device_hyper("cpu")
+    opt.step()
+    assert not norm_calls
+    opt.max_grad_norm = 0.5
+    with opt.capture_of(test_bound_set_at_the_capture_is_followed):
+        capturing(True)
+        with pytest.raises(RuntimeError, match="sync_hyper"):  # refused, not forgotten
+            opt.step()
+        capturing(False)
+        opt.sync_hyper()
+        capturing(True)
+        opt.step()
+        capturing(False)
+    _, on_device, to = norm_calls[-1]
+    assert on_device is not None and to is not None and on_device.item() == 0.5
+    opt.max_grad_norm = 0.25
+    opt.sync_hyper()
+    assert on_device.item() == 0.25
+    opt.max_grad_norm = None
+    opt.sync_hyper()
+    assert on_device.item() == float("inf")
+    # an eager step between, and another user of the same optimizer, leave it in place
+    opt.max_grad_norm = 0.125
+    opt.step()
+    opt.enable_device_hyper("cpu")
+    assert norm_calls[-1][1] is on_device and on_device.item() == 0.125 and opt._clip_dev is on_device
+
+
+def test_refusals_last_as_long_as_the_captured_step(capturing):
+    class Owner:
+        pass
+
+    opt = FusedSGD(_params([(3, 4)]), lr=0.1)
+    opt.enable_device_hyper("cpu")
+
+    def capture(owner, fails=False):
+        with opt.capture_of(owner):
+            capturing(True)
+            opt.step()
+            capturing(False)
+            if fails:
+                raise OSError("capture")
+
+    def set_all():
+        opt.max_grad_norm, opt.param_groups[0]["momentum"] = 0.5, 0.9
+        try:
+            opt.sync_hyper()
+        finally:
+            opt.max_grad_norm, opt.param_groups[0]["momentum"] = None, 0.0
+
+    failed, kept = Owner(), Owner()
+    with pytest.raises(OSError):
+        capture(failed, fails=True)
+    set_all()
+    capture(kept)
+    with pytest.raises(ValueError, match="captured without"):
+        set_all()
+    del kept
+    set_all()

@@ -36,3 +36,41 @@ def test_momentum_without_buffers_is_none(clip):
         ext.sgd_step_multi_dev(table, 1, hyper, False)
     for got in done:  # 0.1 and 0.01 as 32-bit numbers, two products, two sums
         assert ((got.double() - want).abs() <= 6 * U32 * (want.abs() + g.double().abs())).all()
+
+
+@pytest.mark.parametrize("before,at", [(None, 0.5), (0.5, 0.05), (0.05, 0.5)])
+def test_bound_of_the_step_that_is_captured(before, at):
+    """The bound is set, or changed, on exactly the step that the trainer captures, and
+    changed again later: replays follow eager steps."""
+    from active_learning_amd.ops.fp8 import Fp8Linear
+    from active_learning_amd.ops.graph import GraphedTrainStep
+    from active_learning_amd.ops.loss import CrossEntropyLoss
+    from active_learning_amd.ops.optim import FusedSGD
+    from active_learning_amd.ops.rmsnorm import RMSNorm
+    dev = torch.device("cuda", torch.cuda.current_device())
+    xs = [randn(64, 512, seed=s) for s in range(8)]
+    y = torch.arange(64, device="cuda") % 10
+
+    def run(warmup):
+        torch.manual_seed(1)
+        net = torch.nn.Sequential(RMSNorm(512), Fp8Linear(512, 10)).cuda()
+        opt = FusedSGD(net.parameters(), lr=0.1, momentum=0.9, max_grad_norm=before)
+        step = GraphedTrainStep(net, opt, CrossEntropyLoss().to(dev), dev, warmup=warmup)
+        norms = []
+        for i, x in enumerate(xs):
+            if i == 2:
+                opt.max_grad_norm, opt.param_groups[0]["lr"] = at, 0.03
+            if i == 5:
+                opt.max_grad_norm = 0.1
+            if i == 7:
+                opt.max_grad_norm = None
+            step.step(x, y)
+            if 2 <= i < 7:
+                norms.append(opt.last_grad_norm.item())
+        torch.cuda.synchronize()
+        return [p.detach().clone() for p in net.parameters()], norms, step._graph is not None
+
+    eager, graphed = run(100), run(2)
+    assert not eager[2] and graphed[2]
+    assert eager[1] == graphed[1]
+    assert all(torch.equal(a, b) for a, b in zip(eager[0], graphed[0]))
