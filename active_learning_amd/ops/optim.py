@@ -93,9 +93,7 @@ class FusedSGD(torch.optim.Optimizer):
         device = torch.empty(0, device=device).device
         if self._hyper_dev is None or self._hyper_dev.device != device:
             # otherwise a step that was captured before goes on to follow
-            self._hyper_host = torch.zeros(3, dtype=torch.float32)
-            if device.type == "cuda":
-                self._hyper_host = self._hyper_host.pin_memory()
+            self._hyper_host = None
             self._hyper_dev = torch.zeros(3, dtype=torch.float32, device=device)
             self._clip_dev = torch.full((1,), float("inf"), device=device)
             self._clip_to = torch.zeros(2, device=device)
@@ -131,9 +129,14 @@ class FusedSGD(torch.optim.Optimizer):
         if "max_grad_norm" in left_out and self.max_grad_norm is not None:
             raise ValueError("the step was captured without max_grad_norm: set it before the "
                              "capture")
-        if tuple(self._hyper_host.tolist()) != vals:
-            self._hyper_host.copy_(torch.tensor(vals))
-            self._hyper_dev.copy_(self._hyper_host, non_blocking=True)
+        if self._hyper_host != vals:
+            # host memory of its own: the copy before may still be on its way, behind
+            # steps that are queued and read the values that it brings
+            host = torch.tensor(vals)
+            if self._hyper_dev.is_cuda:
+                host = host.pin_memory()
+            self._hyper_dev.copy_(host, non_blocking=True)
+            self._hyper_host = vals
         self._sync_bound()
 
     def _sync_bound(self):

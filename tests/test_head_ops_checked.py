@@ -128,3 +128,24 @@ def test_refusals_last_as_long_as_the_captured_step(capturing):
         set_all()
     del kept
     set_all()
+
+
+def test_hyperparameters_on_their_way_keep_their_values():
+    """A copy to the device runs behind the steps that are queued: the next change does
+    not write into the host memory that it reads."""
+    opt = FusedSGD(_params([(3, 4)]), lr=0.1, momentum=0.9)
+    opt.enable_device_hyper("cpu")
+    sent = []
+
+    class Device:
+        is_cuda = False
+
+        def copy_(self, host, non_blocking=False):
+            sent.append(host)
+
+    opt._hyper_dev = Device()
+    for lr in (0.5, 0.25):
+        opt.param_groups[0]["lr"] = lr
+        opt.sync_hyper()
+        opt.sync_hyper()
+    assert [t[0].item() for t in sent] == [0.5, 0.25]
