@@ -35,11 +35,23 @@ def _check_max_norm(max_grad_norm):
     return max_grad_norm
 
 
+class _Clips:
+    """The bound of an optimizer that clips, checked whenever it is set."""
+
+    @property
+    def max_grad_norm(self):
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, bound):
+        self._max_grad_norm = _check_max_norm(bound)
+
+
 def _all_params(optimizer):
     return [p for group in optimizer.param_groups for p in group["params"]]
 
 
-class FusedSGD(torch.optim.Optimizer):
+class FusedSGD(_Clips, torch.optim.Optimizer):
     """SGD with momentum and weight decay.
 
     ``max_grad_norm``: the step uses gradients scaled so that their norm over all
@@ -65,7 +77,7 @@ class FusedSGD(torch.optim.Optimizer):
         self._hyper_dev = None   # device (lr, momentum, wd); graph-capture mode
         self._hyper_host = None
         self._persistent = False  # grads kept in stable storage, zeroed in-kernel
-        self.max_grad_norm = _check_max_norm(max_grad_norm)
+        self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None
         self._clip_dev = None    # device max_grad_norm; graph-capture mode
         self._clip_to = None     # where captured and eager steps alike leave norm and factor
@@ -132,7 +144,7 @@ class FusedSGD(torch.optim.Optimizer):
         if self._hyper_host != vals:
             # host memory of its own: the copy before may still be on its way, behind
             # steps that are queued and read the values that it brings
-            host = torch.tensor(vals)
+            host = torch.tensor(vals, dtype=torch.float32)
             if self._hyper_dev.is_cuda:
                 host = host.pin_memory()
             self._hyper_dev.copy_(host, non_blocking=True)
@@ -357,14 +369,14 @@ class FusedSGD(torch.optim.Optimizer):
             bump_tick(p)
 
 
-class FusedAdam(torch.optim.Optimizer):
+class FusedAdam(_Clips, torch.optim.Optimizer):
     """Adam; ``max_grad_norm`` and ``last_grad_norm`` as in FusedSGD."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
                  max_grad_norm=None):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(params, defaults)
-        self.max_grad_norm = _check_max_norm(max_grad_norm)
+        self.max_grad_norm = max_grad_norm
         self.last_grad_norm = None
 
     def _clip(self):

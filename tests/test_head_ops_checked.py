@@ -4,7 +4,7 @@ answered wrongly or forgotten, each with what it has to give."""
 import pytest
 import torch
 
-from active_learning_amd.ops.optim import FusedSGD
+from active_learning_amd.ops.optim import FusedSGD, build_optimizer
 
 
 def _params(sizes):
@@ -149,3 +149,16 @@ def test_hyperparameters_on_their_way_keep_their_values():
         opt.sync_hyper()
         opt.sync_hyper()
     assert [t[0].item() for t in sent] == [0.5, 0.25]
+
+
+@pytest.mark.parametrize("name", ["SGD", "Adam"])
+@pytest.mark.parametrize("bound", [-1.0, float("nan")])
+def test_a_bound_that_is_set_later_is_checked(name, bound):
+    """A negative one would turn the gradients round."""
+    opt = build_optimizer(name, _params([(3, 4)]), lr=0.1, max_grad_norm=1.0)
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        opt.max_grad_norm = bound
+    assert opt.max_grad_norm == 1.0
+    opt.max_grad_norm = None
+    opt.step()
+    assert opt.last_grad_norm is None
