@@ -56,8 +56,8 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
 
     ``max_grad_norm``: the step uses gradients scaled so that their norm over all
     parameters is at most this (ops/grad_clip.py). The scaling happens as the
-    update reads them: ``p.grad`` keeps its values, and the norm they had is in
-    ``last_grad_norm``, a 0-d tensor on the device.
+    update reads them: ``p.grad`` keeps its values, and the norm they had is
+    ``last_grad_norm``, a 0-d tensor on the device that later steps leave alone.
     """
 
     _CHUNK = 32768  # elements per workgroup in the multi-tensor kernel
@@ -78,7 +78,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         self._hyper_host = None
         self._persistent = False  # grads kept in stable storage, zeroed in-kernel
         self.max_grad_norm = max_grad_norm
-        self.last_grad_norm = None
+        self._last_norm = None
         self._clip_dev = None    # device max_grad_norm; graph-capture mode
         self._clip_to = None     # where captured and eager steps alike leave norm and factor
         self._clip_host = None
@@ -111,6 +111,13 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
             self._clip_to = torch.zeros(2, device=device)
             self._clip_host = None
         self.sync_hyper()
+
+    @property
+    def last_grad_norm(self):
+        # with device hyperparameters all steps leave theirs in one place
+        if self._last_norm is None or self._clip_to is None:
+            return self._last_norm
+        return self._last_norm.clone()
 
     @contextlib.contextmanager
     def capture_of(self, owner):
@@ -174,7 +181,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         both = _params_norm_factor(_all_params(self), float(self.max_grad_norm),
                                    self._clip_dev, self._clip_to)
         if both is not None:
-            self.last_grad_norm = both[0]
+            self._last_norm = both[0]
         return both
 
     @torch.no_grad()

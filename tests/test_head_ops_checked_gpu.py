@@ -74,3 +74,22 @@ def test_bound_of_the_step_that_is_captured(before, at):
     assert not eager[2] and graphed[2]
     assert eager[1] == graphed[1]
     assert all(torch.equal(a, b) for a, b in zip(eager[0], graphed[0]))
+
+
+def test_norms_that_are_kept():
+    """A list of each step's norm holds them all, captured steps' and eager ones'."""
+    from active_learning_amd.ops.graph import GraphedTrainStep
+    from active_learning_amd.ops.linear import NativeLinear
+    from active_learning_amd.ops.loss import CrossEntropyLoss
+    from active_learning_amd.ops.optim import FusedSGD
+    dev = torch.device("cuda", torch.cuda.current_device())
+    net = NativeLinear(512, 10).cuda()
+    opt = FusedSGD(net.parameters(), lr=0.1, max_grad_norm=0.5)
+    step = GraphedTrainStep(net, opt, CrossEntropyLoss().to(dev), dev, warmup=2)
+    kept, read = [], []
+    for i, n in enumerate((64, 64, 64, 40, 64, 64)):
+        step.step(randn(n, 512, seed=i), torch.arange(n, device="cuda") % 10)
+        kept.append(opt.last_grad_norm)
+        read.append(kept[-1].item())
+    assert step._graph is not None and len(set(read)) == 6
+    assert [t.item() for t in kept] == read
