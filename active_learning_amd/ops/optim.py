@@ -73,7 +73,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         super().__init__(params, defaults)
         self._mt_cache = {}  # group idx -> (fingerprint, device table, nchunks)
         self._wt_cache = {}  # group idx -> (fingerprint, tile table, nrows)
-        self._mt_keepalive = []  # pinned/device tables referenced by live graphs
+        self._mt_keepalive = []  # device tables that a captured step reads, and outgrown ones
         self._hyper_dev = None   # device (lr, momentum, wd); graph-capture mode
         self._hyper_host = None
         self._persistent = False  # grads kept in stable storage, zeroed in-kernel
@@ -278,8 +278,9 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         # shadow's (0: none), and its length
         fp = ext.sgd_addresses(params, bufs, shadows)
         entry = self._mt_cache.get(gi)
+        capturing = torch.cuda.is_current_stream_capturing()
         if entry is None or entry[0] != fp:
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 # a table rebuild needs host allocations, which invalidate
                 # hipGraph capture — fall back to per-tensor launches for
                 # this (captured) step. With persistent grads the
@@ -292,12 +293,9 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                 while off < n:
                     rows.append((pp, gp, bp, sp, off, min(self._CHUNK, n - off)))
                     off += self._CHUNK
-            host = torch.tensor(rows, dtype=torch.int64).pin_memory()
-            dev = torch.empty_like(host, device=params[0].device)
-            dev.copy_(host, non_blocking=True)
-            self._mt_keepalive.append((host, dev))
-            entry = (fp, dev, len(rows))
-            self._mt_cache[gi] = entry
+            entry = self._new_table(self._mt_cache, gi, fp, rows, params[0].device)
+        if capturing:
+            self._keep(entry[1])
         if clip is not None:
             ext.sgd_step_multi_clip(entry[1], entry[2], lr, momentum, wd,
                                     self._hyper_dev, clip, self._persistent)
@@ -328,14 +326,37 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         if wt_fp:
             self._launch_wt_refresh(ext, gi, tuple(wt_fp), wt_entries)
 
+    def _keep(self, table):
+        if not any(table is t for t in self._mt_keepalive):
+            self._mt_keepalive.append(table)
+
+    def _new_table(self, cache, gi, fp, rows, device):
+        """Copies a table to the device, over the one that it replaces: a step whose
+        addresses changed (new gradients) takes no more memory than the one before.
+        Where a captured step reads that one, or it is too short, the new one gets
+        memory of its own, and an outgrown one stays, since a step on another stream
+        may still read it; sizes double, so that these are few."""
+        host = torch.tensor(rows, dtype=torch.int64).pin_memory()
+        dev = cache[gi][1] if gi in cache else None
+        if dev is None or len(dev) < len(rows) or any(dev is t for t in self._mt_keepalive):
+            size = len(rows)
+            if dev is not None and len(dev) < size:
+                self._keep(dev)
+                size = max(size, 2 * len(dev))
+            dev = torch.empty(size, host.shape[1], dtype=torch.int64, device=device)
+        dev[:len(rows)].copy_(host, non_blocking=True)
+        cache[gi] = entry = (fp, dev, len(rows))
+        return entry
+
     def _launch_wt_refresh(self, ext, gi, fp, shadows):
         """Refresh every cached (C,R,S,K) bwd-data weight permutation in one
         launch (64x64 tiles; only full tiles are enqueued — the host gates on
         K, C % 64). Table cached by pointer fingerprint like the sgd chunk
         table, so steady-state (and captured) steps launch with no H2D."""
         entry = self._wt_cache.get(gi)
+        capturing = torch.cuda.is_current_stream_capturing()
         if entry is None or entry[0] != fp:
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 for shadow in shadows:
                     shadow._al_wt = None  # lazy ATen rebuild for this step
                 return
@@ -348,12 +369,9 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                             rows.append((sp, dp,
                                          k0 | (c0 << 16) | (rs << 32),
                                          K | (C << 16) | (RS << 32)))
-            host = torch.tensor(rows, dtype=torch.int64).pin_memory()
-            dev = torch.empty_like(host, device=shadows[0].device)
-            dev.copy_(host, non_blocking=True)
-            self._mt_keepalive.append((host, dev))
-            entry = (fp, dev, len(rows))
-            self._wt_cache[gi] = entry
+            entry = self._new_table(self._wt_cache, gi, fp, rows, shadows[0].device)
+        if capturing:
+            self._keep(entry[1])
         ext.wt_refresh_multi(entry[1], entry[2])
 
     def _per_tensor_fallback(self, ext, params, lr, momentum, wd, clip):

@@ -93,3 +93,64 @@ def test_norms_that_are_kept():
         read.append(kept[-1].item())
     assert step._graph is not None and len(set(read)) == 6
     assert [t.item() for t in kept] == read
+
+
+@pytest.mark.parametrize("bound", [None, 0.5])
+def test_steps_with_new_gradients_take_no_more_memory(bound):
+    from active_learning_amd.ops.optim import FusedSGD
+    sizes = [100003, 7, 40000]
+    ps = [torch.nn.Parameter(randn(n, seed=i)) for i, n in enumerate(sizes)]
+    opt = FusedSGD(ps, lr=0.1, momentum=0.9, max_grad_norm=bound)
+    want, bufs = [p.detach().double() for p in ps], [0.0] * 3
+    used = []
+    gone = []
+    for step in range(30):
+        fresh = [randn(n, seed=10 * step + i) * 1e-2 for i, n in enumerate(sizes)]
+        norm = torch.cat([g.double() for g in fresh]).norm().item()
+        f = 1.0 if bound is None else min(1.0, bound / (norm + 1e-6))
+        for i, (p, g) in enumerate(zip(ps, fresh)):
+            gone.append(p.grad)  # the addresses do not come again
+            p.grad = g
+            bufs[i] = 0.9 * bufs[i] + f * g.double()
+            want[i] = want[i] - 0.1 * bufs[i]
+        before = torch.cuda.memory_allocated()
+        opt.step()
+        used.append(torch.cuda.memory_allocated() - before)
+    assert not any(used[2:]), used  # the second step still replaces the first one's norm
+    for p, w in zip(ps, want):  # at most seven roundings a step, of values under 8
+        assert ((p.double() - w).abs() <= 30 * 7 * U32 * 8).all()
+
+
+def test_captured_step_keeps_its_addresses():
+    """Steps with other gradients, eager, do not change what a captured step reads."""
+    from active_learning_amd.ops.optim import FusedSGD
+    ps = [torch.nn.Parameter(randn(n, seed=n)) for n in (70000, 33)]
+    opt = FusedSGD(ps, lr=0.5, max_grad_norm=1e6)
+    mine = [randn(*p.shape, seed=1) for p in ps]
+    want = [p.detach().double() for p in ps]
+
+    def use(grads):
+        for p, g in zip(ps, grads):
+            p.grad = g
+
+    def expect(grads):
+        for i, g in enumerate(grads):
+            want[i] = want[i] - 0.5 * g.double()
+
+    use(mine)
+    opt.step()
+    expect(mine)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for turn in range(4):
+        other = [randn(*p.shape, seed=2 + turn) for p in ps]
+        use(other)
+        opt.step()
+        expect(other)
+        mine[0].copy_(randn(*mine[0].shape, seed=20 + turn))
+        graph.replay()
+        expect(mine)
+    for p, w in zip(ps, want):  # nine steps of two roundings, of values under 32
+        assert ((p.double() - w).abs() <= 9 * 2 * U32 * 32).all()
