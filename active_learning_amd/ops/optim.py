@@ -195,7 +195,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
             momentum = group["momentum"]
             wd = group["weight_decay"]
             fused = []
-            params = [p for p in group["params"] if p.grad is not None]
+            params = [p for p in group["params"] if p.grad is not None and p.numel()]
             if capturing and momentum == 0 and any(
                     "momentum_buffer" not in self.state.get(p, ()) for p in params):
                 self._leave_out("momentum")

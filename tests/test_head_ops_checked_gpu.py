@@ -154,3 +154,17 @@ def test_captured_step_keeps_its_addresses():
         expect(mine)
     for p, w in zip(ps, want):  # nine steps of two roundings, of values under 32
         assert ((p.double() - w).abs() <= 9 * 2 * U32 * 32).all()
+
+
+@pytest.mark.parametrize("bound", [None, 0.5])
+def test_step_over_nothing(bound):
+    """Parameters of no values launch nothing, and leave no error for the next call."""
+    from active_learning_amd.ops.grad_clip import grad_norm
+    from active_learning_amd.ops.optim import FusedSGD
+    p = torch.nn.Parameter(torch.empty(0, 3, device="cuda"))
+    p.grad = torch.empty(0, 3, device="cuda")
+    opt = FusedSGD([p], lr=0.1, momentum=0.9, max_grad_norm=bound)
+    opt.step()
+    opt.step()
+    assert grad_norm(torch.full((4,), 2.0, device="cuda")).item() == 4.0
+    assert bound is None or opt.last_grad_norm.item() == 0.0
