@@ -213,7 +213,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                 if momentum != 0 and "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
                 buf = state.get("momentum_buffer")
-                if p.is_cuda and ext is not None:
+                if p.is_cuda and ext is not None and p.is_contiguous():
                     cache = getattr(p, "_al_cast", None)
                     shadow = (cache[1] if cache is not None
                               and cache[1].numel() == p.numel()
@@ -230,7 +230,10 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                     else:
                         _invalidate(p)
                     bump_tick(p)  # in-kernel update: no _version bump
-                else:
+                else:  # on the CPU, or of other strides than the kernels take
+                    if p.is_cuda and capturing:
+                        raise RuntimeError("a step that follows hyperparameters on the device "
+                                           "needs contiguous parameters")
                     gf = g.float()
                     if clip is not None:
                         gf = gf * clip[1]
@@ -434,7 +437,7 @@ class FusedAdam(_Clips, torch.optim.Optimizer):
                 t = state["step"]
                 bc1 = 1 - beta1 ** t
                 bc2 = 1 - beta2 ** t
-                if p.is_cuda and ext is not None:
+                if p.is_cuda and ext is not None and p.is_contiguous():
                     if clip is not None:
                         ext.adam_step_clip(p, p.grad.to(torch.float32).contiguous(),
                                            state["exp_avg"], state["exp_avg_sq"], lr, beta1,

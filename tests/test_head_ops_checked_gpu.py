@@ -168,3 +168,35 @@ def test_step_over_nothing(bound):
     opt.step()
     assert grad_norm(torch.full((4,), 2.0, device="cuda")).item() == 4.0
     assert bound is None or opt.last_grad_norm.item() == 0.0
+
+
+@pytest.mark.parametrize("name", ["SGD", "Adam"])
+@pytest.mark.parametrize("bound", [None, 0.5])
+@pytest.mark.parametrize("layout", ["channels_last", "transposed", "sliced"])
+def test_parameters_of_any_strides(name, bound, layout):
+    """A step on parameters that are not contiguous is that on contiguous ones."""
+    from active_learning_amd.ops.optim import build_optimizer
+
+    def parameter(seed):
+        if layout == "channels_last":
+            return randn(8, 5, 3, 3, seed=seed).contiguous(memory_format=torch.channels_last)
+        return randn(40, 30, seed=seed).t() if layout == "transposed" else randn(40, 60, seed=seed)[:, ::2]
+
+    whole = [parameter(s) for s in (1, 2)]
+    a = [torch.nn.Parameter(t) for t in whole]
+    b = [torch.nn.Parameter(t.detach().contiguous().clone()) for t in whole]
+    args = {"lr": 0.1, "weight_decay": 1e-2, "max_grad_norm": bound}
+    if name == "SGD":
+        args["momentum"] = 0.9
+    oa, ob = build_optimizer(name, a, **args), build_optimizer(name, b, **args)
+    for step in range(3):
+        for i, (p, q) in enumerate(zip(a, b)):
+            q.grad = randn(*q.shape, seed=10 * step + i + 3)
+            # one gradient laid out as the parameter, one dense
+            p.grad = parameter(10 * step + 4).detach().clone().copy_(q.grad) if i else q.grad.clone()
+        oa.step()
+        ob.step()
+    for p, q in zip(a, b):
+        assert not p.is_contiguous() and q.is_contiguous()
+        # up to eight roundings a step on each side, of values under 8; Adam's quotient doubles them
+        assert ((p - q).abs() <= 3 * 32 * U32 * 8).all()
