@@ -243,8 +243,8 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                         buf.mul_(momentum).add_(gf)
                         gf = buf
                     p.add_(gf, alpha=-lr)
-                    if self._persistent:
-                        g.zero_()
+                if self._persistent:
+                    g.zero_()
             if fused:
                 self._multi_tensor_step(ext, gi, fused, lr, momentum, wd, clip)
         return loss

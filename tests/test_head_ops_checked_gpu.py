@@ -200,3 +200,15 @@ def test_parameters_of_any_strides(name, bound, layout):
         assert not p.is_contiguous() and q.is_contiguous()
         # up to eight roundings a step on each side, of values under 8; Adam's quotient doubles them
         assert ((p - q).abs() <= 3 * 32 * U32 * 8).all()
+
+
+def test_persistent_gradients_are_used_once():
+    """In persistent-gradient mode the step zeroes every gradient, also one whose strides
+    take it through the per-tensor kernel."""
+    from active_learning_amd.ops.optim import FusedSGD
+    p = torch.nn.Parameter(randn(30, 40, seed=1))
+    p.grad = randn(40, 30, seed=2).t()
+    opt = FusedSGD([p], lr=0.1)
+    opt.enable_persistent_grads()
+    opt.step()
+    assert not p.grad.any()
