@@ -19,7 +19,7 @@ ops/linear.py, for heads and pools large enough that its rate counts.
 """
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from .extension import require_extension
@@ -156,6 +156,14 @@ def _quantize_cpu(x, kind, tile):
     if cols == 0:  # the transpose of no rows
         return Fp8Blocks._of(values, scale, x.shape, tile)
     return Fp8Blocks(values, scale, tile)
+
+
+def no_tangent(name, *tensors):
+    """Refuses dual tensors, whose output without a tangent would read as a derivative
+    of zero."""
+    if torch._C._is_fwd_grad_enabled() and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _matrix(x, name):
@@ -301,6 +309,7 @@ def fp8_linear(x, weight, bias=None, scale="e8m0"):
         bias = bias.contiguous()
     if kept:
         _check_product(weight.scale_kind, flat.shape[1], x.device, weight, bias)
+        no_tangent("fp8_linear", x, bias)
         if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
             raise RuntimeError("a weight kept in Fp8Blocks has no gradient: pass the weight "
                                "itself to train, or use torch.no_grad()")

@@ -6,6 +6,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -143,6 +144,16 @@ Tensor as_rows(const Tensor& t) {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
+// A dual tensor (forward-mode differentiation) need not ask for a gradient: its output
+// without a tangent would read as a derivative of zero.
+void no_tangent(const char* name, const Tensor& x, const OptTensor& y = std::nullopt,
+                const OptTensor& z = std::nullopt) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  const auto dual = [](const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!dual(x) && !(y && dual(*y)) && !(z && dual(*z)), name,
+                              " has no forward-mode derivative");
+}
+
 // Gradients that have none of their own: a second backward pass raises, as
 // once_differentiable does for a function in Python.
 torch::autograd::variable_list once(torch::autograd::variable_list grads,
@@ -238,6 +249,7 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
 // y, or y and the stored sum where there is a residual
 std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& w_in, const OptTensor& res, double eps) {
   check_norm(x, w_in, res, eps);
+  no_tangent("rms_norm", x, w_in, res);
   const Tensor w = w_in.contiguous();
   if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || (res && wants_grad(*res))))
     return RmsNorm::apply(x, w, res, eps);
@@ -251,6 +263,7 @@ std::vector<Tensor> rms_norm(const Tensor& x, const Tensor& w_in, const OptTenso
 std::vector<Tensor> rms_norm_quant(const Tensor& x_in, const Tensor& w_in, const OptTensor& res_in,
                                    double eps, long kind) {
   check_norm(x_in, w_in, res_in, eps);
+  no_tangent("rms_norm_fp8", x_in, w_in, res_in);
   TORCH_CHECK(!torch::GradMode::is_enabled() ||
                   !(wants_grad(x_in) || wants_grad(w_in) || (res_in && wants_grad(*res_in))),
               "rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to train, or torch.no_grad()");
@@ -468,6 +481,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const OptTensor& bias_in, lo
   TORCH_CHECK_TYPE(w.dim() == 2, "weight must be a matrix");
   const OptTensor bias = bias_in ? OptTensor(bias_in->contiguous()) : bias_in;
   check_linear(x, w.size(0), w.size(1), bias, w);
+  no_tangent("fp8_linear", x, w, bias);
   TORCH_CHECK_VALUE(x.is_cuda(), "x must be on the GPU");
   const bool grad = torch::GradMode::is_enabled();
   const bool need_x = grad && x.requires_grad(), need_w = grad && w.requires_grad();
@@ -488,6 +502,7 @@ Tensor fp8_linear_kept(const Tensor& x, const Tensor& b, const Tensor& sb, bool 
                        const OptTensor& bias_in) {
   const OptTensor bias = bias_in ? OptTensor(bias_in->contiguous()) : bias_in;
   check_linear(x, n, k, bias, b);
+  no_tangent("fp8_linear", x, bias);
   TORCH_CHECK(!torch::GradMode::is_enabled() || !(x.requires_grad() || (bias && bias->requires_grad())),
               "a weight kept in Fp8Blocks has no gradient: pass the weight itself to train, or use "
               "torch.no_grad()");

@@ -19,7 +19,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .extension import require_extension
-from .fp8 import Fp8Blocks, check_scale_kind, quantize_fp8
+from .fp8 import Fp8Blocks, check_scale_kind, no_tangent, quantize_fp8
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -108,6 +108,7 @@ def rms_norm_fp8(x, weight, residual=None, eps=1e-6, scale="e8m0"):
         blocks = Fp8Blocks._of(codes, scales, (codes.shape[0], x.shape[-1]), False)
         return blocks if residual is None else (blocks, total)
     _check(x, weight, residual, eps)
+    no_tangent("rms_norm_fp8", x, weight, residual)
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError("rms_norm_fp8 has no gradient: use rms_norm and fp8_linear to "

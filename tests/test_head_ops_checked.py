@@ -4,7 +4,9 @@ answered wrongly or forgotten, each with what it has to give."""
 import pytest
 import torch
 
+from active_learning_amd.ops.fp8 import fp8_linear, quantize_fp8
 from active_learning_amd.ops.optim import FusedSGD, build_optimizer
+from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
 
 
 def _params(sizes):
@@ -162,3 +164,36 @@ def test_a_bound_that_is_set_later_is_checked(name, bound):
     opt.max_grad_norm = None
     opt.step()
     assert opt.last_grad_norm is None
+
+
+def _with_tangents(device):
+    """Calls with one dual tensor each, by name."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(20, 8, device=device), torch.randn(8, device=device)
+    weight, bias = torch.randn(3, 8, device=device), torch.randn(3, device=device)
+    kept = quantize_fp8(weight, tile=True)
+
+    def dual(t):
+        return forward_ad.make_dual(t, torch.ones_like(t))
+
+    return {
+        "norm": lambda: rms_norm(dual(x), w), "norm's weight": lambda: rms_norm(x, dual(w)),
+        "residual": lambda: rms_norm(x, w, residual=dual(x)), "codes": lambda: rms_norm_fp8(dual(x), w),
+        "codes' residual": lambda: rms_norm_fp8(x, w, residual=dual(x)),
+        "linear": lambda: fp8_linear(dual(x), weight), "weight": lambda: fp8_linear(x, dual(weight)),
+        "bias": lambda: fp8_linear(x, weight, dual(bias)), "kept": lambda: fp8_linear(dual(x), kept),
+        "kept, one row": lambda: fp8_linear(dual(x[:1]), kept),
+        "kept weight's bias": lambda: fp8_linear(x, kept, dual(bias)),
+    }
+
+
+@pytest.mark.parametrize("name", list(_with_tangents("cpu")))
+def test_forward_mode_is_refused(name):
+    """An output without a tangent would read as a derivative of zero."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        call = _with_tangents("cpu")[name]
+        with pytest.raises(NotImplementedError):
+            call()
+        with torch.no_grad(), pytest.raises(NotImplementedError):  # it has no say in this mode
+            call()
