@@ -20,7 +20,6 @@ ops/linear.py, for heads and pools large enough that its rate counts.
 
 import torch
 from torch.autograd import Function, forward_ad
-from torch.autograd.function import once_differentiable
 
 from .extension import require_extension
 from .linear import NativeLinear
@@ -253,6 +252,25 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
     return _product(a, b, bias if bias is None else bias.detach().contiguous(), out_dtype)
 
 
+class _Once(Function):
+    @staticmethod
+    def forward(ctx, grad, name):
+        ctx.name = name
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} is differentiable once: its backward pass has no gradient")
+
+
+def once(grad, asked, name):
+    """A gradient that has none of its own though what it depends on asks for one
+    (``asked``): where it is to be differentiable, differentiating it raises."""
+    if grad is None or not asked or not torch.is_grad_enabled():
+        return grad
+    return _Once.apply(grad.detach().requires_grad_(), name)
+
+
 class _Fp8LinearCPU(Function):
     """y = Q(x) Q(w)^T + b,  dx = Q(dy) Q(w),  dw = Q(dy^T) Q(x^T)^T: each
     operand in blocks along its product's contraction. The weight's tiles are the
@@ -270,8 +288,16 @@ class _Fp8LinearCPU(Function):
         return _product(xq, wq, bias, x.dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        with torch.no_grad():
+            dx, dw, db = _Fp8LinearCPU.gradients(ctx, dy)
+        outer = dy.requires_grad
+        return (once(dx, outer or need_w, "fp8_linear"), once(dw, outer or need_x, "fp8_linear"),
+                once(db, outer, "fp8_linear"), None)
+
+    @staticmethod
+    def gradients(ctx, dy):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         xc, xs, wc, ws = ctx.saved_tensors
         dq, dt, db = _pair(dy, ctx.kind, False, need_x, need_w,
@@ -281,7 +307,7 @@ class _Fp8LinearCPU(Function):
             dx = _product(dq, Fp8Blocks._of(wc, ws, ctx.shapes[1], True), None, ctx.types[0])
         if need_w:
             dw = _product(dt, Fp8Blocks._of(xc, xs, ctx.shapes[0], False), None, ctx.types[1])
-        return dx, dw, db if need_b else None, None
+        return dx, dw, db if need_b else None
 
 
 def fp8_linear(x, weight, bias=None, scale="e8m0"):

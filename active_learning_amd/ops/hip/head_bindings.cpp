@@ -154,18 +154,13 @@ void no_tangent(const char* name, const Tensor& x, const OptTensor& y = std::nul
                               " has no forward-mode derivative");
 }
 
-// Gradients that have none of their own: a second backward pass raises, as
-// once_differentiable does for a function in Python.
-torch::autograd::variable_list once(torch::autograd::variable_list grads,
-                                    const torch::autograd::variable_list& outer, const char* name) {
-  if (!torch::GradMode::is_enabled() ||
-      !std::any_of(outer.begin(), outer.end(), [](const Tensor& t) { return wants_grad(t); }))
-    return grads;
-  torch::autograd::variable_list fake;
-  for (auto& g : grads) fake.push_back(g.defined() ? g.detach().requires_grad_() : g);
+// A gradient that has none of its own though what it depends on asks for one (`asked`):
+// where it is to be differentiable, differentiating it raises.
+Tensor once(const Tensor& grad, bool asked, const char* name) {
+  if (!grad.defined() || !asked || !torch::GradMode::is_enabled()) return grad;
   auto stop = std::make_shared<torch::autograd::DelayedError>(
-      std::string(name) + " is differentiable once: its backward pass has no gradient", (int)fake.size());
-  return (*stop)(std::move(fake));
+      std::string(name) + " is differentiable once: its backward pass has no gradient", 1);
+  return (*stop)({grad.detach().requires_grad_()})[0];
 }
 
 struct NormOut {
@@ -208,6 +203,8 @@ std::pair<Tensor, Tensor> norm_rows_bwd(const Tensor& s, const Tensor& w, const 
   return {dx, dw};
 }
 
+enum : int64_t { kResidual = 1, kRowsAsk = 2, kWeightAsks = 4 };
+
 struct RmsNorm : public torch::autograd::Function<RmsNorm> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x,
                                                 const Tensor& w, const OptTensor& res, double eps) {
@@ -217,7 +214,9 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
     const NormOut o = norm_rows(rows, w, res ? OptTensor(as_rows(*res)) : res, eps, true, x.sizes());
     // the sum as it goes out, not a view of it: a change in place is noticed
     ctx->save_for_backward({res ? o.total : rows, w, o.rstd});
-    ctx->saved_data["residual"] = res.has_value();
+    // which inputs ask for a gradient, whichever of them a backward pass is for
+    const bool rows_ask = wants_grad(x) || (res && wants_grad(*res));
+    ctx->saved_data["what"] = (res ? kResidual : 0) | (rows_ask ? kRowsAsk : 0) | (wants_grad(w) ? kWeightAsks : 0);
     if (!res) return {o.y};
     return {o.y, o.total};
   }
@@ -226,7 +225,8 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor total = as_rows(saved[0]), &w = saved[1], &rstd = saved[2];
-    const bool res = ctx->saved_data["residual"].toBool();
+    const int64_t what = ctx->saved_data["what"].toInt();
+    const bool res = what & kResidual;
     const bool need_w = ctx->needs_input_grad(1);
     Tensor dy = grads[0], dsum = res ? grads[1] : Tensor();
     c10::OptionalDeviceGuard guard(total.device());
@@ -241,8 +241,13 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
       std::tie(dx, dw) = norm_rows_bwd(total, w, rstd, dy, dsum, need_w);
       dx = dx.view(shape);
     }
-    return once({ctx->needs_input_grad(0) ? dx : Tensor(), dw,
-                 res && ctx->needs_input_grad(2) ? dx : Tensor(), Tensor()}, grads, "rms_norm");
+    const bool need_x = ctx->needs_input_grad(0), need_r = res && ctx->needs_input_grad(2);
+    if (grads[0].defined()) {  // otherwise dx is the sum's gradient itself
+      const bool outer = wants_grad(grads[0]) || (res && wants_grad(grads[1]));
+      dx = once(dx, outer || what & (kRowsAsk | kWeightAsks), "rms_norm");
+      dw = once(dw, outer || what & kRowsAsk, "rms_norm");
+    }
+    return {need_x ? dx : Tensor(), dw, need_r ? dx : Tensor(), Tensor()};
   }
 };
 
@@ -433,6 +438,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     ctx->save_for_backward({xq[2], xq[3], wq[2], wq[3]});
     ctx->saved_data["k"] = k;
     ctx->saved_data["kind"] = kind;
+    ctx->saved_data["asks"] = (need_x ? kRowsAsk : 0) | (need_w ? kWeightAsks : 0);
     ctx->saved_data["w"] = (int64_t)w.scalar_type();
     ctx->saved_data["x"] = (int64_t)x.scalar_type();
     ctx->saved_data["bias"] = bias ? (int64_t)value(bias).scalar_type() : -1;
@@ -463,7 +469,10 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     if (need_w)
       dw = fp8_gemm(dq[2], dq[3], saved[0], saved[1], false, n, k, m, std::nullopt,
                     (torch::ScalarType)ctx->saved_data["w"].toInt());
-    return once({dx, dw, need_b ? dq[4] : Tensor(), Tensor(), Tensor(), Tensor()}, grads, "fp8_linear");
+    const bool outer = wants_grad(grads[0]);
+    const int64_t asks = ctx->saved_data["asks"].toInt();
+    return {once(dx, outer || asks & kWeightAsks, "fp8_linear"), once(dw, outer || asks & kRowsAsk, "fp8_linear"),
+            need_b ? once(dq[4], outer, "fp8_linear") : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 

@@ -16,10 +16,9 @@ heads, whose rows are independent of the batch.
 import torch
 import torch.nn as nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from .extension import require_extension
-from .fp8 import Fp8Blocks, check_scale_kind, no_tangent, quantize_fp8
+from .fp8 import Fp8Blocks, check_scale_kind, no_tangent, once, quantize_fp8
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -63,13 +62,21 @@ class _RMSNormCPU(Function):
         return y if residual is None else (y, total)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dsum=None):
-        total, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r, _ = ctx.needs_input_grad
         if dy is None:  # only the sum was used
-            dw = torch.zeros_like(weight) if need_w else None
-            return dsum if need_x else None, dw, dsum if need_r else None, None
+            dx, dw = dsum, torch.zeros_like(ctx.saved_tensors[1])
+        else:
+            with torch.no_grad():
+                dx, dw = _RMSNormCPU.gradients(ctx, dy, dsum)
+            outer = dy.requires_grad or (dsum is not None and dsum.requires_grad)
+            dx = once(dx, outer or need_x or need_r or need_w, "rms_norm")
+            dw = once(dw, outer or need_x or need_r, "rms_norm")
+        return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
+
+    @staticmethod
+    def gradients(ctx, dy, dsum):
+        total, weight, rstd = ctx.saved_tensors
         u = total.float() * rstd
         g = dy.float() * weight.float()
         dx = (g - u * (g * u).mean(-1, keepdim=True)) * rstd
@@ -77,7 +84,7 @@ class _RMSNormCPU(Function):
             dx = dx + dsum.float()
         dx = dx.to(total.dtype)
         dw = (dy.float() * u).reshape(-1, u.shape[-1]).sum(0).to(weight.dtype)
-        return dx if need_x else None, dw if need_w else None, dx if need_r else None, None
+        return dx, dw
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6):

@@ -247,3 +247,38 @@ def test_forward_mode_is_refused(name):
             call()
         with torch.no_grad(), pytest.raises(NotImplementedError):  # it has no say in this mode
             call()
+
+
+@pytest.mark.parametrize("device", ["cuda"])
+def test_second_gradients_are_refused_not_zero(device):
+    """A penalty on a gradient would have no effect; what does not depend on anything that
+    asks for a gradient may be used as the constant that it is."""
+    x, r, w = (torch.randn(*s, device=device).requires_grad_() for s in ((20, 8), (20, 8), (8,)))
+    weight = torch.randn(3, 8, device=device).requires_grad_()
+    bias = torch.randn(3, device=device).requires_grad_()
+    cases = [
+        (lambda: rms_norm(x, w), (x, w)), (lambda: rms_norm(x, w), (x,)), (lambda: rms_norm(x, w.detach()), (x,)),
+        (lambda: rms_norm(x, w), (w,)), (lambda: rms_norm(x.detach(), w, residual=r)[0], (r, w)),
+        (lambda: sum(rms_norm(x, w, residual=r)), (x, r, w)),
+        (lambda: fp8_linear(x, weight, bias), (x,)), (lambda: fp8_linear(x, weight, bias), (weight,)),
+    ]
+    for f, leaves in cases:
+        want = torch.autograd.grad(f().sum(), leaves)
+        grads = torch.autograd.grad(f().sum(), leaves, create_graph=True)
+        for g, v in zip(grads, want):
+            assert torch.equal(g, v)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                g.square().sum().backward(retain_graph=True)
+    constants = [
+        (lambda: rms_norm(x.detach(), w), w), (lambda: fp8_linear(x, weight.detach()), x),
+        (lambda: fp8_linear(x.detach(), weight), weight), (lambda: fp8_linear(x, weight, bias), bias),
+        (lambda: rms_norm(x, w, residual=r)[1], x),
+    ]
+    for f, leaf in constants:
+        (g,) = torch.autograd.grad(f().sum(), leaf, create_graph=True)
+        assert not g.requires_grad
+    # the sum's gradient goes through as it is
+    dsum = torch.randn(20, 8, device=device).requires_grad_()
+    (g,) = torch.autograd.grad(rms_norm(x, w, residual=r)[1], r, dsum, create_graph=True)
+    (back,) = torch.autograd.grad(g.square().sum(), dsum)
+    assert torch.equal(back, 2 * dsum)
