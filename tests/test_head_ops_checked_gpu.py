@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from active_learning_amd.ops.extension import require_extension
-from active_learning_amd.ops.fp8 import fp8_linear, quantize_fp8
+from active_learning_amd.ops.fp8 import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8
 from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
 
 pytestmark = pytest.mark.gpu
@@ -282,3 +282,95 @@ def test_second_gradients_are_refused_not_zero(device):
     (g,) = torch.autograd.grad(rms_norm(x, w, residual=r)[1], r, dsum, create_graph=True)
     (back,) = torch.autograd.grad(g.square().sum(), dsum)
     assert torch.equal(back, 2 * dsum)
+
+
+# every kernel of the products: 32x32 tiles straight from memory, 64x64 (whole and split), 128x128 in
+# four stages and in two, 128x256, 256x256, and a last round of smaller tiles behind 256x256
+SHAPES = [(20, 40, 512), (500, 500, 4100), (1500, 1300, 600), (2048, 2048, 2176), (3500, 2100, 700), (4099, 2100, 2100),
+          (4200, 4352, 384), (4096, 4452, 2100), (2500, 2501, 2100)]
+
+
+def relative(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("size", [1e-19, 3e-19, 1e-17])
+def test_small_operands_keep_their_bits(m, n, k, size, kind):
+    """Operands whose scales' product has no place in 32 bits, though the results have: off by
+    roundings as at any other magnitude."""
+    x, w = randn(m, k, seed=1) * size, randn(n, k, seed=2) * size
+    a, av = quantize_fp8(x, scale=kind), None
+    for tile in (True, False):
+        b = quantize_fp8(w, tile=tile, scale=kind)
+        av, bv = a.dequantize(torch.float64), b.dequantize(torch.float64)
+        want = av @ bv.t()
+        # below the normal range a sum, a product or an output is off by half a step, 2^-150, for
+        # each of its k products and k / 128 blocks, which add up as the root of their count
+        least = 2.0 ** -150 * (2 * k) ** 0.5 / want.square().mean().sqrt().item()
+        got = fp8_matmul(a, b, out_dtype=torch.float32)
+        assert relative(got, want) <= 4 * (k + 20) ** 0.5 * U32 + 4 * least
+        got = fp8_matmul(a, b, out_dtype=torch.bfloat16)
+        # the 8-bit instruction's own loss, 2e-4 at most, a rounding, and half a step at its end
+        assert relative(got, want) <= 2.0 ** -8 + 2e-4 + 4 * least + 2.0 ** -134 / want.square().mean().sqrt().item()
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_scales_of_any_value(m, n, k):
+    """Scales that a caller brings: near the ends of both kinds' ranges, zero, negative, below
+    the normal range, NaN; each meets one that brings the result back into range, and others."""
+    codes_a = quantize_fp8(randn(m, k, seed=1)).values
+    codes_b = quantize_fp8(randn(n, k, seed=2)).values
+    blocks = -(-k // 128)
+
+    def check(kind, rows, tile):
+        sa = torch.full((m, blocks), 1.0, device="cuda")
+        sb = torch.full((-(-n // 128) if tile else n, blocks), 1.0, device="cuda")
+        for i, (va, vb) in enumerate(rows):
+            sa[i % m] = va
+            sb[i % len(sb)] = vb
+        if kind == "e8m0":
+            a, b = (Fp8Blocks(c, s.to(torch.float8_e8m0fnu), tile=t) for c, s, t in ((codes_a, sa, False), (codes_b, sb, tile)))
+            sa, sb = a.scale.float(), b.scale.float()
+        else:
+            a, b = Fp8Blocks(codes_a, sa), Fp8Blocks(codes_b, sb, tile=tile)
+        # the scales as 64-bit numbers, since products of the dequantised values may leave 32 bits
+        spread = lambda s, r: s.double().repeat_interleave(128, 1)[:, :k]  # noqa: E731
+        av = codes_a.double() * spread(sa, m)
+        bv = codes_b.double() * (spread(sb, n).repeat_interleave(128, 0)[:n] if tile else spread(sb, n))
+        want = av @ bv.t()
+        size = av.abs() @ bv.abs().t()
+        for out in (torch.float32, torch.bfloat16):
+            got = fp8_matmul(a, b, out_dtype=out)
+            assert torch.isnan(got)[torch.isnan(want)].all()
+            inside = size < 3.3e38  # no sum on the way leaves the range
+            assert torch.isfinite(got[inside]).all()
+            loss = (k + 20) * 2 * U32 if out == torch.float32 else 2.0 ** -8 + 2.0 ** -10 + (k + 20) * 2 * U32
+            least = 2.0 ** -150 * 2 * k if out == torch.float32 else 2.0 ** -134 + 2.0 ** -150 * 2 * k
+            off = (got.double() - want).abs()
+            assert (off[inside] <= loss * size[inside] + least).all(), (off[inside] / (loss * size[inside] + least)).max()
+            assert not torch.isfinite(got[want.abs() > 3.5e38]).any()
+
+    for tile in (True, False):
+        check("e8m0", [(2.0 ** -127, 2.0 ** 60), (2.0 ** 119, 2.0 ** -119), (2.0 ** -60, 2.0 ** -60),
+                       (float("nan"), 1.0), (2.0 ** 100, 1.0)], tile)
+        check("fp32", [(2.0 ** -127, 2.0 ** 100), (1.5 * 2.0 ** 119, 2.0 ** -119), (2.0 ** -70, 1.25 * 2.0 ** -60),
+                       (0.0, 1.0), (-3.0, 2.0 ** -140), (2.0 ** -149, 2.0 ** 120), (float("nan"), 1.0), (3e38, 1e-38)], tile)
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [40, 9000, 17000])
+def test_small_operands_of_few_rows_keep_their_bits(n, dtype, kind):
+    k = 1100
+    x, w = randn(7, k, seed=1, dtype=torch.float32).mul(1e-19).to(dtype), randn(n, k, seed=2) * 1e-19
+    a = quantize_fp8(x, scale=kind).dequantize(torch.float64)
+    for tile in (True, False):
+        b = quantize_fp8(w, tile=tile, scale=kind)
+        want = a @ b.dequantize(torch.float64).t()
+        got = fp8_linear(x, b)
+        rms = want.square().mean().sqrt().item()
+        least = 2.0 ** -150 * (2 * k) ** 0.5 / rms
+        loss = 4 * (k + 20) ** 0.5 * U32 if dtype == torch.float32 else 2.0 ** -8 + 2e-4 + 2.0 ** -134 / rms
+        assert relative(got, want) <= loss + 4 * least
