@@ -36,8 +36,12 @@ constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 // the grid so that the weight stays in registers. VPT == 0: rows of any length,
 // read twice.
 //
-// In front of an e4m3 output the sum is held in 64 bits, and 1 / root and the first
-// product as pairs of floats: y is then the exact value rounded once, and a value next
+// Squares are summed in 64 bits: those of values over 1.8e19 leave the range of 32, and a
+// row of finite values would become zeros. (Where the root is over 2^126, 1 / root is below
+// the normal range and has 21 bits.)
+//
+// In front of an e4m3 output 1 / root and the first
+// product are held as pairs of floats: y is then the exact value rounded once, and a value next
 // to a border between two codes or scales falls on its own side of it (with 32 bits throughout,
 // 50 codes in 123 million did not). At 130000x2048 in bf16 with a residual that costs
 // 355 us against 336, at 5.3 and 5.5 TB/s; the reductions go through lane permutations
@@ -54,8 +58,7 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
                                unsigned char* __restrict__ q, void* __restrict__ scale,
                                long rows, int dim, int pitch, int scale_stride,
                                float eps) {
-  typedef typename std::conditional<OUT == kOutPlain, float, double>::type Sum;
-  __shared__ Sum lds[16];
+  __shared__ double lds[16];
   constexpr int RPB = block_of(TPR) / TPR;
   constexpr int N = VPT ? VPT : 1;
   const int t = threadIdx.x % TPR;
@@ -71,7 +74,7 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
     const long r = r0 + threadIdx.x / TPR;
     if (RPB > 1 && r >= rows) break;  // whole waves; no barrier when RPB > 1
     f32x8 v[N];
-    Sum ss = 0;
+    double ss = 0;
     auto take = [&](int c) {
       f32x8 f = load8_upto(x + r * x_stride + c, dim - c);
       if (RES) {
@@ -86,20 +89,15 @@ __global__ void rms_fwd_kernel(const T* __restrict__ x, long x_stride,
       for (int k = i; k < sweeps; k += N) {
         v[i] = take((k * TPR + t) * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += (Sum)v[i][j] * (Sum)v[i][j];
+        for (int j = 0; j < 8; ++j) ss += (double)v[i][j] * (double)v[i][j];
       }
     }
     ss = row_sum<TPR>(ss, lds);
-    float rstd, rstd_low = 0.f;
-    if (OUT == kOutPlain) {
-      rstd = 1.f / sqrtf((float)ss / (float)dim + eps);
-    } else {  // the hardware's root has 23 bits; a step of Newton's method doubles them
-      const double mean = (double)ss * per_value + (double)eps;
-      double r = __builtin_amdgcn_rsq(mean);
-      if (!isinf(mean)) r *= 1.5 - 0.5 * mean * r * r;
-      rstd = (float)r;
-      rstd_low = (float)(r - (double)rstd);
-    }
+    // the hardware's root has 23 bits; a step of Newton's method doubles them
+    const double mean = ss * per_value + (double)eps;
+    double root = __builtin_amdgcn_rsq(mean);
+    if (!isinf(mean)) root *= 1.5 - 0.5 * mean * root * root;
+    const float rstd = (float)root, rstd_low = (float)(root - (double)rstd);
     if (rstd_out && t == 0) rstd_out[r] = rstd;
 #pragma unroll
     for (int i = 0; i < N; ++i) {

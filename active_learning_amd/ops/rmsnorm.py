@@ -4,8 +4,8 @@
     y = s * rstd * weight
 
 The norm is that of the rounded sum, which is also what comes back for the next
-residual and what the backward pass reads. Arithmetic is in 32 bits or more (64 in
-front of an e4m3 output) and rounded to the type once. GPU tensors run rmsnorm.hip;
+residual and what the backward pass reads. Squares are summed in 64 bits; the other
+arithmetic is in 32 (64 in front of an e4m3 output) and rounded to the type once. GPU tensors run rmsnorm.hip;
 CPU tensors run the torch math below, which defines the semantics that the kernels
 are tested against.
 
@@ -47,9 +47,9 @@ def _check(x, weight, residual, eps):
 
 def _forward_cpu(x, weight, residual, eps, wide=torch.float32):
     total = x if residual is None else (x.float() + residual.float()).to(x.dtype)
-    s = total.to(wide)
-    rstd = 1.0 / torch.sqrt(s.square().mean(-1, keepdim=True) + eps)
-    return s * rstd * weight.to(wide), total, rstd
+    mean = total.double().square().mean(-1, keepdim=True)  # squares may leave the range of 32 bits
+    rstd = (1.0 / torch.sqrt(mean + eps)).to(wide)
+    return total.to(wide) * rstd * weight.to(wide), total, rstd
 
 
 class _RMSNormCPU(Function):

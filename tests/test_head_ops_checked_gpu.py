@@ -374,3 +374,38 @@ def test_small_operands_of_few_rows_keep_their_bits(n, dtype, kind):
         least = 2.0 ** -150 * (2 * k) ** 0.5 / rms
         loss = 4 * (k + 20) ** 0.5 * U32 if dtype == torch.float32 else 2.0 ** -8 + 2e-4 + 2.0 ** -134 / rms
         assert relative(got, want) <= loss + 4 * least
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e19, 3e19, 1e20, 1e30, 1e37])
+@pytest.mark.parametrize("dim", [8, 300, 2048, 5000, 40000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_norm_of_large_and_small_values(dim, size, dtype):
+    """Squares that leave the range of 32 bits: the norm is that of any other row, forward,
+    backward and in front of codes."""
+    x = (torch.randn(3, dim, device="cuda") * size).to(dtype).requires_grad_()
+    w = (torch.rand(dim, device="cuda") + 0.5).requires_grad_()
+    dy = torch.randn(3, dim, device="cuda").to(dtype)
+    eps = 1e-6 if size > 1 else 1e-38  # the smallest normal one and a root that counts in 64 bits
+    y = rms_norm(x, w, eps=eps)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    s = x.detach().double()
+    root = (s.square().mean(-1, keepdim=True) + torch.tensor(eps).double().item()).sqrt()
+    u, g = s / root, dy.double() * w.detach().double()
+    half = torch.finfo(dtype).eps / 2
+    # 1 / root, two products and a rounding; the dot product's 32-bit sum of dim / 1024 + 24 terms
+    # behind each other at most, which the gradients are off by as well (CPU: pairwise sums, fewer)
+    many = (dim / 1024 + 24) * 2.0 ** -24
+    want = u * w.detach().double()
+    assert ((y.double() - want).abs() <= (half + 4 * 2.0 ** -24) * want.abs() + 2.0 ** -133).all()
+    dot = (g * u).mean(-1, keepdim=True)
+    want = (g - u * dot) / root
+    scale = (g.abs() + u.abs() * (g * u).abs().mean(-1, keepdim=True)) / root
+    least = 2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -148
+    assert ((dx.double() - want).abs() <= half * want.abs() + 4 * many * scale + least).all()
+    want = (dy.double() * u).sum(0)
+    assert ((dw.double() - want).abs() <= 6 * 2.0 ** -24 * (dy.double() * u).abs().sum(0)).all()
+    with torch.no_grad():
+        q = rms_norm_fp8(x, w, eps=eps)
+    spread = q.scale.double().repeat_interleave(128, 1)[:, :dim]
+    want = u * w.detach().double()
+    assert ((q.values.double() * spread - want).abs() <= (2.0 ** -4 + 2.0 ** -20) * want.abs() + 2.0 ** -10 * spread).all()
