@@ -184,7 +184,7 @@ def _pair(x, kind, tile, plain, transposed, sums=None):
     x = x.float()
     return (_quantize_cpu(x, kind, tile) if plain else None,
             _quantize_cpu(x.t(), kind, tile) if transposed else None,
-            x.sum(0).to(sums) if sums is not None else None)
+            x.sum(0, dtype=torch.float64).float().to(sums) if sums is not None else None)
 
 
 def quantize_fp8(x, tile=False, scale="e8m0"):

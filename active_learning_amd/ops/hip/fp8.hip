@@ -44,7 +44,7 @@ __global__ void quant_rows_kernel(const T* __restrict__ x, long row_stride, long
 // 128x128 tiles, each read once, 8x8 values a thread, the next one's while this one is
 // worked on. Writes a tile's codes by rows (q), and transposed (qt), with blocks along
 // the rows that each is stored in; with TILE one scale serves all of it. part: sums of
-// each column over the tile's rows, for the gradient of a bias. By rows and transposed
+// each column over the tile's rows in 64 bits, for the gradient of a bias. By rows and transposed
 // 8192x4096 in bf16 takes 23 us (its bytes at a copy's rate: 25), 16384x8192 121 (100),
 // with 32-bit scales 27 and 128.
 template <typename T, int KIND, bool TILE>
@@ -53,10 +53,10 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
                                   unsigned char* __restrict__ q, void* __restrict__ scale,
                                   int pitch, int scale_stride,
                                   unsigned char* __restrict__ qt, void* __restrict__ scale_t,
-                                  int pitch_t, int scale_t_stride, float* __restrict__ part,
+                                  int pitch_t, int scale_t_stride, double* __restrict__ part,
                                   int across, int tiles) {
   constexpr bool WIDE = std::is_same<T, float>::value;
-  // column maxima (16-bit types: of two columns a word) or sums of each 8 rows
+  // column maxima (16-bit types: of two columns a word) of each 8 rows
   __shared__ unsigned words[16][kQB];
   __shared__ unsigned col_code[kQB];
   // a column's eight bytes of rows 8u .. 8u + 7 lie at u ^ (column >> 3): lanes that
@@ -117,16 +117,19 @@ __global__ void quant_tile_kernel(const T* __restrict__ x, long row_stride, int 
       }
     }
     if (part) {
-      f32x8 s = unpack<T>(v[0]);
+      double* sums = (double*)bytes;  // of each 8 rows, in the codes' place
 #pragma unroll
-      for (int j = 1; j < 8; ++j) s += unpack<T>(v[j]);
+      for (int i = 0; i < 8; ++i) {
+        double s = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) words[rg][c8 * 8 + i] = __float_as_uint(s[i]);
+        for (int j = 0; j < 8; ++j) s += (double)(float)__builtin_bit_cast(typename Vec8<T>::V, v[j])[i];
+        sums[rg * kQB + c8 * 8 + i] = s;
+      }
       __syncthreads();
       if (t < kQB && c0 + t < cols) {
-        float s = 0.f;
+        double s = 0;
 #pragma unroll
-        for (int g = 0; g < 16; ++g) s += __uint_as_float(words[g][t]);
+        for (int g = 0; g < 16; ++g) s += sums[g * kQB + t];
         part[(long)by * cols + c0 + t] = s;
       }
       __syncthreads();
@@ -248,7 +251,7 @@ extern "C" void al_quant_rows(int type, int kind, const void* x, long row_stride
 extern "C" void al_quant_tile(int type, int kind, int tile, const void* x, long row_stride,
                               int rows, int cols, void* q, void* scale, int pitch,
                               int scale_stride, void* qt, void* scale_t, int pitch_t,
-                              int scale_t_stride, float* part, hipStream_t stream) {
+                              int scale_t_stride, double* part, hipStream_t stream) {
   const int across = (cols + kQB - 1) / kQB, tiles = across * ((rows + kQB - 1) / kQB);
   // as many as are resident, 32-bit scales' registers leaving three blocks a unit (fp32
   // input, two: 1024 blocks are two even rounds)

@@ -29,12 +29,12 @@ int al_rms_bwd_parts(int type, long rows, int dim);
 void al_rms_bwd(int type, int wtype, const void* s, long s_stride, const void* dy,
                 const void* dsum, const void* w, const float* rstd, void* dx, float* part,
                 void* dw, int parts, long rows, int dim, void* stream);
-void al_col_sum(const float* part, void* out, int type, int parts, int dim, void* stream);
+void al_col_sum(const double* part, void* out, int type, int parts, int dim, void* stream);
 void al_quant_rows(int type, int kind, const void* x, long row_stride, long col_stride, void* q,
                    void* scale, long rows, int dim, int pitch, int scale_stride, void* stream);
 void al_quant_tile(int type, int kind, int tile, const void* x, long row_stride, int rows,
                    int cols, void* q, void* scale, int pitch, int scale_stride, void* qt,
-                   void* scale_t, int pitch_t, int scale_t_stride, float* part, void* stream);
+                   void* scale_t, int pitch_t, int scale_t_stride, double* part, void* stream);
 int al_fp8_gemm_splits(int kind, int out_type, int m, int n, int blocks);
 void al_fp8_gemm(int kind, const void* a, const void* sa, long lda, int sa_stride, const void* b,
                  const void* sb, long ldb, int sb_stride, int b_tile, int m, int n, int blocks,
@@ -330,15 +330,15 @@ std::vector<Tensor> fp8_quant_tile(const Tensor& x, long kind, bool tile, bool p
     if (sums) sum.zero_();
     return {q, scale, qt, scale_t, sum};
   }
-  if (sums) part = fresh({blocks_of(rows), cols}, torch::kFloat32, x);
+  if (sums) part = fresh({blocks_of(rows), cols}, torch::kFloat64, x);
   al_quant_tile(type, (int)kind, tile, x.data_ptr(), row_stride(x), (int)rows, (int)cols,
                 plain ? q.data_ptr() : nullptr, plain ? scale.data_ptr() : nullptr,
                 plain ? (int)q.size(1) : 0, plain ? (int)scale.size(1) : 0,
                 transposed ? qt.data_ptr() : nullptr, transposed ? scale_t.data_ptr() : nullptr,
                 transposed ? (int)qt.size(1) : 0, transposed ? (int)scale_t.size(1) : 0,
-                sums ? part.data_ptr<float>() : nullptr, cur_stream());
+                sums ? part.data_ptr<double>() : nullptr, cur_stream());
   if (sums)
-    al_col_sum(part.data_ptr<float>(), sum.data_ptr(), type_of(sum, "sum"), (int)part.size(0),
+    al_col_sum(part.data_ptr<double>(), sum.data_ptr(), type_of(sum, "sum"), (int)part.size(0),
                (int)cols, cur_stream());
   check_launch("quantize_fp8");
   return {q, scale, qt, scale_t, sum};

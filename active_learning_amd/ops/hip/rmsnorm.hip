@@ -250,23 +250,24 @@ __global__ void rms_dw_kernel(const T* __restrict__ s, long s_stride,
   part[(long)blockIdx.y * dim + c] = sum;
 }
 
-// out[c] = sum over p of part[p][c]: 16 columns a block, the partial rows over 64
-// threads each, joined in order
-template <typename W>
+// out[c] = sum over p of part[p][c] in 64 bits: 16 columns a block, the partial rows over
+// 64 threads each, joined in order
+template <typename P, typename W>
 __launch_bounds__(1024)
-__global__ void col_sum_kernel(const float* __restrict__ part, W* __restrict__ out,
+__global__ void col_sum_kernel(const P* __restrict__ part, W* __restrict__ out,
                                int parts, int dim) {
-  __shared__ float lds[64][17];
+  __shared__ double lds[64][17];
   const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
-  float s = 0.f;
+  double s = 0;
   if (c < dim)
-    for (int p = y; p < parts; p += 64) s += part[(long)p * dim + c];
+    for (int p = y; p < parts; p += 64) s += (double)part[(long)p * dim + c];
   lds[y][x] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && c < dim) {
-    for (int i = 1; i < 64; ++i) s += lds[i][x];
-    out[c] = (W)s;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    __syncthreads();
+    if (y < o) lds[y][x] += lds[y + o][x];
   }
+  if (y == 0 && c < dim) out[c] = (W)(float)lds[0][x];
 }
 
 struct Shape { int tpr, vpt; };
@@ -364,7 +365,7 @@ void bwd(const void* s, long s_stride, const void* dy, const void* dsum, const v
                          (const T*)s, s_stride, (const T*)dy, rstd, part, rows, dim);
   });
   if (dw)
-    hipLaunchKernelGGL(col_sum_kernel<W>, dim3((dim + 15) / 16), dim3(1024), 0, stream, part,
+    hipLaunchKernelGGL((col_sum_kernel<float, W>), dim3((dim + 15) / 16), dim3(1024), 0, stream, part,
                        (W*)dw, parts, dim);
 }
 
@@ -405,13 +406,13 @@ extern "C" void al_rms_bwd(int type, int wtype, const void* s, long s_stride,
   });
 }
 
-extern "C" void al_col_sum(const float* part, void* out, int type, int parts, int dim,
+extern "C" void al_col_sum(const double* part, void* out, int type, int parts, int dim,
                            hipStream_t stream) {
   const dim3 grid((dim + 15) / 16), block(1024);
   if (type == kTypeF32)
-    hipLaunchKernelGGL(col_sum_kernel<float>, grid, block, 0, stream, part, (float*)out, parts, dim);
+    hipLaunchKernelGGL((col_sum_kernel<double, float>), grid, block, 0, stream, part, (float*)out, parts, dim);
   else if (type == kTypeBF16)
-    hipLaunchKernelGGL(col_sum_kernel<__bf16>, grid, block, 0, stream, part, (__bf16*)out, parts, dim);
+    hipLaunchKernelGGL((col_sum_kernel<double, __bf16>), grid, block, 0, stream, part, (__bf16*)out, parts, dim);
   else
-    hipLaunchKernelGGL(col_sum_kernel<_Float16>, grid, block, 0, stream, part, (_Float16*)out, parts, dim);
+    hipLaunchKernelGGL((col_sum_kernel<double, _Float16>), grid, block, 0, stream, part, (_Float16*)out, parts, dim);
 }

@@ -267,3 +267,19 @@ def test_norm_of_large_and_small_values(dim, size, dtype):
     spread = q.scale.double().repeat_interleave(128, 1)[:, :dim]
     want = u * w.detach().double()
     assert ((q.values.double() * spread - want).abs() <= (2.0 ** -4 + 2.0 ** -20) * want.abs() + 2.0 ** -10 * spread).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 20), (8000, 300)])
+def test_bias_gradient_is_rounded_once(rows, cols):
+    """Its sum is held in 64 bits: off by the one rounding to its type."""
+    x, w = torch.randn(rows, 64, device="cpu"), torch.randn(cols, 64, device="cpu")
+    for dtype in (torch.float32, torch.bfloat16):
+        bias = torch.zeros(cols, device="cpu", dtype=dtype).requires_grad_()
+        for kind in ("e8m0", "fp32"):
+            y = fp8_linear(x, w, bias, scale=kind)
+            dy = torch.randn_like(y)
+            (db,) = torch.autograd.grad(y, bias, dy)
+            want, size = dy.double().sum(0), dy.double().abs().sum(0)
+            # a 16-bit one through 32 bits
+            half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8 + 2.0 ** -23
+            assert ((db.double() - want).abs() <= half * want.abs() + rows * 2.0 ** -52 * size).all()

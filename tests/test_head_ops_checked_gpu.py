@@ -409,3 +409,30 @@ def test_norm_of_large_and_small_values(dim, size, dtype):
     spread = q.scale.double().repeat_interleave(128, 1)[:, :dim]
     want = u * w.detach().double()
     assert ((q.values.double() * spread - want).abs() <= (2.0 ** -4 + 2.0 ** -20) * want.abs() + 2.0 ** -10 * spread).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 20), (8000, 300)])
+def test_bias_gradient_is_rounded_once(rows, cols):
+    """Its sum is held in 64 bits: off by the one rounding to its type."""
+    x, w = torch.randn(rows, 64, device="cuda"), torch.randn(cols, 64, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        bias = torch.zeros(cols, device="cuda", dtype=dtype).requires_grad_()
+        for kind in ("e8m0", "fp32"):
+            y = fp8_linear(x, w, bias, scale=kind)
+            dy = torch.randn_like(y)
+            (db,) = torch.autograd.grad(y, bias, dy)
+            want, size = dy.double().sum(0), dy.double().abs().sum(0)
+            # a 16-bit one through 32 bits
+            half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8 + 2.0 ** -23
+            assert ((db.double() - want).abs() <= half * want.abs() + rows * 2.0 ** -52 * size).all()
+
+
+def test_small_norm_weight_gradient_keeps_its_bits():
+    """256 rows, each a partial row of its own. A term has four roundings (1 / root, two
+    products, the sum's at the end), each off by U32 / sqrt(3) in the mean at most, and the
+    terms' errors add up as the terms do: 2 U32 / sqrt(3), 6.9e-8."""
+    x, w, dy = randn(256, 2048, seed=1).requires_grad_(), (randn(2048, seed=2) * 0.3 + 1).requires_grad_(), randn(256, 2048, seed=3)
+    (dw,) = torch.autograd.grad(rms_norm(x, w), w, dy)
+    s = x.detach().double()
+    want = (dy.double() * s / (s.square().mean(1, keepdim=True) + 1e-6).sqrt()).sum(0)
+    assert relative(dw, want) <= 2 * U32 / 3 ** 0.5
