@@ -8,6 +8,7 @@ import torch
 from active_learning_amd.ops.extension import require_extension
 from active_learning_amd.ops.fp8 import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8
 from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
+from test_head_ops_gpu import _norm_64, _norm_inputs, half, product_within, same_blocks, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -436,3 +437,157 @@ def test_small_norm_weight_gradient_keeps_its_bits():
     s = x.detach().double()
     want = (dy.double() * s / (s.square().mean(1, keepdim=True) + 1e-6).sqrt()).sum(0)
     assert relative(dw, want) <= 2 * U32 / 3 ** 0.5
+
+
+# --------------------------------------------------------------------------- #
+# loops and indices that smaller inputs and even scales do not reach
+# --------------------------------------------------------------------------- #
+
+# more rows than a grid has blocks: each block walks over several, and sums its part of dw
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,dim", [(9001, 300), (9000, 1000), (3001, 2048), (2500, 4096), (2100, 8192), (2051, 12289), (1100, 20001)])
+def test_norm_of_more_rows_than_blocks(rows, dim, residual, dtype):
+    x, w, r = _norm_inputs(rows, dim, dtype, residual, torch.float32)
+    leaves = [t.requires_grad_() for t in (x, w, r) if t is not None]
+    out = rms_norm(x, w, residual=r)
+    y, total = out if residual else (out, x)
+    dy, ds = randn(rows, dim, dtype=dtype, seed=4), randn(rows, dim, dtype=dtype, seed=5)
+    grads = torch.autograd.grad((y, total) if residual else y, leaves, (dy, ds) if residual else dy)
+    with torch.no_grad():
+        s, root, want = _norm_64(x, w, r, 1e-6)
+        h, many = half(dtype), (dim / 1024 + 24) * U32
+        within(y, want, (h + 4 * U32) * want.abs() + tiny(dtype))
+        u, g = s / root, dy.double() * w.double()
+        dot = (g * u).mean(-1, keepdim=True)
+        dx = (g - u * dot) / root
+        size = (g.abs() + u.abs() * (g * u).abs().mean(-1, keepdim=True)) / root
+        if residual:
+            assert torch.equal(total.double(), s) and torch.equal(grads[2], grads[0])
+            dx, size = dx + ds.double(), size + ds.double().abs()
+        within(grads[0], dx, h * dx.abs() + 4 * many * size + tiny(dtype))
+        # a block's rows behind each other in 32 bits, at most one in 768 of them
+        dw, size = (dy.double() * u).sum(0), (dy.double() * u).abs().sum(0)
+        within(grads[1], dw, (rows / 768 + 6) * U32 * size)
+        assert relative(grads[1], dw) <= ((rows / 768) ** 0.5 + 2) * U32
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantise_more_tiles_than_blocks(dtype, kind):
+    """33 x 41 tiles: each block goes on to the next, loaded ahead."""
+    x = randn(33 * 128 - 3, 41 * 128 - 5, seed=1) * torch.exp2(randn(33 * 128 - 3, 1, seed=2) * 3)
+    x = (x * torch.exp2(randn(1, x.shape[1], seed=3) * 3)).to(dtype)
+    cpu = x.cpu()
+    same_blocks(quantize_fp8(x, tile=True, scale=kind), quantize_fp8(cpu, tile=True, scale=kind))
+    same_blocks(quantize_fp8(x.t(), scale=kind), quantize_fp8(cpu.t(), scale=kind))
+    both = require_extension().fp8_quant_tile(x, 0 if kind == "e8m0" else 1, False, True, True, torch.float32)
+    same_blocks(Fp8Blocks._of(both[0], both[1], x.shape, False), quantize_fp8(cpu, scale=kind))
+    same_blocks(Fp8Blocks._of(both[2], both[3], x.t().shape, False), quantize_fp8(cpu.t(), scale=kind))
+    want, size = x.double().sum(0), x.double().abs().sum(0)  # fp16 has infinities here
+    fine = torch.isfinite(size)
+    within(both[4][fine], want[fine], (U32 * want.abs() + len(x) * 2.0 ** -52 * size)[fine])
+    assert torch.equal(both[4][~fine].double().nan_to_num(5, 6, 7), want[~fine].nan_to_num(5, 6, 7))
+
+
+def _uneven(rows, cols, seed, tile):
+    """Normal values, each block times a power of two of its own: 2^-6 to 2^6."""
+    by = torch.randint(-6, 7, (-(-rows // 128) if tile else rows, -(-cols // 128)),
+                       generator=torch.Generator().manual_seed(seed)).cuda()
+    by = by.repeat_interleave(128, 1)[:, :cols]
+    return randn(rows, cols, seed=seed) * torch.exp2((by.repeat_interleave(128, 0)[:rows] if tile else by).float())
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m,n,k", SHAPES + [(70, 500, 4200), (300, 33000, 900), (5000, 4100, 1100), (4097, 4500, 256), (8000, 2300, 640)])
+def test_every_block_has_its_own_scale(m, n, k, kind):
+    x = _uneven(m, k, 1, False)
+    a = quantize_fp8(x, scale=kind)
+    av = a.dequantize()
+    for tile in (True, False):
+        b = quantize_fp8(_uneven(n, k, 2, tile), tile=tile, scale=kind)
+        bv = b.dequantize()
+        for out in (torch.bfloat16, torch.float32):
+            product_within(fp8_matmul(a, b, out_dtype=out), av, bv)
+    few = x[:9].bfloat16()
+    product_within(fp8_linear(few, b), quantize_fp8(few, scale=kind).dequantize(), bv)
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_not_finite_blocks_in_every_kernel(m, n, k, kind):
+    x, w = randn(m, k, seed=1), randn(n, k, seed=2)
+    x[m // 2, k - 1], x[m - 1, 3], w[n - 2, 200] = float("nan"), float("inf"), float("-inf")
+    a, clean = quantize_fp8(x, scale=kind), quantize_fp8(w.nan_to_num(0, 0, 0), scale=kind)
+    for out in (torch.bfloat16, torch.float32):
+        for tile in (True, False):
+            y = fp8_matmul(a, quantize_fp8(w, tile=tile, scale=kind), out_dtype=out)
+            nan = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+            nan[m // 2], nan[m - 1] = True, True
+            first, past = ((n - 2) // 128 * 128, (n - 2) // 128 * 128 + 128) if tile else (n - 2, n - 1)
+            nan[:, first:past] = True
+            assert torch.equal(torch.isnan(y), nan)
+        y = fp8_matmul(a, clean, out_dtype=out)
+        nan = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+        nan[m // 2], nan[m - 1] = True, True
+        assert torch.equal(torch.isnan(y), nan)
+
+
+@pytest.mark.parametrize("kind", ["e8m0", "fp32"])
+@pytest.mark.parametrize("m,n,k,dtype", [(8, 10, 512, torch.float32), (130, 257, 200, torch.bfloat16), (300, 129, 640, torch.float16),
+                                         (2100, 1500, 700, torch.bfloat16), (4200, 4352, 400, torch.float32)])
+def test_linear_gradients_with_both_kinds_of_scales(m, n, k, dtype, kind):
+    x, w = _uneven(m, k, 1, False).to(dtype).requires_grad_(), _uneven(n, k, 2, True).requires_grad_()
+    b = randn(n, seed=3).requires_grad_()
+    dy = (_uneven(m, n, 4, False) * 1e-3).to(dtype)
+    y = fp8_linear(x, w, b, scale=kind)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    back = lambda t, tile=False: quantize_fp8(t.detach().cpu(), tile=tile, scale=kind).dequantize().cuda()  # noqa: E731
+    wq = back(w, True)
+    if dtype != torch.float16:  # this one's results may leave its range
+        product_within(y, back(x), wq, b.detach())
+        product_within(dx, back(dy), wq.t().contiguous())
+    product_within(dw, back(dy.t()), back(x.t()))
+    want = dy.double().sum(0)
+    within(db, want, U32 * want.abs() + m * 2.0 ** -52 * dy.double().abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clip_more_chunks_than_blocks(dtype):
+    """Two tensors of more than 2048 chunks of 16384 values together."""
+    from active_learning_amd.ops.grad_clip import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=dtype)) for n in (20000003, 17000001)]
+    for i, p in enumerate(ps):
+        p.grad = randn(*p.shape, seed=i, dtype=dtype)
+    kept = [p.grad.double() for p in ps]
+    want = sum(k.square().sum().item() for k in kept) ** 0.5
+    norm = clip_grad_norm_(ps, 7.0).item()
+    assert abs(norm - want) <= 2 * U32 * want
+    for p, k in zip(ps, kept):
+        e = k * (7.0 / (want + 1e-6))
+        within(p.grad, e, (half(dtype) + 4 * U32) * e.abs() + tiny(dtype))
+
+
+def test_head_moves_alike_on_both_devices():
+    """Each parameter's way over three clipped steps. The devices' 32-bit sums differ by some
+    1e-6, which moves about one in 10^5 values over a border of e4m3, by 2^-3 of itself: 4e-4 of
+    a gradient, and again in each step that follows."""
+    from active_learning_amd.ops.fp8 import Fp8Linear
+    from active_learning_amd.ops.loss import cross_entropy
+    from active_learning_amd.ops.optim import FusedSGD
+    from active_learning_amd.ops.rmsnorm import RMSNorm
+    xs, y = [randn(256, 512, seed=s) for s in range(3)], torch.arange(256, device="cuda") % 10
+
+    def moves(device):
+        torch.manual_seed(0)
+        net = torch.nn.Sequential(RMSNorm(512), Fp8Linear(512, 10)).to(device)
+        opt = FusedSGD(net.parameters(), lr=0.1, momentum=0.9, max_grad_norm=0.5)
+        before = [p.detach().clone() for p in net.parameters()]
+        for x in xs:
+            opt.zero_grad()
+            cross_entropy(net(x.to(device)), y.to(device)).backward()
+            opt.step()
+        return [(p.detach() - b).cpu() for p, b in zip(net.parameters(), before)]
+
+    for a, b in zip(moves("cuda"), moves("cpu")):
+        assert b.norm() > 0 and relative(a, b.double()) <= 0.02
