@@ -8,7 +8,8 @@ hipGraph after a few eager warmup steps and replays it per batch, with:
 * static input/target buffers (H2D copy lands outside the graph);
 * the LR schedule routed through a device hyper buffer
   (FusedSGD.enable_device_hyper) so scheduler.step() never forces re-capture;
-* an eager fallback for odd-sized batches (the non-drop_last tail) and for
+* an eager fallback for odd-sized batches (the non-drop_last tail), for
+  optimizers without that buffer (Adam, several parameter groups) and for
   anything that fails capture — capture failure can never lose training;
 * post-replay cache upkeep: in-graph kernels update BN running stats and
   bf16 weight shadows in place without bumping the python-side version
@@ -112,6 +113,9 @@ class GraphedTrainStep:
             # captured step is allocation-free and the chunk table is stable
             optimizer.enable_persistent_grads()
             self._persistent = True
+        # a step whose state lives on the host (Adam's count, several groups' rates) or
+        # that does not zero its gradients would repeat itself in a replay: eager
+        self._failed = not self._persistent
 
     # ------------------------------------------------------------------ #
     def _dealias_grads(self):

@@ -283,3 +283,11 @@ def test_bias_gradient_is_rounded_once(rows, cols):
             # a 16-bit one through 32 bits
             half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8 + 2.0 ** -23
             assert ((db.double() - want).abs() <= half * want.abs() + rows * 2.0 ** -52 * size).all()
+
+
+def test_only_steps_that_a_replay_can_follow_are_captured():
+    from active_learning_amd.ops.graph import GraphedTrainStep
+    net = torch.nn.Linear(4, 3)
+    for opt in (build_optimizer("Adam", net.parameters(), max_grad_norm=0.5),
+                FusedSGD([{"params": [net.weight]}, {"params": [net.bias]}], lr=0.1)):
+        assert GraphedTrainStep(net, opt, torch.nn.CrossEntropyLoss(), torch.device("cuda"))._failed

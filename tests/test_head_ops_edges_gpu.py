@@ -591,3 +591,36 @@ def test_head_moves_alike_on_both_devices():
 
     for a, b in zip(moves("cuda"), moves("cpu")):
         assert b.norm() > 0 and relative(a, b.double()) <= 0.02
+
+
+@pytest.mark.parametrize("what", ["Adam", "groups"])
+def test_trainer_with_steps_that_are_not_captured(what):
+    """Adam and SGD with two groups, clipped, through the trainer's step: as step by step."""
+    from active_learning_amd.ops.fp8 import Fp8Linear
+    from active_learning_amd.ops.graph import GraphedTrainStep
+    from active_learning_amd.ops.loss import CrossEntropyLoss
+    from active_learning_amd.ops.optim import FusedAdam, FusedSGD
+    from active_learning_amd.ops.rmsnorm import RMSNorm
+    dev = torch.device("cuda", torch.cuda.current_device())
+    crit, y = CrossEntropyLoss().to(dev), torch.arange(64, device="cuda") % 10
+
+    def run(through_trainer):
+        torch.manual_seed(1)
+        net = torch.nn.Sequential(RMSNorm(512), Fp8Linear(512, 10)).cuda()
+        if what == "Adam":
+            opt = FusedAdam(net.parameters(), lr=0.01, max_grad_norm=0.5)
+        else:
+            opt = FusedSGD([{"params": net[0].parameters(), "lr": 0.3}, {"params": net[1].parameters()}],
+                           lr=0.1, momentum=0.9, max_grad_norm=0.5)
+        step = GraphedTrainStep(net, opt, crit, dev, warmup=2)
+        for i in range(6):
+            x = randn(64, 512, seed=i)
+            if through_trainer:
+                step.step(x, y)
+            else:
+                opt.zero_grad()
+                crit(net(x), y).backward()
+                opt.step()
+        return [p.detach().clone() for p in net.parameters()]
+
+    assert all(torch.equal(a, b) for a, b in zip(run(True), run(False)))
