@@ -114,7 +114,8 @@ const Tensor& value(const OptTensor& t) { return *t; }
 void check_norm(const Tensor& x, const Tensor& w, const OptTensor& res, double eps) {
   type_of(x, "input");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "the norm needs a last axis of at least one value");
-  TORCH_CHECK_VALUE(x.size(-1) <= INT_MAX - kBlock, "the last axis is too long");
+  // a row's places are counted in 32 bits, up to a whole sweep of a workgroup behind its end
+  TORCH_CHECK_VALUE(x.size(-1) <= 1 << 30, "the last axis is too long: ", x.size(-1), " values, at most 2^30");
   TORCH_CHECK_VALUE(w.dim() == 1 && w.size(0) == x.size(-1), "weight has shape ", w.sizes(), ", not [",
                     x.size(-1), "]");
   TORCH_CHECK_TYPE(w.scalar_type() == torch::kFloat32 || w.scalar_type() == x.scalar_type(),
@@ -415,6 +416,7 @@ Tensor fp8_few_rows(const Tensor& x, const Tensor& b, const Tensor& sb, bool b_t
   c10::OptionalDeviceGuard guard(x.device());
   Tensor out = fresh({m, n}, x.scalar_type(), x);
   TORCH_CHECK_VALUE(k > 0, "x needs a last axis of at least one value");
+  TORCH_CHECK_VALUE(n < 1 << 29, "a weight of ", n, " rows is too large");  // 2^32 threads
   if (!m || !n) return out;
   al_fp8_few_rows(kind_of(sb), type, x.data_ptr(), row_stride(x), (int)k, b.data_ptr(), sb.data_ptr(),
                   b.size(1), (int)sb.size(1), b_tile, (int)m, (int)n, (int)blocks_of(k),

@@ -624,3 +624,13 @@ def test_trainer_with_steps_that_are_not_captured(what):
         return [p.detach().clone() for p in net.parameters()]
 
     assert all(torch.equal(a, b) for a, b in zip(run(True), run(False)))
+
+
+def test_rows_too_long_for_32_bits_are_refused():
+    """Views of one value: nothing is read."""
+    one = torch.ones(1, device="cuda", dtype=torch.bfloat16)
+    for dim in (2 ** 30 + 1, 2 ** 31 - 129, 2 ** 31 - 128, 2 ** 31 + 5):
+        x = one.expand(1, dim)
+        for f in (rms_norm, rms_norm_fp8):
+            with pytest.raises(ValueError, match="too long"):
+                f(x, x[0])
