@@ -32,6 +32,39 @@ def _distinct(tensors):
     return kept
 
 
+def _dense(t):
+    """Whether the values fill their memory, in any order."""
+    size = 1
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim()) if t.shape[i] != 1):
+        if stride != size:
+            return False
+        size *= n
+    return True
+
+
+def _scale(grads, factor):
+    """Scales gradients on the CPU in place."""
+    spans, copies = [], []
+    for g in grads:
+        if not g.numel():
+            continue
+        if any(n > 1 and s == 0 for n, s in zip(g.shape, g.stride())):
+            raise RuntimeError("a gradient whose values share memory cannot be scaled in place")
+        if _dense(g):
+            spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()))
+        else:  # may be part of another one
+            copies.append((g, g * factor))
+    spans.sort()
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise RuntimeError("gradients that share memory cannot be scaled in place")
+    apart = {id(g) for g, _ in copies}
+    for g in grads:
+        if id(g) not in apart:
+            g.mul_(factor)
+    for g, scaled in copies:
+        g.copy_(scaled)
+
+
 def _norm_factor(grads, max_norm):
     """Norm and factor of gradients on the CPU."""
     norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
@@ -70,7 +103,9 @@ def clip_grad_norm_(parameters, max_norm):
 
     A NaN makes all gradients NaN; an infinity makes the factor zero, so that it
     becomes NaN itself and everything else zero; an infinite ``max_norm`` leaves
-    everything as it is. Gradients that share memory are refused.
+    everything as it is. Gradients that share memory, and a gradient whose own values
+    do (an expanded one), are refused; one that is a sparse part of another's memory
+    is scaled once.
     """
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm = float(max_norm)
@@ -83,11 +118,5 @@ def clip_grad_norm_(parameters, max_norm):
         if both.is_cuda:
             require_extension().scale_grads(parameters, both)
         else:
-            grads = _distinct(p.grad for p in parameters)
-            spans = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size())
-                           for g in grads if g.is_contiguous() and g.numel())
-            if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
-                raise RuntimeError("gradients that share memory cannot be scaled in place")
-            for g in grads:
-                g.mul_(both[1])
+            _scale(_distinct(p.grad for p in parameters), both[1])
     return both[0]

@@ -5,6 +5,7 @@
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -616,6 +617,8 @@ void scale_grads(const std::vector<Tensor>& params, const Tensor& norm_factor) {
   const std::vector<Tensor> grads = grads_of(params);
   for (const Tensor& g : grads) {
     TORCH_CHECK(g.is_cuda() && g.device() == norm_factor.device(), "gradients must be on one GPU");
+    TORCH_CHECK(at::has_internal_overlap(g) != at::MemOverlap::Yes,
+                "a gradient whose values share memory cannot be scaled in place");
     Tensor at = g;
     if (!dense(g)) {
       copies.emplace_back(g, g.contiguous());

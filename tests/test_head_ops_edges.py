@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from active_learning_amd.ops.fp8 import fp8_linear, quantize_fp8
+from active_learning_amd.ops.grad_clip import clip_grad_norm_
 from active_learning_amd.ops.optim import FusedSGD, build_optimizer
 from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
 
@@ -291,3 +292,27 @@ def test_only_steps_that_a_replay_can_follow_are_captured():
     for opt in (build_optimizer("Adam", net.parameters(), max_grad_norm=0.5),
                 FusedSGD([{"params": [net.weight]}, {"params": [net.bias]}], lr=0.1)):
         assert GraphedTrainStep(net, opt, torch.nn.CrossEntropyLoss(), torch.device("cuda"))._failed
+
+
+def test_clip_scales_shared_memory_once_or_refuses():
+    base = torch.arange(1.0, 13.0, device="cpu")
+
+    def clip(*grads):
+        ps = [torch.nn.Parameter(torch.zeros(g.shape, device="cpu")) for g in grads]
+        for p, g in zip(ps, grads):
+            p.grad = g
+        return clip_grad_norm_(ps, 1.0)
+
+    keep, square = base.clone(), base.view(3, 4)
+    for shared in ((square, square.t()), (torch.ones(1, device="cpu").expand(5),),
+                   (base, torch.ones(2, 1, device="cpu").expand(2, 4)), (base[:8], base[4:])):
+        before = [g.clone() for g in shared]
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip(*shared)
+        assert all(torch.equal(g, b) for g, b in zip(shared, before))
+    # every second value is there twice: it counts twice in the norm, and is scaled once
+    norm = (keep.double().square().sum() + keep[::2].double().square().sum()).sqrt().item()
+    assert abs(clip(base, base[::2]).item() - norm) <= 2 * 2.0 ** -24 * norm
+    assert ((base.double() - keep.double() / (norm + 1e-6)).abs() <= 4 * 2.0 ** -24 * base.double()).all()
+    empty = torch.empty(3, 0, device="cpu")
+    assert clip(empty, empty.t()).item() == 0.0

@@ -7,6 +7,7 @@ import torch
 
 from active_learning_amd.ops.extension import require_extension
 from active_learning_amd.ops.fp8 import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8
+from active_learning_amd.ops.grad_clip import clip_grad_norm_
 from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
 from test_head_ops_gpu import _norm_64, _norm_inputs, half, product_within, same_blocks, tiny, within
 
@@ -555,7 +556,6 @@ def test_linear_gradients_with_both_kinds_of_scales(m, n, k, dtype, kind):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_clip_more_chunks_than_blocks(dtype):
     """Two tensors of more than 2048 chunks of 16384 values together."""
-    from active_learning_amd.ops.grad_clip import clip_grad_norm_
     ps = [torch.nn.Parameter(torch.zeros(n, device="cuda", dtype=dtype)) for n in (20000003, 17000001)]
     for i, p in enumerate(ps):
         p.grad = randn(*p.shape, seed=i, dtype=dtype)
@@ -634,3 +634,27 @@ def test_rows_too_long_for_32_bits_are_refused():
         for f in (rms_norm, rms_norm_fp8):
             with pytest.raises(ValueError, match="too long"):
                 f(x, x[0])
+
+
+def test_clip_scales_shared_memory_once_or_refuses():
+    base = torch.arange(1.0, 13.0, device="cuda")
+
+    def clip(*grads):
+        ps = [torch.nn.Parameter(torch.zeros(g.shape, device="cuda")) for g in grads]
+        for p, g in zip(ps, grads):
+            p.grad = g
+        return clip_grad_norm_(ps, 1.0)
+
+    keep, square = base.clone(), base.view(3, 4)
+    for shared in ((square, square.t()), (torch.ones(1, device="cuda").expand(5),),
+                   (base, torch.ones(2, 1, device="cuda").expand(2, 4)), (base[:8], base[4:])):
+        before = [g.clone() for g in shared]
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip(*shared)
+        assert all(torch.equal(g, b) for g, b in zip(shared, before))
+    # every second value is there twice: it counts twice in the norm, and is scaled once
+    norm = (keep.double().square().sum() + keep[::2].double().square().sum()).sqrt().item()
+    assert abs(clip(base, base[::2]).item() - norm) <= 2 * 2.0 ** -24 * norm
+    assert ((base.double() - keep.double() / (norm + 1e-6)).abs() <= 4 * 2.0 ** -24 * base.double()).all()
+    empty = torch.empty(3, 0, device="cuda")
+    assert clip(empty, empty.t()).item() == 0.0
