@@ -211,7 +211,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                 g = p.grad
                 state = self.state[p]
                 if momentum != 0 and "momentum_buffer" not in state:
-                    state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+                    state["momentum_buffer"] = self._new_buffer(p)
                 buf = state.get("momentum_buffer")
                 if p.is_cuda and ext is not None and p.is_contiguous():
                     cache = getattr(p, "_al_cast", None)
@@ -249,6 +249,14 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
                 self._multi_tensor_step(ext, gi, fused, lr, momentum, wd, clip)
         return loss
 
+    @staticmethod
+    def _new_buffer(p):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            # each replay would fill it with zeros again
+            raise RuntimeError("a step without its momentum buffers cannot be captured: take one "
+                               "before")
+        return torch.zeros_like(p, dtype=torch.float32)
+
     def _sgd_step(self, ext, p, g, buf, lr, momentum, wd, shadow, clip):
         if buf is None:
             buf = p.new_empty(0)
@@ -269,7 +277,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         if momentum != 0:
             for p in params:
                 if "momentum_buffer" not in state[p]:
-                    state[p]["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+                    state[p]["momentum_buffer"] = self._new_buffer(p)
         bufs = [state[p].get("momentum_buffer") for p in params]
         shadows = []
         for p in params:

@@ -658,3 +658,25 @@ def test_clip_scales_shared_memory_once_or_refuses():
     assert ((base.double() - keep.double() / (norm + 1e-6)).abs() <= 4 * 2.0 ** -24 * base.double()).all()
     empty = torch.empty(3, 0, device="cuda")
     assert clip(empty, empty.t()).item() == 0.0
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_first_step_with_momentum_is_not_captured(strided):
+    from active_learning_amd.ops.optim import FusedSGD
+    p = torch.nn.Parameter(randn(30, 40, seed=1))
+    p.grad = randn(40, 30, seed=2).t() if strided else randn(30, 40, seed=2)
+    opt = FusedSGD([p], lr=0.1, momentum=0.9)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    torch.cuda.synchronize()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    # 1, 1.9, 2.71, 3.439 times the gradient: sums of five roundings a step
+    want = randn(30, 40, seed=1).double() - 0.1 * (1 + 1.9 + 2.71 + 3.439) * p.grad.double()
+    assert ((p.double() - want).abs() <= 4 * 5 * U32 * 8).all()
