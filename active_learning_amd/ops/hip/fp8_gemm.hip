@@ -65,43 +65,38 @@ AL_DEV bf16x8v to_bf16(int lo, int hi, float scale) {
   return bf16x8v{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// A block's scales leave the range of a float when they are multiplied with each other,
-// where the result does not (both operands around 1e-19: 2^-140 times sums around 2^17).
-// So each is a power of two, which the matrix instruction or the conversion in front of
-// it applies, times the factor that is left; factors may be multiplied.
+// Both scales of a block, multiplied with each other, leave the range of a float where the
+// result does not (operands around 1e-19: 2^-140 times sums around 2^17). So the left one
+// is a power of two, which the matrix instruction or the conversion in front of it
+// applies, times a factor of 1 to 2, and only the factor is multiplied with the right one.
+// Powers are 2^-60 to 2^103: a block's sum, of 2^-18 to 2^25 where it is not zero, stays
+// normal, and where the factor takes over beyond them its product leaves the range only
+// with a result that does.
 struct Scale {
   unsigned code;  // of the power of two, 2^(code - 127)
   float factor;
 };
-AL_DEV Scale split_at(unsigned bits, int least, int most) {
-  const int e = (int)(bits >> 23 & 255u);
-  const int code = e < least ? least : e > most ? most : e;
-  return {(unsigned)code, __builtin_ldexpf(__uint_as_float(bits), 127 - code)};
+AL_DEV Scale split(float scale) {
+  const int e = (int)(__float_as_uint(scale) >> 23 & 255u);
+  const int code = e < 127 - 60 ? 127 - 60 : e > 127 + 103 ? 127 + 103 : e;
+  return {(unsigned)code, __builtin_ldexpf(scale, 127 - code)};
 }
-// For the 8-bit instruction, which holds any power: factors of 1 to 2 (less below the
-// normal range; an infinity or a NaN keeps itself).
-AL_DEV Scale hw_scale(unsigned bits) { return split_at(bits, 1, 254); }
-// For bf16, whose values, products and sums have to stay normal: powers of 2^-50 to
-// 2^110. Smaller factors than 1 on both sides belong to results that are zero.
-template <int KIND> AL_DEV Scale bf16_scale(unsigned code) {
-  const unsigned bits = KIND == kF32 ? code : code == 255u ? 0x7fc00000u : code ? code << 23 : 0x400000u;
-  return split_at(bits, 127 - 50, 127 + 110);
-}
-template <int KIND, bool EXACT> AL_DEV Scale scale_of_code(unsigned code) {
-  if constexpr (EXACT) return bf16_scale<KIND>(code);
-  else return hw_scale(code);
+template <int KIND> AL_DEV float scale_value(unsigned code) {
+  return __uint_as_float(KIND == kF32 ? code : code == 255u ? 0x7fc00000u : code ? code << 23 : 0x400000u);
 }
 
-// one block's 16x16 products times the scales' powers of two; EXACT: in bf16 instructions
-template <bool EXACT> AL_DEV f32x4 block_product(i32x8 x, i32x8 y, unsigned sx, unsigned sy) {
+constexpr int kOne = 127;  // the power 2^0
+
+// one block's 16x16 products times y's power of two; EXACT: in bf16 instructions
+template <bool EXACT> AL_DEV f32x4 block_product(i32x8 x, i32x8 y, unsigned power) {
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  if (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, zero, 0, 0, 0, (int)sx, 0, (int)sy);
-  const float px = __uint_as_float(sx << 23), py = __uint_as_float(sy << 23);
+  if (!EXACT) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, zero, 0, 0, 0, kOne, 0, (int)power);
+  const float by = __uint_as_float(power << 23);
   f32x4 d = zero;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(x[2 * i], x[2 * i + 1], px),
-                                                to_bf16(y[2 * i], y[2 * i + 1], py), d, 0, 0, 0);
+    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(x[2 * i], x[2 * i + 1], 1.f),
+                                                to_bf16(y[2 * i], y[2 * i + 1], by), d, 0, 0, 0);
   return d;
 }
 
@@ -216,11 +211,10 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       f32x4 by;
-      Scale sb;
       if (!HW) {
-        sb = scale_of_code<KIND, EXACT>(r.sb[j]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) by[e] = BTILE ? sb.factor : __shfl(sb.factor, l4 * 4 + e, 64);
+        for (int e = 0; e < 4; ++e)
+          by[e] = scale_value<KIND>(BTILE ? r.sb[j] : (unsigned)__shfl((int)r.sb[j], l4 * 4 + e, 64));
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
@@ -229,8 +223,8 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(r.b[j], fa, acc[i][j], 0, 0, 0,
                                                                       (int)r.sb[j], 0, (int)r.sa[i]);
         } else {
-          const Scale s = scale_of_code<KIND, EXACT>(r.sa[i]);
-          const f32x4 d = block_product<EXACT>(r.b[j], fa, sb.code, s.code);
+          const Scale s = split(scale_value<KIND>(r.sa[i]));
+          const f32x4 d = block_product<EXACT>(r.b[j], fa, s.code);
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s.factor * by[e], acc[i][j][e]);
         }
@@ -340,7 +334,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   constexpr int SB = KIND == kE8M0 ? 4 : 16;  // bytes of four steps' scales
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = wid >> 2, wc = wid & 3, l31 = lane & 31;
+  const int wr = wid >> 2, wc = wid & 3, l31 = lane & 31, l5 = lane >> 5;
   int tm, tn;
   tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * 256, n0 = tn * 256;
@@ -419,17 +413,12 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
   const unsigned lds = (unsigned)(unsigned long)(__attribute__((address_space(3))) unsigned char*)smem;
 
   i32x8 fa[2][2], fb[2][2];
-  int sa[2], sb[2];  // this step's scales, or their powers of two, in the lowest byte
-  float ga[2], gb[2];  // 32-bit scales: the factors left
+  int sa[2], sb[2];  // e8m0: this step's scales, in the lowest byte; else a's powers and b's bits
+  float ga[2];       // 32-bit scales: a's factors
   // where the scales of step k (the s-th of its four) are
   auto scale_of = [&](int row, int k, int s) __attribute__((always_inline)) {
     const unsigned char* p = smem + kRingS + ((k >> 2 & 1) * 512 + row) * SB;
     return KIND == kF32 ? ((const int*)p)[s] : (int)(*(const unsigned*)p >> (8 * s));
-  };
-  auto split = [](int& scale, float& factor) __attribute__((always_inline)) {
-    const Scale s = hw_scale((unsigned)scale);
-    scale = (int)s.code;
-    factor = s.factor;
   };
   auto read_a = [&](int k, int s, int h, int ring) __attribute__((always_inline)) {
     const int l = this_lane(), l31 = l & 31;
@@ -439,7 +428,11 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
       fa[i][0] = fragment(p + i * 32 * 128, 0);
       fa[i][1] = fragment(p + i * 32 * 128, 1);
       sa[i] = scale_of(h * 128 + wr * 64 + i * 32 + l31, k, s);
-      if (KIND == kF32) split(sa[i], ga[i]);
+      if (KIND == kF32) {
+        const Scale x = split(__int_as_float(sa[i]));
+        sa[i] = (int)x.code;
+        ga[i] = x.factor;
+      }
     }
   };
   auto read_b = [&](int k, int s) __attribute__((always_inline)) {
@@ -449,8 +442,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
     for (int j = 0; j < 2; ++j) {
       fb[j][0] = fragment(p + j * 32 * 128, 0);
       fb[j][1] = fragment(p + j * 32 * 128, 1);
-      sb[j] = scale_of(256 + wc * 64 + j * 32 + l31, k, s);
-      if (KIND == kF32) split(sb[j], gb[j]);
+      if (KIND == kE8M0 || BTILE) sb[j] = scale_of(256 + wc * 64 + j * 32 + l31, k, s);
     }
   };
   auto multiply = [&](int k, int s, f32x16 (&c)[2][2]) __attribute__((always_inline)) {
@@ -491,16 +483,14 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
           d = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[t >> 1][half], fa[t & 1][half], d, 0, 0, 0,
-                                                              sb[t >> 1], 0, sa[t & 1]);
+                                                              kOne, 0, sa[t & 1]);
       };
       auto add = [&](f32x16& d, int t) __attribute__((always_inline)) {
         const int i = t & 1, j = t >> 1;
-        const int four = (this_lane() >> 5) * 16;  // the lane that has the first row's factor, in bytes
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float by = BTILE ? gb[j] : __int_as_float(__builtin_amdgcn_ds_bpermute(
-                                               four + ((r >> 2) * 8 + (r & 3)) * 4, __float_as_int(gb[j])));
-          c[i][j][r] = fmaf(d[r], ga[i] * by, c[i][j][r]);
+          const int by = BTILE ? sb[j] : scale_of(256 + wc * 64 + j * 32 + (r >> 2) * 8 + l5 * 4 + (r & 3), k, s);
+          c[i][j][r] = fmaf(d[r], ga[i] * __int_as_float(by), c[i][j][r]);
         }
       };
       start(d[0], 0);
@@ -660,8 +650,10 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 // the cycles and the vector units, which convert, in 35%: waves that meet at a barrier each
 // step do both at the same times. Fragments read a step ahead, 16 waves of 32x64 and four
 // of 64x128 took 119, 128 and 141 us.
+// Two stages fit twice: no more registers than let both workgroups run (130 instead of 128
+// with 32-bit scales by row: 8192x1000x2048 34.6 us, 30.1 this way).
 template <int KIND, bool EXACT, bool BTILE, int TM, int TN, int WM, int WN, int STAGES>
-__launch_bounds__(WM * WN * 64)
+__launch_bounds__(WM * WN * 64, STAGES == 2 ? 4 : 1)
 __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
   constexpr bool HW = KIND == kE8M0 && !EXACT;
   constexpr int WAVES = WM * WN, MT = TM / WM / 16, NT = TN / WN / 16;
@@ -742,13 +734,13 @@ __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
     };
     i32x8 fa[MT], fb[NT];
     unsigned sa[MT];
-    float xa[MT];  // 32-bit scales: the factors left
+    float xa[MT];  // 32-bit scales: the factors beside the powers
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       fa[i] = fragment(wm + i * 16);
       sa[i] = scale_of(wm + i * 16 + l15);
       if (KIND == kF32) {
-        const Scale s = scale_of_code<KIND, EXACT>(sa[i]);
+        const Scale s = split(__uint_as_float(sa[i]));
         sa[i] = s.code;
         xa[i] = s.factor;
       }
@@ -773,13 +765,12 @@ __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
           }
         }
       } else {
-        const Scale sb = scale_of_code<KIND, EXACT>(scale_of(TM + wn + j * 16 + l15));
         f32x4 by;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) by[e] = BTILE ? sb.factor : __shfl(sb.factor, l4 * 4 + e, 64);
+        for (int e = 0; e < 4; ++e) by[e] = __uint_as_float(scale_of(TM + wn + j * 16 + (BTILE ? 0 : l4 * 4 + e)));
         f32x4 d[MT];  // all before the first is used: 2500x2500x8192 77 us, one by one 81
 #pragma unroll
-        for (int i = 0; i < MT; ++i) d[i] = block_product<EXACT>(fb[j], fa[i], sb.code, sa[i]);
+        for (int i = 0; i < MT; ++i) d[i] = block_product<EXACT>(fb[j], fa[i], sa[i]);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
