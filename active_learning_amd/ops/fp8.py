@@ -50,7 +50,8 @@ class Fp8Blocks:
     Kernels read whole blocks and four scales at a time, so the storage is padded
     (zero behind the last column). The constructor copies into that layout what
     does not have it already: build it once and keep it, as a program keeps its
-    weights.
+    weights. quantize_fp8 and rms_norm_fp8 write it themselves. Values times scales
+    have to lie in float32's range.
     """
 
     __slots__ = ("_codes", "_scales", "shape", "tile")
@@ -239,8 +240,8 @@ def fp8_matmul(a, b, bias=None, out_dtype=torch.bfloat16):
 
     Sums are held in 32 bits. Products for a bfloat16 or float16 result are added
     by the 8-bit matrix instruction, which is a few 1e-5 off; for a float32 result
-    they are computed by bf16 instructions, exactly, at half the rate. Not
-    differentiable.
+    they are computed by bf16 instructions, exactly (with e8m0 scales of values
+    under 2^-126 what bf16 holds), at half the rate. Not differentiable.
     """
     if not isinstance(a, Fp8Blocks) or not isinstance(b, Fp8Blocks):
         raise TypeError("fp8_matmul takes two Fp8Blocks")
@@ -316,8 +317,13 @@ def fp8_linear(x, weight, bias=None, scale="e8m0"):
     ``x``: (..., in) in bfloat16, float16 or float32; the result has its type.
     ``weight``: Fp8Blocks (out, in), to serve with a weight that is kept
     quantised (``scale`` is then the weight's own), or a tensor (out, in), which
-    is quantised by 128x128 tiles in every call and is differentiable, as are x
-    and bias: both of the gradients' products are e4m3 products too.
+    is quantised by 128x128 tiles in every call and is differentiable once, as are
+    x and bias: both of the gradients' products are e4m3 products too.
+
+    Products for a bfloat16 or float16 result (y and dx in x's type, dw in the
+    weight's) are added by the 8-bit matrix instruction, which is a few 1e-5 off;
+    float32 ones by bf16 instructions, exactly, as in fp8_matmul. The bias' gradient
+    is summed in 64 bits. Forward-mode differentiation is refused.
     """
     kept = isinstance(weight, Fp8Blocks)
     if x.is_cuda:  # checked, and differentiated, by the extension

@@ -2,11 +2,12 @@
 
     norm = sqrt(sum over all tensors of g^2),   factor = min(1, max_norm / (norm + 1e-6))
 
-Squares are summed in 64 bits in a fixed order: the norm is exact to its 32-bit
-rounding, has the range of a float, and does not change from run to run. GPU
-tensors run optim.hip; nothing here waits for the device. The optimizers of
-ops/optim.py clip inside their step (``max_grad_norm``), without the pass over
-the gradients that clip_grad_norm_ writes.
+Gradients are bfloat16, float16 or float32; others are refused. Squares are summed
+in 64 bits in a fixed order: the norm is exact to its 32-bit rounding, has the
+range of a float, and does not change from run to run. GPU tensors run optim.hip;
+nothing here waits for the device. The optimizers of ops/optim.py clip inside
+their step (``max_grad_norm``), without the pass over the gradients that
+clip_grad_norm_ writes.
 """
 
 import torch

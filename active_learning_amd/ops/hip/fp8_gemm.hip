@@ -115,7 +115,7 @@ template <int KIND> AL_DEV unsigned scale_code(const void* p, long at) {
 // a launch less, and b's bytes are what it costs. With T unsigned char they come
 // as codes.
 //
-// 1x1000x2048 with values takes 4.6 us, a launch; 16x8192x8192 21 us for 67 MB of b, which a
+// 1x1000x2048 with values takes 5.1 us, a launch; 16x8192x8192 21 us for 67 MB of b, which a
 // copy moves in 12.5, and 16x16384x8192 31.5 us (24.9): each unit takes 25 KB a microsecond of
 // x and b together, with 16 waves (21), three blocks in flight a wave (24) and blocks in an
 // order of each workgroup's own (22) too.
@@ -280,12 +280,13 @@ __global__ void direct_kernel(const T* __restrict__ x, long x_stride, int dim, G
 //
 // With e8m0 scales the matrix instruction applies them, or, in the EXACT form (bf16
 // instructions), the conversion to bf16. 32-bit scales multiply each block's sum as
-// it is added to the total.
+// it is added to the total, but for the left one's power of two.
 //
-// 8192x8192x8192: e8m0 376 to 395 us, 2.8 to 2.9 PFLOP/s, the matrix cores busy in 79% of
-// the cycles and the clock at 1.66 GHz, which power leaves; 32-bit scales 460 us, where the
-// scaling takes as many vector cycles as the products take matrix cycles; EXACT 737 us,
-// 1.49 PFLOP/s. LDS conflicts: 1 cycle in 150.
+// 8192x8192x8192: e8m0 384 to 407 us, 2.7 to 2.86 PFLOP/s, the matrix cores busy in 79% of
+// the cycles and the clock at 1.66 GHz, which power leaves; 32-bit scales 484 to 501 us, where
+// the scaling takes as many vector cycles as the products take matrix cycles (780 where the
+// right one's scales differ from row to row and come from LDS for each value); EXACT 751 us,
+// 1.46 PFLOP/s. LDS conflicts: 1 cycle in 150.
 
 constexpr int kHalf = 128 * 128;       // bytes of half a tile: 128 rows of a block
 constexpr int kRingB = 5 * kHalf;      // where b's ring begins
@@ -475,7 +476,7 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
         }
     } else {
       // three tiles' products ahead of their scaling, as many as registers hold: one ahead
-      // 472 us where this takes 460
+      // takes 12 us more of 8192x8192x8192
       f32x16 d[3];
       auto start = [&](f32x16& d, int t) __attribute__((always_inline)) {
 #pragma unroll
@@ -645,8 +646,8 @@ __global__ void gemm256_kernel(Gemm g, int tiles_m, int tiles_n) {
 // for anew. The order of the 16-byte chunks within a block is the same on both
 // sides: a lane has chunks l4 and l4 + 4 of its row.
 //
-// 2048x2048x8192 takes 44 us, and for 32-bit results 73; 4096x2048x8192 for 32-bit results
-// 118 (a bf16 product at the library's rate: 97). There the matrix cores are busy in 44% of
+// 2048x2048x8192 takes 44 us, and for 32-bit results 72; 4096x2048x8192 for 32-bit results
+// 117 (a bf16 product at the library's rate: 97). There the matrix cores are busy in 44% of
 // the cycles and the vector units, which convert, in 35%: waves that meet at a barrier each
 // step do both at the same times. Fragments read a step ahead, 16 waves of 32x64 and four
 // of 64x128 took 119, 128 and 141 us.
@@ -768,7 +769,7 @@ __global__ void gemm_mid_kernel(Gemm g, int tiles_m, int tiles_n) {
         f32x4 by;
 #pragma unroll
         for (int e = 0; e < 4; ++e) by[e] = __uint_as_float(scale_of(TM + wn + j * 16 + (BTILE ? 0 : l4 * 4 + e)));
-        f32x4 d[MT];  // all before the first is used: 2500x2500x8192 77 us, one by one 81
+        f32x4 d[MT];  // all before the first is used: 2500x2500x8192 80 us, one by one 4 more
 #pragma unroll
         for (int i = 0; i < MT; ++i) d[i] = block_product<EXACT>(fb[j], fa[i], sa[i]);
 #pragma unroll
@@ -832,10 +833,10 @@ template <typename F> void with_kind(int kind, F f) {
 //   64x64 while each unit has two: 1024x1000x2048 9.7 against 16 of 32x32 and 13 of
 //     128x128; 512x4096x4096 19 against 24;
 //   128x128 in four stages while each has one, in two (which fit twice) while each has
-//     two and tiles are short: 2048x2048x8192 47 against 54 of 256x256, 8192x1000x2048
-//     23 against 25, but 3000x3000x5120 76 against 50;
-//   128x256 while each has one, for 32-bit results, 4096x2048x8192 121 against 139, and
-//     for 32-bit scales, 2500x2500x8192 77 against 96 (with e8m0 256x256 is as fast: 70
+//     two and tiles are short: 2048x2048x8192 44 against 54 of 256x256, 8192x1000x2048
+//     23 against 25, but 3000x3000x5120 76 against 48;
+//   128x256 while each has one, for 32-bit results, 4096x2048x8192 117 against 139, and
+//     for 32-bit scales, 2500x2500x8192 80 against 96 (with e8m0 256x256 is as fast: 70
 //     and 67); and wherever both have 32 bits, for which 256x256 has no registers;
 //   256x256 for the rest: 8192x8192x8192 386 against 575 of 128x128.
 enum Tile { kDirect32, kMid64, kMid128Deep, kMid128, kMid128x256, kBig };
@@ -854,8 +855,8 @@ static Tile tile_for(int kind, int out_type, int m, int n, int blocks) {
 // How many columns 256x256 tiles take where their last round on the 256 units would be
 // the shorter part of one: whole rounds, if smaller tiles compute the rest in less than
 // the round that it saves (a half with 128x128, three quarters with 128x256), and a
-// round is long enough for another launch. 4096x4452x4096 87 us in one launch, 71 in
-// two; 8192x4608x8192 252 and 235; with 32-bit scales 114 and 84, 330 and 289.
+// round is long enough for another launch. 4096x4452x4096 89 us in one launch, 76 in
+// two; 8192x4608x8192 258 and 248; with 32-bit scales 117 and 89, 340 and 308.
 static int columns_of_rounds(int kind, int out_type, int m, int n, int blocks) {
   const int down = (m + 255) / 256, rounds = (int)((long)down * ((n + 255) / 256) / 256);
   const int columns = rounds * 256 / down * 256;

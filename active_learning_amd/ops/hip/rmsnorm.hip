@@ -7,8 +7,8 @@
 //   dw = sum over rows of dy * u
 //
 // The norm is that of the stored, rounded sum: the backward pass reads the same
-// numbers and differentiates what the forward pass computed. Arithmetic is in 32
-// bits or more, rounded to the type on the store.
+// numbers and differentiates what the forward pass computed. Squares, and dw over its
+// partial rows, are summed in 64 bits, the rest is in 32, rounded to the type on the store.
 
 #include "al_fp8.h"
 
@@ -38,13 +38,14 @@ constexpr int block_of(int tpr) { return tpr < 256 ? 256 : tpr; }
 //
 // Squares are summed in 64 bits: those of values over 1.8e19 leave the range of 32, and a
 // row of finite values would become zeros. (Where the root is over 2^126, 1 / root is below
-// the normal range and has 21 bits.)
+// the normal range and has 21 bits.) 16383x4096 in bf16 with a residual, traced: 93 us,
+// with 32 bits 88.
 //
-// In front of an e4m3 output 1 / root and the first
-// product are held as pairs of floats: y is then the exact value rounded once, and a value next
-// to a border between two codes or scales falls on its own side of it (with 32 bits throughout,
-// 50 codes in 123 million did not). At 130000x2048 in bf16 with a residual that costs
-// 355 us against 336, at 5.3 and 5.5 TB/s; the reductions go through lane permutations
+// In front of an e4m3 output 1 / root and the first product are held as pairs of floats: y
+// is then the exact value rounded once, and a value next to a border between two codes or
+// scales falls on its own side of it (with 32 bits throughout, 50 codes in 123 million did
+// not). At 130000x2048 in bf16 with a residual that and the sum cost 355 us against 336, at
+// 5.3 and 5.5 TB/s; the reductions go through lane permutations
 // of the vector unit (LDS shuffles: 187 us for 160 without a residual).
 //
 // One vector a thread: no more registers than let eight waves share a SIMD, as the
@@ -274,12 +275,13 @@ struct Shape { int tpr, vpt; };
 
 // The forward pass. Up to 1024 values a wave holds a row and needs no barrier, longer
 // rows are spread with one vector a thread, up to 32768 with a few: beyond that a row is
-// read twice. Measured on 266 million values in bf16, us with the residual / without:
-//   1024 values, plain:  64 threads x 2 vectors 462 / 189, x 4 (half of them idle, fewer
-//                        waves at once) 396 / 211; to e4m3, x 2, 355 / 183
-//   2048 values:         64 x 4 plain 384 / 206, to e4m3 411; 256 x 1 388 / 192, 355 / 160
-//   4096 values, plain:  256 x 2 460 / 191, 512 x 1 393 / 192
-//   8192 values, e4m3:   256 x 4 403 / 167, 1024 x 1 346 / 171; plain 388 / 209, 391 / 185
+// read twice. Measured on 266 million values in bf16, us with the residual / without (of
+// the plain form's shapes those that are not taken with sums in 32 bits):
+//   1024 values, plain:  64 threads x 2 vectors 462 / 190, x 4 (half of them idle, fewer
+//                        waves at once) 404 / 211; to e4m3, x 2, 355 / 165
+//   2048 values:         64 x 4 plain 384 / 206, to e4m3 411; 256 x 1 389 / 192, 356 / 166
+//   4096 values, plain:  256 x 2 460 / 191, 512 x 1 399 / 193
+//   8192 values, e4m3:   256 x 4 403 / 167, 1024 x 1 340 / 179; plain 388 / 209, 387 / 185
 // (their bytes at a copy's rate: plain 396 / 198, e4m3 346 / 148). The rule does not ask
 // for the number of rows, so a row's numbers do not depend on the rows beside it.
 Shape fwd_shape(int dim, bool res, int out) {

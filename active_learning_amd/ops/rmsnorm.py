@@ -92,7 +92,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 
     ``x``: (..., dim) in bfloat16, float16 or float32; ``residual``: the same
     shape and type; ``weight``: (dim,) in float32 or x's type. Returns y, or
-    (y, sum) where a residual is given. Differentiable in all three.
+    (y, sum) where a residual is given. Differentiable in all three, once, and not in
+    forward mode.
     """
     if x.is_cuda:  # checked, and differentiated, by the extension
         out = require_extension().rms_norm(x, weight, residual, eps)
