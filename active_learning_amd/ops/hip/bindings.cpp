@@ -484,9 +484,18 @@ Tensor ce_bwd(const Tensor& probs, const Tensor& targets, const Tensor& scale) {
   return dl;
 }
 
+// the kernels read and write a parameter's state value for value
+void check_like(const Tensor& p, const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == torch::kFloat32 && t.numel() == p.numel() &&
+                        t.is_contiguous() && t.device() == p.device(),
+                    name, " must be a dense float32 tensor like its parameter");
+}
+
 void sgd_step(Tensor& p, const Tensor& g, Tensor& buf, double lr, double momentum,
               double wd, const Tensor& shadow) {
   TORCH_CHECK(p.is_cuda() && p.scalar_type() == torch::kFloat32);
+  TORCH_CHECK_VALUE(g.numel() == p.numel() && g.device() == p.device(), "gradient");
+  if (buf.numel()) check_like(p, buf, "momentum_buffer");
   void* sh = nullptr;
   if (shadow.numel()) {
     TORCH_CHECK(shadow.numel() == p.numel() &&
@@ -530,6 +539,9 @@ void wt_refresh_multi(const Tensor& table, int64_t nrows) {
 void adam_step(Tensor& p, const Tensor& g, Tensor& m, Tensor& v, double lr, double b1,
                double b2, double eps, double wd, double bc1, double bc2) {
   TORCH_CHECK(p.is_cuda() && p.scalar_type() == torch::kFloat32);
+  TORCH_CHECK_VALUE(g.numel() == p.numel() && g.device() == p.device(), "gradient");
+  check_like(p, m, "exp_avg");
+  check_like(p, v, "exp_avg_sq");
   al_adam_step(p.data_ptr<float>(), g.contiguous().data_ptr<float>(),
                m.data_ptr<float>(), v.data_ptr<float>(), (float)lr, (float)b1,
                (float)b2, (float)eps, (float)wd, (float)bc1, (float)bc2, p.numel(),

@@ -650,6 +650,13 @@ bool sgd_fusable(const std::vector<Tensor>& params) {
   return true;
 }
 
+// what an update reads and writes beside a parameter, value for value
+void check_state(const Tensor& p, const Tensor& t, const char* name, torch::ScalarType type = torch::kFloat32) {
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.is_contiguous() && t.numel() == p.numel() && t.device() == p.device(),
+                    name, " must be a dense ", type, " tensor like its parameter: ", t.sizes(), " ", t.scalar_type(),
+                    " on ", t.device(), ", the parameter is ", p.sizes(), " on ", p.device());
+}
+
 // five words a parameter: the addresses of its values, gradient, momentum and bf16
 // copy (0: none), and its length
 py::bytes sgd_addresses(const std::vector<Tensor>& params, const std::vector<OptTensor>& bufs,
@@ -658,6 +665,8 @@ py::bytes sgd_addresses(const std::vector<Tensor>& params, const std::vector<Opt
   std::vector<int64_t> words;
   words.reserve(params.size() * 5);
   for (size_t i = 0; i < params.size(); ++i) {
+    if (bufs[i]) check_state(params[i], *bufs[i], "momentum_buffer");
+    if (shadows[i]) check_state(params[i], *shadows[i], "the bf16 copy", torch::kBFloat16);
     words.push_back((int64_t)params[i].data_ptr());
     words.push_back((int64_t)params[i].grad().data_ptr());
     words.push_back(bufs[i] ? (int64_t)bufs[i]->data_ptr() : 0);
@@ -698,6 +707,8 @@ void sgd_step_clip(Tensor& p, const Tensor& g, Tensor& buf, double lr, double mo
                    const OptTensor& hyper, Tensor& shadow, const Tensor& norm_factor) {
   check_update(p, g, "SGD step");
   if (!p.numel()) return;
+  if (buf.numel()) check_state(p, buf, "momentum_buffer");
+  if (shadow.numel()) check_state(p, shadow, "the bf16 copy", torch::kBFloat16);
   c10::OptionalDeviceGuard guard(p.device());
   al_sgd_step_clip(p.data_ptr<float>(), g.data_ptr<float>(), buf.numel() ? buf.data_ptr<float>() : nullptr,
                    (float)lr, buf.numel() ? (float)momentum : 0.f, (float)wd, hyper_of(hyper), p.numel(),
@@ -709,6 +720,8 @@ void adam_step_clip(Tensor& p, const Tensor& g, Tensor& m, Tensor& v, double lr,
                     double eps, double wd, double bc1, double bc2, const Tensor& norm_factor) {
   check_update(p, g, "Adam step");
   if (!p.numel()) return;
+  check_state(p, m, "exp_avg");
+  check_state(p, v, "exp_avg_sq");
   c10::OptionalDeviceGuard guard(p.device());
   al_adam_step_clip(p.data_ptr<float>(), g.data_ptr<float>(), m.data_ptr<float>(), v.data_ptr<float>(),
                     (float)lr, (float)b1, (float)b2, (float)eps, (float)wd, (float)bc1, (float)bc2, p.numel(),

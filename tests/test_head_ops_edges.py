@@ -316,3 +316,16 @@ def test_clip_scales_shared_memory_once_or_refuses():
     assert ((base.double() - keep.double() / (norm + 1e-6)).abs() <= 4 * 2.0 ** -24 * base.double()).all()
     empty = torch.empty(3, 0, device="cpu")
     assert clip(empty, empty.t()).item() == 0.0
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(11), torch.zeros(12, dtype=torch.float64), torch.zeros(3, 4).t(), torch.zeros(12).expand(2, 12)[:, ::2]])
+def test_momentum_that_does_not_fit_is_refused(bad):
+    """The table of the multi-tensor step takes addresses only of what fits its parameter."""
+    from active_learning_amd.ops.extension import load_extension
+    ext, p = load_extension(), torch.nn.Parameter(torch.zeros(3, 4))
+    p.grad = torch.zeros(3, 4)
+    assert len(ext.sgd_addresses([p], [torch.zeros(12)], [None])) == 40
+    with pytest.raises(ValueError, match="momentum_buffer"):
+        ext.sgd_addresses([p], [bad], [None])
+    with pytest.raises(ValueError, match="bf16"):
+        ext.sgd_addresses([p], [None], [bad])

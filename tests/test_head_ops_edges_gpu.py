@@ -680,3 +680,22 @@ def test_first_step_with_momentum_is_not_captured(strided):
     # 1, 1.9, 2.71, 3.439 times the gradient: sums of five roundings a step
     want = randn(30, 40, seed=1).double() - 0.1 * (1 + 1.9 + 2.71 + 3.439) * p.grad.double()
     assert ((p.double() - want).abs() <= 4 * 5 * U32 * 8).all()
+
+
+@pytest.mark.parametrize("bound", [None, 1.0])
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("name,key", [("SGD", "momentum_buffer"), ("Adam", "exp_avg"), ("Adam", "exp_avg_sq")])
+def test_state_that_does_not_fit_is_refused(name, key, strided, bound):
+    from active_learning_amd.ops.optim import build_optimizer
+    p = torch.nn.Parameter(randn(30, 40, seed=1))
+    p.grad = randn(40, 30, seed=2).t() if strided else randn(30, 40, seed=2)
+    args = {"momentum": 0.9} if name == "SGD" else {}
+    opt = build_optimizer(name, [p], lr=0.1, max_grad_norm=bound, **args)
+    opt.step()
+    keep = p.detach().clone()
+    for bad in (torch.zeros(1199, device="cuda"), torch.zeros(30, 40), torch.zeros(40, 30, device="cuda").t(),
+                torch.zeros(30, 40, device="cuda", dtype=torch.bfloat16)):
+        opt.state[p][key] = bad
+        with pytest.raises(ValueError, match=key):
+            opt.step()
+    assert torch.equal(p, keep)
