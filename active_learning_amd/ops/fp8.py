@@ -135,13 +135,13 @@ class Fp8Blocks:
 def _quantize_cpu(x, kind, tile):
     rows, cols = x.shape
     up, across = (_blocks(rows) * BLOCK if tile else rows), _blocks(cols) * BLOCK
-    wide = torch.zeros(up, across)
+    wide = torch.zeros(up, across, dtype=torch.float32)
     wide[:rows, :cols] = x
     tall = BLOCK if tile else 1
     grid = wide.view(up // tall, tall, across // BLOCK, BLOCK)
     amax = grid.abs().amax((1, 3))  # NaN stays
     bad = ~torch.isfinite(amax)
-    amax = torch.where(bad, torch.ones(()), amax).clamp_min(_AMAX_FLOOR)
+    amax = torch.where(bad, amax.new_ones(()), amax).clamp_min(_AMAX_FLOOR)
     if kind == 0:
         code = ((amax.view(torch.int32) + 0x1FFFFF) >> 23) - 8
         inverse = ((254 - code) << 23).view(torch.float32)
@@ -149,8 +149,8 @@ def _quantize_cpu(x, kind, tile):
     else:
         # a tensor over a tensor: a number over one is rounded twice
         inverse = torch.full_like(amax, FP8_MAX) / amax
-        scale = torch.where(bad, torch.tensor(float("nan")), amax / FP8_MAX)
-    inverse = torch.where(bad, torch.tensor(float("nan")), inverse)
+        scale = torch.where(bad, amax.new_tensor(float("nan")), amax / FP8_MAX)
+    inverse = torch.where(bad, amax.new_tensor(float("nan")), inverse)
     scaled = (grid * inverse[:, None, :, None]).reshape(up, across)[:rows, :cols]
     values = scaled.clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
     if cols == 0:  # the transpose of no rows

@@ -92,7 +92,7 @@ def grad_norm(tensors):
         tensors = [tensors]
     tensors = [t for t in tensors if t is not None]
     if not tensors:
-        return torch.zeros(())
+        return torch.zeros((), dtype=torch.float32)
     if tensors[0].is_cuda:
         return require_extension().grad_norm_factor(tensors, float("inf"), None)[0]
     return _norm_factor(_distinct(tensors), float("inf"))[0]
@@ -114,7 +114,7 @@ def clip_grad_norm_(parameters, max_norm):
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     both = _params_norm_factor(parameters, max_norm)
     if both is None:
-        return torch.zeros(())
+        return torch.zeros((), dtype=torch.float32)
     with torch.no_grad():
         if both.is_cuda:
             require_extension().scale_grads(parameters, both)

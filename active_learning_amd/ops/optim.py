@@ -35,6 +35,10 @@ def _check_max_norm(max_grad_norm):
     return max_grad_norm
 
 
+def _stream_capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
 class _Clips:
     """The bound of an optimizer that clips, checked whenever it is set."""
 
@@ -107,8 +111,8 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
             # otherwise a step that was captured before goes on to follow
             self._hyper_host = None
             self._hyper_dev = torch.zeros(3, dtype=torch.float32, device=device)
-            self._clip_dev = torch.full((1,), float("inf"), device=device)
-            self._clip_to = torch.zeros(2, device=device)
+            self._clip_dev = torch.full((1,), float("inf"), dtype=torch.float32, device=device)
+            self._clip_to = torch.zeros(2, dtype=torch.float32, device=device)
             self._clip_host = None
         self.sync_hyper()
 
@@ -137,7 +141,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         self._left_out.setdefault(owner, set()).add(what)
 
     def _capturing(self):
-        return self._hyper_dev is not None and torch.cuda.is_current_stream_capturing()
+        return self._hyper_dev is not None and _stream_capturing()
 
     def sync_hyper(self):
         g = self.param_groups[0]
@@ -251,7 +255,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
 
     @staticmethod
     def _new_buffer(p):
-        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+        if p.is_cuda and _stream_capturing():
             # each replay would fill it with zeros again
             raise RuntimeError("a step without its momentum buffers cannot be captured: take one "
                                "before")
@@ -289,7 +293,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         # shadow's (0: none), and its length
         fp = ext.sgd_addresses(params, bufs, shadows)
         entry = self._mt_cache.get(gi)
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _stream_capturing()
         if entry is None or entry[0] != fp:
             if capturing:
                 # a table rebuild needs host allocations, which invalidate
@@ -365,7 +369,7 @@ class FusedSGD(_Clips, torch.optim.Optimizer):
         K, C % 64). Table cached by pointer fingerprint like the sgd chunk
         table, so steady-state (and captured) steps launch with no H2D."""
         entry = self._wt_cache.get(gi)
-        capturing = torch.cuda.is_current_stream_capturing()
+        capturing = _stream_capturing()
         if entry is None or entry[0] != fp:
             if capturing:
                 for shadow in shadows:

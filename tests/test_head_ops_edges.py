@@ -19,9 +19,10 @@ def _params(sizes):
 
 @pytest.fixture
 def capturing(monkeypatch):
-    """A switch that makes torch say that the stream is being captured."""
+    """A switch that makes the optimizer see a stream that is being captured."""
+    from active_learning_amd.ops import optim
     state = {"on": False}
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["on"])
+    monkeypatch.setattr(optim, "_stream_capturing", lambda: state["on"])
     return lambda on: state.update(on=on)
 
 
@@ -329,3 +330,31 @@ def test_momentum_that_does_not_fit_is_refused(bad):
         ext.sgd_addresses([p], [bad], [None])
     with pytest.raises(ValueError, match="bf16"):
         ext.sgd_addresses([p], [None], [bad])
+
+
+def test_default_type_of_64_bits():
+    """What torch makes by default has no say in types that are fixed."""
+    x, w = torch.randn(20, 300, device="cpu"), torch.randn(40, 300, device="cpu")
+    norm_weight = torch.rand(300, device="cpu")
+    x[3, 7] = float("nan")
+
+    def run():
+        out = []
+        for kind in ("e8m0", "fp32"):
+            q = rms_norm_fp8(x, norm_weight, scale=kind)
+            out += [q.values.float(), q.scale.float(), fp8_linear(x, quantize_fp8(w, tile=True, scale=kind))]
+        p = torch.nn.Parameter(x[:2].clone())
+        p.grad = x[4:6].clone()
+        opt = FusedSGD([p], lr=0.5, momentum=0.9, max_grad_norm=0.5)
+        opt.enable_device_hyper("cpu")
+        opt.step()
+        return [*out, rms_norm(x, norm_weight), p.detach(), opt.last_grad_norm, clip_grad_norm_([], 1.0)]
+
+    want = run()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    for g, v in zip(got, want):
+        assert g.dtype == v.dtype == torch.float32 and torch.equal(g.nan_to_num(9), v.nan_to_num(9))

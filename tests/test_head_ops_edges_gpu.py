@@ -8,6 +8,7 @@ import torch
 from active_learning_amd.ops.extension import require_extension
 from active_learning_amd.ops.fp8 import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8
 from active_learning_amd.ops.grad_clip import clip_grad_norm_
+from active_learning_amd.ops.optim import FusedSGD
 from active_learning_amd.ops.rmsnorm import rms_norm, rms_norm_fp8
 from test_head_ops_gpu import _norm_64, _norm_inputs, half, product_within, same_blocks, tiny, within
 
@@ -49,7 +50,6 @@ def test_bound_of_the_step_that_is_captured(before, at):
     from active_learning_amd.ops.fp8 import Fp8Linear
     from active_learning_amd.ops.graph import GraphedTrainStep
     from active_learning_amd.ops.loss import CrossEntropyLoss
-    from active_learning_amd.ops.optim import FusedSGD
     from active_learning_amd.ops.rmsnorm import RMSNorm
     dev = torch.device("cuda", torch.cuda.current_device())
     xs = [randn(64, 512, seed=s) for s in range(8)]
@@ -85,7 +85,6 @@ def test_norms_that_are_kept():
     from active_learning_amd.ops.graph import GraphedTrainStep
     from active_learning_amd.ops.linear import NativeLinear
     from active_learning_amd.ops.loss import CrossEntropyLoss
-    from active_learning_amd.ops.optim import FusedSGD
     dev = torch.device("cuda", torch.cuda.current_device())
     net = NativeLinear(512, 10).cuda()
     opt = FusedSGD(net.parameters(), lr=0.1, max_grad_norm=0.5)
@@ -101,7 +100,6 @@ def test_norms_that_are_kept():
 
 @pytest.mark.parametrize("bound", [None, 0.5])
 def test_steps_with_new_gradients_take_no_more_memory(bound):
-    from active_learning_amd.ops.optim import FusedSGD
     sizes = [100003, 7, 40000]
     ps = [torch.nn.Parameter(randn(n, seed=i)) for i, n in enumerate(sizes)]
     opt = FusedSGD(ps, lr=0.1, momentum=0.9, max_grad_norm=bound)
@@ -127,7 +125,6 @@ def test_steps_with_new_gradients_take_no_more_memory(bound):
 
 def test_captured_step_keeps_its_addresses():
     """Steps with other gradients, eager, do not change what a captured step reads."""
-    from active_learning_amd.ops.optim import FusedSGD
     ps = [torch.nn.Parameter(randn(n, seed=n)) for n in (70000, 33)]
     opt = FusedSGD(ps, lr=0.5, max_grad_norm=1e6)
     mine = [randn(*p.shape, seed=1) for p in ps]
@@ -164,7 +161,6 @@ def test_captured_step_keeps_its_addresses():
 def test_step_over_nothing(bound):
     """Parameters of no values launch nothing, and leave no error for the next call."""
     from active_learning_amd.ops.grad_clip import grad_norm
-    from active_learning_amd.ops.optim import FusedSGD
     p = torch.nn.Parameter(torch.empty(0, 3, device="cuda"))
     p.grad = torch.empty(0, 3, device="cuda")
     opt = FusedSGD([p], lr=0.1, momentum=0.9, max_grad_norm=bound)
@@ -209,7 +205,6 @@ def test_parameters_of_any_strides(name, bound, layout):
 def test_persistent_gradients_are_used_once():
     """In persistent-gradient mode the step zeroes every gradient, also one whose strides
     take it through the per-tensor kernel."""
-    from active_learning_amd.ops.optim import FusedSGD
     p = torch.nn.Parameter(randn(30, 40, seed=1))
     p.grad = randn(40, 30, seed=2).t()
     opt = FusedSGD([p], lr=0.1)
@@ -574,7 +569,6 @@ def test_head_moves_alike_on_both_devices():
     a gradient, and again in each step that follows."""
     from active_learning_amd.ops.fp8 import Fp8Linear
     from active_learning_amd.ops.loss import cross_entropy
-    from active_learning_amd.ops.optim import FusedSGD
     from active_learning_amd.ops.rmsnorm import RMSNorm
     xs, y = [randn(256, 512, seed=s) for s in range(3)], torch.arange(256, device="cuda") % 10
 
@@ -662,7 +656,6 @@ def test_clip_scales_shared_memory_once_or_refuses():
 
 @pytest.mark.parametrize("strided", [False, True])
 def test_first_step_with_momentum_is_not_captured(strided):
-    from active_learning_amd.ops.optim import FusedSGD
     p = torch.nn.Parameter(randn(30, 40, seed=1))
     p.grad = randn(40, 30, seed=2).t() if strided else randn(30, 40, seed=2)
     opt = FusedSGD([p], lr=0.1, momentum=0.9)
@@ -699,3 +692,31 @@ def test_state_that_does_not_fit_is_refused(name, key, strided, bound):
         with pytest.raises(ValueError, match=key):
             opt.step()
     assert torch.equal(p, keep)
+
+
+def test_default_type_of_64_bits():
+    """What torch makes by default has no say in types that are fixed."""
+    x, w = torch.randn(20, 300, device="cuda"), torch.randn(40, 300, device="cuda")
+    norm_weight = torch.rand(300, device="cuda")
+    x[3, 7] = float("nan")
+
+    def run():
+        out = []
+        for kind in ("e8m0", "fp32"):
+            q = rms_norm_fp8(x, norm_weight, scale=kind)
+            out += [q.values.float(), q.scale.float(), fp8_linear(x, quantize_fp8(w, tile=True, scale=kind))]
+        p = torch.nn.Parameter(x[:2].clone())
+        p.grad = x[4:6].clone()
+        opt = FusedSGD([p], lr=0.5, momentum=0.9, max_grad_norm=0.5)
+        opt.enable_device_hyper("cuda")
+        opt.step()
+        return [*out, rms_norm(x, norm_weight), p.detach(), opt.last_grad_norm, clip_grad_norm_([], 1.0)]
+
+    want = run()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    for g, v in zip(got, want):
+        assert g.dtype == v.dtype == torch.float32 and torch.equal(g.nan_to_num(9), v.nan_to_num(9))
